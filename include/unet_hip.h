@@ -191,6 +191,43 @@ int unet_batch_norm_relu_backward_f32(const float *grad_activations, const float
                                       float *grad_weights, int num_channels, int H, int W, int batch_size,
                                       unet_stream_t stream);
 
+/* ---- layer norm ----------------------------------------------------------- */
+/* Layer norm over the channels of each row of a [rows][channels] matrix (a token of a transformer block, a pixel
+ * of an NHWC image); no counterpart in the reference, next to its batch norm.  Row strides (`*_ld`) are in
+ * elements and at least `channels`, so a matrix may be a column slice of a wider buffer; any alignment of the
+ * element type will do.  weights are interleaved [gamma0,beta0,gamma1,beta1,...] like the batch norm's and fp32
+ * for both storage types; NULL = gamma 1, beta 0.
+ *   mean = sum_c x / C, rstd = 1 / sqrt(sum_c (x - mean)^2 / C + eps)
+ *   activations = gamma * (x - mean) * rstd + beta
+ * row_stats (may be NULL: inference) receives [mean, rstd] per row for the backward.  Statistics are fp32 from two
+ * passes over the values; one rounding to the storage type at the end.  activations may be the inputs' own buffer
+ * (same pointer, same stride).  rows = 0 is a valid empty call. */
+int unet_layer_norm_f32(const float *inputs, int64_t in_ld, float *activations, int64_t out_ld, const float *weights,
+                        float *row_stats, int64_t rows, int channels, float eps, unet_stream_t stream);
+int unet_layer_norm_bf16(const uint16_t *inputs, int64_t in_ld, uint16_t *activations, int64_t out_ld,
+                         const float *weights, float *row_stats, int64_t rows, int channels, float eps,
+                         unet_stream_t stream);
+/* With xhat = (x - mean) * rstd and g = gamma * grad_activations:
+ *   grad_inputs = rstd * (g - mean_c g - xhat * mean_c (g * xhat)) (+ grad_skip)
+ *   grad_weights[2c] = sum_rows grad_activations * xhat, grad_weights[2c+1] = sum_rows grad_activations
+ * grad_skip (may be NULL; skip_ld is then ignored) is the gradient that reaches the inputs around the layer norm
+ * (the residual connection), added before the one rounding.  grad_inputs may be the buffer of grad_activations, of
+ * grad_skip or of inputs (same pointer, same stride).  grad_weights (fp32, overwritten) or grad_inputs may be NULL to skip
+ * that half.  weights NULL = gamma 1.  Sums over rows have a fixed order: equal calls give equal bits.
+ * `workspace` is device memory of at least unet_layer_norm_backward_workspace_bytes() bytes, 16-byte aligned, free
+ * for other use once the call's work on `stream` has finished; it may be NULL when grad_weights is.  The calls
+ * allocate nothing and can be captured into a graph. */
+int unet_layer_norm_backward_workspace_bytes(int64_t rows, int channels, size_t *bytes_host);
+int unet_layer_norm_backward_f32(const float *grad_activations, int64_t grad_ld, const float *inputs, int64_t in_ld,
+                                 const float *row_stats, const float *weights, const float *grad_skip, int64_t skip_ld,
+                                 float *grad_inputs, int64_t grad_in_ld, float *grad_weights, int64_t rows, int channels,
+                                 void *workspace, size_t workspace_bytes, unet_stream_t stream);
+int unet_layer_norm_backward_bf16(const uint16_t *grad_activations, int64_t grad_ld, const uint16_t *inputs,
+                                  int64_t in_ld, const float *row_stats, const float *weights,
+                                  const uint16_t *grad_skip, int64_t skip_ld, uint16_t *grad_inputs, int64_t grad_in_ld,
+                                  float *grad_weights, int64_t rows, int channels, void *workspace,
+                                  size_t workspace_bytes, unet_stream_t stream);
+
 /* ---- activations (cuda_lib.h:90-98, 151-161) ---------------------------- */
 
 int unet_relu_f32(const float *inputs, float *activations, int64_t num_activations, unet_stream_t stream);
@@ -212,6 +249,35 @@ int unet_leaky_relu_backward_f32(const float *grad_activations, const float *inp
 int unet_tanh_f32(const float *inputs, float *activations, int64_t num_activations, unet_stream_t stream);
 int unet_tanh_backward_f32(const float *grad_activations, const float *activations, float *grad_inputs,
                            int64_t num_activations, unet_stream_t stream);
+
+/* ---- dropout ---------------------------------------------------------------- */
+/* activations = residual + (kept(e) ? inputs / (1 - p) : 0) on a [rows][channels] matrix (no counterpart in the
+ * reference).  Which elements are kept is a function of (seed, offset, e) alone, e = row * channels + channel, so no
+ * mask is stored, strides and storage type do not matter, and the backward asks the same question again:
+ *   - Philox4x32-10 (Salmon, Moraes, Dror, Shaw 2011) with key (seed low, seed high) and counter
+ *     (b low, b high + 2^31 * f, o low, o high), b = e / 8, o = offset (+ *offset_device), gives four words per f; the
+ *     16-bit number of element e is (word[j / 2] >> 16 * (j % 2)) % 2^16, j = e % 8;
+ *   - u(e) = 2^16 * (number for f = 0) + (number for f = 1); kept iff u(e) >= round(p * 2^32).
+ * 0 <= p <= 1; at p = 1 nothing is kept.  A dropped element contributes exactly 0, also where the input is not finite.
+ * Calls that shall draw independent masks use different offsets (or seeds).  offset_device (may be NULL) is a 64-bit number in
+ * device memory, read when the kernel runs and added to `offset`: a captured graph draws a new mask per replay when
+ * something between replays changes it.  Row strides (`*_ld`) in elements, at least `channels`; any alignment of
+ * the element type.  residual may be NULL (residual_ld is then ignored).  activations may be the buffer of inputs or
+ * of residual (same pointer, same stride).  The sum is taken in fp32 and rounded once. */
+int unet_dropout_f32(const float *inputs, int64_t in_ld, const float *residual, int64_t residual_ld, float *activations,
+                     int64_t out_ld, int64_t rows, int channels, double p, uint64_t seed, uint64_t offset,
+                     const uint64_t *offset_device, unet_stream_t stream);
+int unet_dropout_bf16(const uint16_t *inputs, int64_t in_ld, const uint16_t *residual, int64_t residual_ld,
+                      uint16_t *activations, int64_t out_ld, int64_t rows, int channels, double p, uint64_t seed,
+                      uint64_t offset, const uint64_t *offset_device, unet_stream_t stream);
+/* grad_inputs = kept(e) ? grad_activations / (1 - p) : 0 with the p, seed and offset of the forward call (the
+ * residual's gradient is grad_activations itself).  grad_inputs may be the buffer of grad_activations. */
+int unet_dropout_backward_f32(const float *grad_activations, int64_t grad_ld, float *grad_inputs, int64_t grad_in_ld,
+                              int64_t rows, int channels, double p, uint64_t seed, uint64_t offset,
+                              const uint64_t *offset_device, unet_stream_t stream);
+int unet_dropout_backward_bf16(const uint16_t *grad_activations, int64_t grad_ld, uint16_t *grad_inputs,
+                               int64_t grad_in_ld, int64_t rows, int channels, double p, uint64_t seed, uint64_t offset,
+                               const uint64_t *offset_device, unet_stream_t stream);
 
 /* ---- max pool (cuda_lib.h:69-77, 202-211) -------------------------------- */
 
@@ -283,6 +349,60 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
                                  uint16_t *dg, int dg_ld, int dg_accumulate, float *grad_weights,
                                  int batch_size, int H_x, int W_x, int channels_in_x, int channels_in_g,
                                  int int_channels, unet_stream_t stream);
+
+/* ---- dot-product attention over sequences ---------------------------------- */
+/* softmax(scale * Q K^T) V for a batch of sequences packed one behind the other (no counterpart in the reference,
+ * whose only attention is the additive gate above).
+ *   q, out [total_q][heads_q * head_dim], k, v [total_k][heads_kv * head_dim], head h in columns
+ *   [h*head_dim, (h+1)*head_dim); `*_ld` = token stride in elements (q, k and v may be column slices of one
+ *   projection's output); any alignment of the element type.  heads_q is a multiple of heads_kv: query head h
+ *   reads key/value head h / (heads_q / heads_kv).
+ *   cu_q, cu_k (device, int32, num_seqs + 1 values, not decreasing): sequence s has the queries
+ *   [cu_q[s], cu_q[s+1]) and the keys [cu_k[s], cu_k[s+1]); lengths may differ and may be zero.
+ *   causal != 0: query i of a sequence sees the keys j <= i + (keys - queries), i.e. the last query sees all.
+ *   lse [total_q][heads_q] (fp32, may be NULL: inference) = log sum_j exp(scale * q.k_j), for the backward.
+ * A query that sees no key gets out = 0 and lse = -inf, and adds nothing to any gradient.  What a query does not see
+ * does not reach it, whatever it holds (NaN and infinities included).  Rows of out and lse in front of the first or behind
+ * the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
+ * accumulators are fp32; the bf16 form rounds the softmax weights to bf16 for their product with V.  Equal calls
+ * give equal bits.  out must not overlap q, k or v.
+ * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
+ * do), 16-byte aligned, free for other use once the call's work on `stream` has finished.  The calls allocate
+ * nothing and can be captured into a graph. */
+int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv,
+                                       int head_dim, size_t *bytes_host);
+int unet_dot_attention_f32(const float *q, int64_t q_ld, const float *k, int64_t k_ld, const float *v, int64_t v_ld,
+                           float *out, int64_t out_ld, float *lse, const int32_t *cu_q, const int32_t *cu_k,
+                           int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv, int head_dim,
+                           float scale, int causal, void *workspace, size_t workspace_bytes, unet_stream_t stream);
+int unet_dot_attention_bf16(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t k_ld, const uint16_t *v,
+                            int64_t v_ld, uint16_t *out, int64_t out_ld, float *lse, const int32_t *cu_q,
+                            const int32_t *cu_k, int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
+                            int heads_kv, int head_dim, float scale, int causal, void *workspace,
+                            size_t workspace_bytes, unet_stream_t stream);
+/* Gradients of the above from grad_out and the forward's out and lse: with P the softmax weights,
+ * dP = grad_out V^T and dS = P * (dP - sum_d grad_out * out):
+ *   grad_v = P^T grad_out, grad_q = scale * dS K, grad_k = scale * dS^T Q, all overwritten; grad_k and grad_v sum over the query heads that
+ * share a key/value head.  The bf16 form rounds P and dS to bf16 for their products.  No atomics: every sum has a
+ * fixed order.  Rows outside the sequences are left as they were; keys that no query sees get 0.  The gradients must not
+ * overlap the inputs or each other's columns (they may be column slices of one buffer). */
+int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
+                                                int heads_kv, int head_dim, size_t *bytes_host);
+int unet_dot_attention_backward_f32(const float *grad_out, int64_t grad_out_ld, const float *q, int64_t q_ld,
+                                    const float *k, int64_t k_ld, const float *v, int64_t v_ld, const float *out,
+                                    int64_t out_ld, const float *lse, float *grad_q, int64_t grad_q_ld, float *grad_k,
+                                    int64_t grad_k_ld, float *grad_v, int64_t grad_v_ld, const int32_t *cu_q,
+                                    const int32_t *cu_k, int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
+                                    int heads_kv, int head_dim, float scale, int causal, void *workspace,
+                                    size_t workspace_bytes, unet_stream_t stream);
+int unet_dot_attention_backward_bf16(const uint16_t *grad_out, int64_t grad_out_ld, const uint16_t *q, int64_t q_ld,
+                                     const uint16_t *k, int64_t k_ld, const uint16_t *v, int64_t v_ld,
+                                     const uint16_t *out, int64_t out_ld, const float *lse, uint16_t *grad_q,
+                                     int64_t grad_q_ld, uint16_t *grad_k, int64_t grad_k_ld, uint16_t *grad_v,
+                                     int64_t grad_v_ld, const int32_t *cu_q, const int32_t *cu_k, int num_seqs,
+                                     int64_t total_q, int64_t total_k, int heads_q, int heads_kv, int head_dim,
+                                     float scale, int causal, void *workspace, size_t workspace_bytes,
+                                     unet_stream_t stream);
 
 /* ---- upsample = transposed conv, kernel = stride = scale ---------------- */
 /* (cuda_lib.h:79-88, 213-224) */

@@ -19,6 +19,7 @@ LIB_PATH = os.path.join(_ROOT, "unet_amd", "lib", "libunet_hip.so")
 _SCALARS = {
     "int": ctypes.c_int,
     "float": ctypes.c_float,
+    "double": ctypes.c_double,
     "int64_t": ctypes.c_int64,
     "uint64_t": ctypes.c_uint64,
     "size_t": ctypes.c_size_t,

@@ -1,0 +1,807 @@
+// Dot-product attention over packed sequences, forward and backward (fp32 and bf16 storage).
+//
+//   S = scale Q K^T,  P = softmax over the visible keys,  out = P V,  lse = log sum exp S
+//   delta = sum_d dout * out,  dP = dout V^T,  dS = P * (dP - delta)
+//   dV = P^T dout,  dQ = scale dS K,  dK = scale dS^T Q
+//
+// Three kernels of one shape.  A wavefront keeps 32 "columns" in registers as matrix-core B operands (queries in the
+// forward and in the dQ kernel, keys in the dK/dV kernel) and streams "rows" (keys, or queries) through LDS in
+// tiles that the workgroup shares.  Scores are computed transposed, rows x columns, so that
+//   - a column's scores lie in one lane (and in the lane 32 further): maxima, sums, masks and rescaling need no
+//     exchange inside the loop;
+//   - the 32x32 result layout (lane: column l % 32; rows 8 * (i / 4) + 4 * (l / 32) + i % 4, i < 16) is, 16 rows at a time,
+//     a B operand again for the second product acc[d][column] += X^T[d][rows] W[rows][column], if the A operand takes its
+//     rows in the same order: the softmax weights never leave the registers.
+// Query heads that share a key/value head are packed into the row axis of that head: row r of a sequence is query
+// r / G, head r % G of the group.  One tile of keys and values serves all of them, and the sums of dK and dV over the
+// group are part of the loop.
+//
+// LDS holds a tile as rows of DP elements in 16-byte chunks, chunk c of row r at c ^ key(r): both the reads along a row
+// (A operands of the scores) and the transposing reads down the rows (A operands of the second product) then
+// spread over all banks.
+#include <math.h>
+
+#include "rows_util.h"
+
+namespace {
+
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int COLS = 32;            // columns (queries or keys) per wavefront
+constexpr int WAVES = 4;
+constexpr int BM = COLS * WAVES;    // columns per workgroup
+constexpr int ROWS = 64;            // streamed rows per tile
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// The running maximum follows a score only when that exceeds it by this much (in powers of two): until then the
+// weights are at most 2^8 and nothing is rescaled.  The final division makes up for it exactly.
+constexpr float LAZY = 8.f;
+
+template <typename T>
+struct FragOf;
+template <>
+struct FragOf<bf16_t> { typedef bf16x8 type; };
+template <>
+struct FragOf<float> { typedef f32x8 type; };
+template <typename T>
+using Frag = typename FragOf<T>::type;
+
+// c += A B over 16 k: lane l holds A[l % 32][8 * (l / 32) + j] and B[8 * (l / 32) + j][l % 32], j < 8.
+__device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+__device__ __forceinline__ f32x16 zero16() {
+  f32x16 z;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) z[i] = 0.f;
+  return z;
+}
+// Weights of 16 rows as a B operand; bf16 rounds them (relative 2^-9, half of what rounding the output costs).
+template <typename T>
+__device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
+  Frag<T> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    if constexpr (sizeof(T) == 2) f[j] = (__bf16)w[8 * t + j];
+    else f[j] = w[8 * t + j];
+  }
+  return f;
+}
+
+// ---- division by the group size (rows -> queries), by a multiplication -------------------------------
+struct Div {
+  uint32_t mul, shift, by;
+};
+Div make_div(uint32_t by) {
+  uint32_t s = 0;
+  while ((1ull << s) < by) ++s;
+  return Div{(uint32_t)((((1ull << s) - by) << 32) / by + 1), s, by};
+}
+__device__ __forceinline__ int div_by(int r, const Div &d) {  // r < 2^31
+  return (int)((__umulhi((uint32_t)r, d.mul) + (uint32_t)r) >> d.shift);
+}
+
+// ---- arguments ------------------------------------------------------------------------------------------
+template <typename T>
+struct Args {
+  const T *q, *k, *v, *o, *dout;
+  T *out, *dq, *dk, *dv;
+  i64 q_ld, k_ld, v_ld, o_ld, dout_ld, out_ld, dq_ld, dk_ld, dv_ld;
+  float *lse, *delta;
+  const int *cu_q, *cu_k;
+  int num_seqs, total_q, total_k, Hq, Hkv, D, causal, tiles;
+  Div G;
+  float scale, scale2;  // scale * log2(e)
+};
+
+// Bounds of a sequence, inside [0, total] whatever the array holds.
+__device__ __forceinline__ int bound_of(const int *cu, int s, int total) { return min(max(cu[s], 0), total); }
+
+// The sequence and first row of tile `tile` where sequence s owns the tiles from floor(start(s) * g / BM) + s on: at
+// least ceil(len * g / BM) of them, without a prefix sum over the lengths.  Tiles behind the last row are empty.
+struct Where {
+  int seq, row0;
+};
+template <int TILE>
+__device__ __forceinline__ Where find_tile(const int *cu, int num_seqs, int total, int g, int tile) {
+  int lo = 0, hi = num_seqs;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if ((bound_of(cu, mid, total) * g) / TILE + mid <= tile) lo = mid;
+    else hi = mid;
+  }
+  return Where{lo, (tile - ((bound_of(cu, lo, total) * g) / TILE + lo)) * TILE};
+}
+struct Seq {
+  int q0, nq, k0, nk;  // first query / key and their numbers
+};
+template <typename A>
+__device__ __forceinline__ Seq seq_of(const A &a, int s) {
+  Seq r;
+  r.q0 = bound_of(a.cu_q, s, a.total_q);
+  r.nq = max(bound_of(a.cu_q, s + 1, a.total_q) - r.q0, 0);
+  r.k0 = bound_of(a.cu_k, s, a.total_k);
+  r.nk = max(bound_of(a.cu_k, s + 1, a.total_k) - r.k0, 0);
+  return r;
+}
+
+// ---- tiles in LDS ----------------------------------------------------------------------------------------
+template <typename T, int DP>
+struct Tile {
+  static constexpr int RB = DP * (int)sizeof(T), NC = RB / 16, CH = 16 / (int)sizeof(T);
+  static constexpr int BYTES = ROWS * RB, PER = ROWS * NC / 256;
+  static __device__ __forceinline__ int key(int row) {
+    return NC == 4 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
+  }
+  // Lane offsets: reads along a row (lane l: row l % 32, elements 16 t + 8 (l / 32) + j) and down 16 rows (lane l:
+  // element 32 db + l % 32 of the rows 4 (l / 32) + j and 8 + 4 (l / 32) + j, j < 4).
+  struct Lane {
+    int row[4], down[4];
+  };
+  static __device__ __forceinline__ Lane lane_offsets(int lane) {
+    Lane o;
+    const int h = lane >> 5, l = lane & 31;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        o.row[i] = l * RB + ((2 * i + h) ^ key(l)) * 16;
+        const int q = (lane & 15) >> 2, p = lane & 3, r = 4 * h + q;  // a 16-lane group transposes 4 rows x 16 elements
+        o.down[i] = r * RB + (((4 * (i & 1) + 2 * ((lane >> 4) & 1) + (p >> 1)) ^ key(r)) * 16) + (p & 1) * 8;
+      } else {
+        o.row[i] = l * RB + ((4 * (i >> 1) + 2 * h + (i & 1)) ^ key(l)) * 16;
+        const int r = 4 * h + i;
+        o.down[i] = r * RB + (((l >> 2) ^ key(r)) * 16) + (l & 3) * 4;
+      }
+    }
+    return o;
+  }
+  static __device__ __forceinline__ Frag<T> along(const unsigned char *rows32, const Lane &o, int t) {
+    Frag<T> f;
+    if constexpr (sizeof(T) == 2) {
+      f = *reinterpret_cast<const bf16x8 *>(rows32 + o.row[t & 3] + (t >> 2) * 128);
+    } else {
+      const f32x4 a = *reinterpret_cast<const f32x4 *>(rows32 + o.row[(t & 1) * 2] + (t >> 1) * 128);
+      const f32x4 b = *reinterpret_cast<const f32x4 *>(rows32 + o.row[(t & 1) * 2 + 1] + (t >> 1) * 128);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
+    }
+    return f;
+  }
+  static __device__ __forceinline__ Frag<T> down(const unsigned char *rows16, const Lane &o, int db) {
+    if constexpr (sizeof(T) == 2) {
+      const unsigned char *p = rows16 + o.down[db & 1] + (db >> 1) * 128;
+      return tr_read_pair(p, p + 8 * RB);
+    } else {
+      Frag<T> f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float *>(rows16 + o.down[j & 3] + (j >> 2) * 8 * RB + db * 128);
+      return f;
+    }
+  }
+  // This thread's chunks of a tile, on their way from memory to LDS.  Row r of the tile is row first + r of a
+  // sequence of n rows; rows and elements that do not exist become zeros.
+  struct Chunks {
+    u32x4 c[PER];
+  };
+  template <typename Row>
+  static __device__ __forceinline__ void fetch(Chunks &to, int first, int n, int D, Row row_ptr) {
+    const int chunk = threadIdx.x % NC, e = chunk * CH;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = first + threadIdx.x / NC + i * (256 / NC);
+      u32x4 v = {0, 0, 0, 0};
+      if (r < n && e < D) {
+        const T *p = row_ptr(r) + e;
+        if (e + CH <= D) {
+          __builtin_memcpy(&v, p, 16);
+        } else {
+          T tmp[CH];
+#pragma unroll
+          for (int x = 0; x < CH; ++x) tmp[x] = e + x < D ? p[x] : (T)0;
+          __builtin_memcpy(&v, tmp, 16);
+        }
+      }
+      to.c[i] = v;
+    }
+  }
+  static __device__ __forceinline__ void put(const Chunks &from, unsigned char *tile) {
+    const int chunk = threadIdx.x % NC;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int r = threadIdx.x / NC + i * (256 / NC);
+      *reinterpret_cast<u32x4 *>(tile + r * RB + ((chunk ^ key(r)) * 16)) = from.c[i];
+    }
+  }
+  // Whether any of 32 rows of the tile holds an infinity or NaN.
+  static __device__ __forceinline__ bool not_finite(const unsigned char *rows32, const Lane &o) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      const Frag<T> f = along(rows32, o, t);
+      uint32_t w[sizeof(f) / 4];
+      __builtin_memcpy(w, &f, sizeof(f));
+#pragma unroll
+      for (int i = 0; i < (int)(sizeof(f) / 4); ++i) {
+        if constexpr (sizeof(T) == 2) {
+          top |= ((w[i] & 0x7f80u) == 0x7f80u) | ((w[i] & 0x7f800000u) == 0x7f800000u);
+        } else {
+          top |= (w[i] & 0x7f800000u) == 0x7f800000u;
+        }
+      }
+    }
+    return __any(top != 0);
+  }
+  // acc[d][column] += sum over 32 rows of X[row][d] W[row][column]
+  static __device__ __forceinline__ void add(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const Lane &o,
+                                             const f32x16 &w) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Frag<T> b = pack8<T>(w, t);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(rows32 + 16 * t * RB, o, db), b, acc[db]);
+    }
+  }
+  // The same where some rows are hidden from some columns (their weight is 0) and hold infinities or NaN: 0 * inf
+  // must not reach a column that does not see the row.  One row at a time, the result taken only by the columns
+  // that see it.  Rare, so slow is fine.
+  template <typename Sees>
+  static __device__ __forceinline__ void add_careful(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const Lane &o,
+                                                     const f32x16 &w, Sees sees) {
+    const int h = (threadIdx.x & 63) >> 5;
+    const Frag<T> b0 = pack8<T>(w, 0), b1 = pack8<T>(w, 1);
+#pragma unroll 1
+    for (int k = 0; k < 32; ++k) {
+      const int j = ((k >> 3) & 1) * 4 + (k & 3);
+      const bool mine = ((k >> 2) & 1) == h, seen = sees(k);
+      Frag<T> b;
+#pragma unroll
+      for (int x = 0; x < 8; ++x) b[x] = k < 16 ? b0[x] : b1[x];
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        Frag<T> f = down(rows32 + (k & 16) * RB, o, db);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) f[x] = mine && x == j ? f[x] : 0;
+        const f32x16 r = mma(f, b, zero16());
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] = seen ? acc[db][i] + r[i] : acc[db][i];
+      }
+    }
+  }
+};
+
+// Eight consecutive elements p[0..8), zero from element n on, as (half of) a B operand.
+template <typename T>
+__device__ __forceinline__ Frag<T> load_frag(const T *p, int n) {
+  Frag<T> f;
+  if (n >= 8) {
+    __builtin_memcpy(&f, p, sizeof(f));
+  } else {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : (T)0;
+    __builtin_memcpy(&f, e, sizeof(f));
+  }
+  return f;
+}
+// Four consecutive results p[0..4), as many as n allows.
+template <typename T>
+__device__ __forceinline__ void store4(T *p, int n, float a, float b, float c, float d) {
+  T e[4];
+  from_f32(a, e[0]);
+  from_f32(b, e[1]);
+  from_f32(c, e[2]);
+  from_f32(d, e[3]);
+  if (n >= 4) {
+    __builtin_memcpy(p, e, sizeof(e));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = e[i];
+  }
+}
+// acc[d][column] * f -> p[d] of the lane's column
+template <typename T, int DP>
+__device__ __forceinline__ void store_column(T *p, int D, const f32x16 (&acc)[DP / 32], float f) {
+  const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int d = 32 * db + 8 * b + 4 * h;
+      store4(p + d, D - d, acc[db][4 * b] * f, acc[db][4 * b + 1] * f, acc[db][4 * b + 2] * f, acc[db][4 * b + 3] * f);
+    }
+}
+
+// The queries of a workgroup: what the forward and the dQ kernel share.
+struct Rows {
+  Seq s;
+  int nrows, off, row, query, head, lim;  // lim: last visible key of the lane's query, negative: none
+  bool live;
+};
+template <typename T>
+__device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, Rows &r, int &row0) {
+  const int g = (int)a.G.by;
+  const Where w = find_tile<BM>(a.cu_q, a.num_seqs, a.total_q, g, tile);
+  r.s = seq_of(a, w.seq);
+  r.nrows = r.s.nq * g;
+  row0 = w.row0;
+  if (row0 < 0 || row0 >= r.nrows) return false;
+  r.off = r.s.nk - r.s.nq;
+  r.row = row0 + (threadIdx.x >> 6) * COLS + (threadIdx.x & 31);
+  r.live = r.row < r.nrows;
+  const int rr = min(r.row, r.nrows - 1);
+  r.query = div_by(rr, a.G);
+  r.head = kvh * g + (rr - r.query * g);
+  r.lim = a.causal ? min(r.query + r.off, r.s.nk - 1) : r.s.nk - 1;
+  return true;
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(const Args<T> a) {
+  typedef Tile<T, DP> TL;
+  __shared__ __align__(16) unsigned char lds[2 * TL::BYTES];
+  unsigned char *const ldsK = lds, *const ldsV = lds + TL::BYTES;
+  const int kvh = blockIdx.x % a.Hkv;
+  const int t0 = blockIdx.x / a.Hkv;
+  const int tile = a.causal ? a.tiles - 1 - t0 : t0;  // the queries with the most keys first
+  Rows r;
+  int row0;
+  if (!rows_of(a, tile, kvh, r, row0)) return;
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  const auto lo = TL::lane_offsets(lane);
+
+  Frag<T> q[DP / 16];
+  {
+    const T *p = a.q + (i64)(r.s.q0 + r.query) * a.q_ld + r.head * a.D;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) q[t] = load_frag<T>(p + 16 * t + 8 * h, r.live ? a.D - 16 * t - 8 * h : 0);
+  }
+  // key range of the workgroup, and which tiles of the wavefront lie under its first / behind its last query
+
+  const int last = min(row0 + BM, r.nrows) - 1;
+  const int kend = a.causal ? min(max(div_by(last, a.G) + r.off + 1, 0), r.s.nk) : r.s.nk;
+  const int wfirst = min(row0 + wave * COLS, r.nrows - 1), wlast = min(row0 + wave * COLS + COLS, r.nrows) - 1;
+  const int all_see = a.causal ? min(div_by(wfirst, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
+  const int some_see = a.causal ? min(div_by(wlast, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
+
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
+  float m = -INFINITY, l = 0.f;  // of the scores times scale2 (base 2); l over this lane's rows only
+
+  const T *const kp = a.k + (i64)r.s.k0 * a.k_ld + kvh * a.D, *const vp = a.v + (i64)r.s.k0 * a.v_ld + kvh * a.D;
+  auto k_row = [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; };
+  auto v_row = [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; };
+  typename TL::Chunks ck, cv;
+  TL::fetch(ck, 0, kend, a.D, k_row);
+  TL::fetch(cv, 0, kend, a.D, v_row);
+  for (int key0 = 0; key0 < kend; key0 += ROWS) {
+    __syncthreads();
+    TL::put(ck, ldsK);
+    TL::put(cv, ldsV);
+    __syncthreads();
+    if (key0 + ROWS < kend) {
+      TL::fetch(ck, key0 + ROWS, kend, a.D, k_row);
+      TL::fetch(cv, key0 + ROWS, kend, a.D, v_row);
+    }
+#pragma unroll
+    for (int sub = 0; sub < ROWS; sub += 32) {
+      const int kb = key0 + sub;
+      if (kb > some_see) break;
+      f32x16 s = zero16();
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) s = mma(TL::along(ldsK + sub * TL::RB, lo, t), q[t], s);
+      const bool edge = kb + 31 > all_see;
+      if (edge) {
+        const int rel = r.lim - kb - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 <= rel ? s[i] : -INFINITY;
+      }
+      float top = s[0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+      top *= a.scale2;
+      if (__any(top > m + LAZY)) {
+        const float m_new = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+        const float f = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+        m = m_new;
+        l *= f;
+#pragma unroll
+        for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) acc[db][i] *= f;
+      }
+      const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: every weight is 0
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale2 - base);
+        sum[i & 3] += s[i];
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const unsigned char *const v32 = ldsV + sub * TL::RB;
+      if (edge && TL::not_finite(v32, lo))
+        TL::add_careful(acc, v32, lo, s, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
+      else
+        TL::add(acc, v32, lo, s);
+    }
+  }
+  l += __shfl_xor(l, 32, 64);
+  if (!r.live) return;
+  const float f = r.lim < 0 ? 0.f : 1.f / l;
+  store_column<T, DP>(a.out + (i64)(r.s.q0 + r.query) * a.out_ld + r.head * a.D, a.D, acc, f);
+  if (a.lse && h == 0)
+    a.lse[(i64)(r.s.q0 + r.query) * a.Hq + r.head] = r.lim < 0 ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
+// dQ, and delta for the kernel below.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(const Args<T> a) {
+  typedef Tile<T, DP> TL;
+  __shared__ __align__(16) unsigned char lds[2 * TL::BYTES];
+  unsigned char *const ldsK = lds, *const ldsV = lds + TL::BYTES;
+  const int kvh = blockIdx.x % a.Hkv;
+  const int t0 = blockIdx.x / a.Hkv;
+  const int tile = a.causal ? a.tiles - 1 - t0 : t0;
+  Rows r;
+  int row0;
+  if (!rows_of(a, tile, kvh, r, row0)) return;
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  const auto lo = TL::lane_offsets(lane);
+
+  Frag<T> q[DP / 16], dout[DP / 16];
+  float delta = 0.f;
+  {
+    const i64 token = r.s.q0 + r.query;
+    const T *p = a.q + token * a.q_ld + r.head * a.D, *pd = a.dout + token * a.dout_ld + r.head * a.D,
+            *po = a.o + token * a.o_ld + r.head * a.D;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      const int e = 16 * t + 8 * h, n = r.live ? a.D - e : 0;
+      q[t] = load_frag<T>(p + e, n);
+      dout[t] = load_frag<T>(pd + e, n);
+      const Frag<T> o = load_frag<T>(po + e, n);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) delta += (float)dout[t][j] * (float)o[j];
+    }
+    delta += __shfl_xor(delta, 32, 64);
+  }
+  const i64 at = (i64)(r.s.q0 + r.query) * a.Hq + r.head;
+  float lse2 = INFINITY;  // a row that does not exist has no weight anywhere
+  if (r.live) {
+    lse2 = a.lse[at] * LOG2E;
+    if (h == 0) a.delta[at] = delta;
+  }
+  const int last = min(row0 + BM, r.nrows) - 1;
+  const int kend = a.causal ? min(max(div_by(last, a.G) + r.off + 1, 0), r.s.nk) : r.s.nk;
+  const int wfirst = min(row0 + wave * COLS, r.nrows - 1), wlast = min(row0 + wave * COLS + COLS, r.nrows) - 1;
+  const int all_see = a.causal ? min(div_by(wfirst, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
+  const int some_see = a.causal ? min(div_by(wlast, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
+
+  f32x16 acc[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
+  const T *const kp = a.k + (i64)r.s.k0 * a.k_ld + kvh * a.D, *const vp = a.v + (i64)r.s.k0 * a.v_ld + kvh * a.D;
+  auto k_row = [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; };
+  auto v_row = [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; };
+  typename TL::Chunks ck, cv;
+  TL::fetch(ck, 0, kend, a.D, k_row);
+  TL::fetch(cv, 0, kend, a.D, v_row);
+  for (int key0 = 0; key0 < kend; key0 += ROWS) {
+    __syncthreads();
+    TL::put(ck, ldsK);
+    TL::put(cv, ldsV);
+    __syncthreads();
+    if (key0 + ROWS < kend) {
+      TL::fetch(ck, key0 + ROWS, kend, a.D, k_row);
+      TL::fetch(cv, key0 + ROWS, kend, a.D, v_row);
+    }
+#pragma unroll
+    for (int sub = 0; sub < ROWS; sub += 32) {
+      const int kb = key0 + sub;
+      if (kb > some_see) break;
+      const unsigned char *const k32 = ldsK + sub * TL::RB;
+      f32x16 s = zero16(), dp = zero16();
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) {
+        s = mma(TL::along(k32, lo, t), q[t], s);
+        dp = mma(TL::along(ldsV + sub * TL::RB, lo, t), dout[t], dp);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale2 - lse2) * (dp[i] - delta);
+      const bool edge = kb + 31 > all_see;
+      if (edge) {
+        const int rel = r.lim - kb - 4 * h;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 <= rel ? s[i] : 0.f;
+      }
+      if (edge && TL::not_finite(k32, lo))
+        TL::add_careful(acc, k32, lo, s, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
+      else
+        TL::add(acc, k32, lo, s);
+    }
+  }
+  if (r.live) store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale);
+}
+
+// dK and dV: keys in registers, the packed queries of the group streamed.
+template <typename T, int DP>
+__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(const Args<T> a) {
+  typedef Tile<T, DP> TL;
+  __shared__ __align__(16) unsigned char lds[2 * TL::BYTES + 2 * ROWS * 4];
+  unsigned char *const ldsQ = lds, *const ldsD = lds + TL::BYTES;
+  float *const ldsL = reinterpret_cast<float *>(lds + 2 * TL::BYTES), *const ldsDelta = ldsL + ROWS;
+  const int kvh = blockIdx.x % a.Hkv;
+  const Where w = find_tile<BM>(a.cu_k, a.num_seqs, a.total_k, 1, blockIdx.x / a.Hkv);
+  const Seq s = seq_of(a, w.seq);
+  if (w.row0 < 0 || w.row0 >= s.nk) return;
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  const auto lo = TL::lane_offsets(lane);
+  const int g = (int)a.G.by, nrows = s.nq * g, off = s.nk - s.nq;
+  const int wkey = w.row0 + wave * COLS, key = wkey + (lane & 31);
+  const bool live = key < s.nk;
+
+  Frag<T> k[DP / 16], v[DP / 16];
+  {
+    const i64 token = s.k0 + min(key, s.nk - 1);
+    const T *pk = a.k + token * a.k_ld + kvh * a.D, *pv = a.v + token * a.v_ld + kvh * a.D;
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+      const int e = 16 * t + 8 * h, n = live ? a.D - e : 0;
+      k[t] = load_frag<T>(pk + e, n);
+      v[t] = load_frag<T>(pv + e, n);
+    }
+  }
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = zero16();
+
+  // the first query that sees the workgroup's first key
+  const int first = a.causal ? min(max(w.row0 - off, 0), s.nq) * g : 0;
+  auto row_of = [&](const T *base, i64 ld, int r) __attribute__((always_inline)) {
+    const int query = div_by(r, a.G);
+    return base + (i64)(s.q0 + query) * ld + (kvh * g + (r - query * g)) * a.D;
+  };
+  auto q_row = [&](int r) __attribute__((always_inline)) { return row_of(a.q, a.q_ld, r); };
+  auto d_row = [&](int r) __attribute__((always_inline)) { return row_of(a.dout, a.dout_ld, r); };
+  typename TL::Chunks cq, cd;
+  float fl, fd;
+  auto fetch_all = [&](int r0) __attribute__((always_inline)) {
+    TL::fetch(cq, r0, nrows, a.D, q_row);
+    TL::fetch(cd, r0, nrows, a.D, d_row);
+    fl = INFINITY, fd = 0.f;  // rows that do not exist have no weight
+    const int r = r0 + (int)threadIdx.x;
+    if (threadIdx.x < ROWS && r < nrows) {
+      const int query = div_by(r, a.G);
+      const i64 at = (i64)(s.q0 + query) * a.Hq + kvh * g + (r - query * g);
+      fl = a.lse[at] * LOG2E;
+      fd = a.delta[at];
+    }
+  };
+  fetch_all(first);
+  for (int r0 = first; r0 < nrows; r0 += ROWS) {
+    __syncthreads();
+    TL::put(cq, ldsQ);
+    TL::put(cd, ldsD);
+    if (threadIdx.x < ROWS) {
+      ldsL[threadIdx.x] = fl;
+      ldsDelta[threadIdx.x] = fd;
+    }
+    __syncthreads();
+    if (r0 + ROWS < nrows) fetch_all(r0 + ROWS);
+#pragma unroll
+    for (int sub = 0; sub < ROWS; sub += 32) {
+      const int rb = r0 + sub;
+      if (rb >= nrows) break;
+      if (a.causal && div_by(min(rb + 31, nrows - 1), a.G) + off < wkey) continue;  // no row sees the wavefront's keys
+      const unsigned char *const q32 = ldsQ + sub * TL::RB, *const d32 = ldsD + sub * TL::RB;
+      f32x16 p = zero16(), ds = zero16();
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) {
+        p = mma(TL::along(q32, lo, t), k[t], p);
+        ds = mma(TL::along(d32, lo, t), v[t], ds);
+      }
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(ldsL + sub + 8 * b + 4 * h);
+        const f32x4 delta = *reinterpret_cast<const f32x4 *>(ldsDelta + sub + 8 * b + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[4 * b + i] = __builtin_amdgcn_exp2f(p[4 * b + i] * a.scale2 - lse2[i]);
+          ds[4 * b + i] = p[4 * b + i] * (ds[4 * b + i] - delta[i]);
+        }
+      }
+      const bool edge = a.causal && div_by(rb, a.G) + off < wkey + 31;
+      if (edge) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const bool sees = div_by(rb + 8 * (i / 4) + 4 * h + i % 4, a.G) + off >= key;
+          p[i] = sees ? p[i] : 0.f;
+          ds[i] = sees ? ds[i] : 0.f;
+        }
+      }
+      if (edge && (TL::not_finite(q32, lo) || TL::not_finite(d32, lo))) {
+        auto sees = [&](int i) __attribute__((always_inline)) { return div_by(rb + i, a.G) + off >= key; };
+        TL::add_careful(dv, d32, lo, p, sees);
+        TL::add_careful(dk, q32, lo, ds, sees);
+      } else {
+        TL::add(dv, d32, lo, p);
+        TL::add(dk, q32, lo, ds);
+      }
+    }
+  }
+  if (!live) return;
+  store_column<T, DP>(a.dk + (i64)(s.k0 + key) * a.dk_ld + kvh * a.D, a.D, dk, a.scale);
+  store_column<T, DP>(a.dv + (i64)(s.k0 + key) * a.dv_ld + kvh * a.D, a.D, dv, 1.f);
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+template <typename T>
+bool aligned(const void *p) { return ((uintptr_t)p & (sizeof(T) - 1)) == 0; }
+
+int check_shape(const char *name, int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
+  UNET_REQUIRE(num_seqs >= 0 && total_q >= 0 && total_k >= 0, "%s: num_seqs %d, total_q %lld, total_k %lld", name, num_seqs,
+               (long long)total_q, (long long)total_k);
+  UNET_REQUIRE(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "%s: %d query heads are no multiple of %d key/value heads", name, Hq, Hkv);
+  UNET_REQUIRE(D >= 1, "%s: head_dim %d", name, D);
+  if (D > 128) return unet_set_error(UNET_ERR_UNSUPPORTED, "%s: head_dim %d is larger than 128", name, D);
+  // rows and tiles are counted in 32 bits; a grid has fewer than 2^31 workgroups
+  const i64 most = ((i64)1 << 31) - 256, rows = total_q * (Hq / Hkv);
+  UNET_REQUIRE(total_q <= most && total_k <= most && rows <= most &&
+                   (rows / BM + num_seqs) * Hkv <= most && (total_k / BM + num_seqs) * Hkv <= most,
+               "%s: too many tokens (%lld queries, %lld keys, %d and %d heads)", name, (long long)total_q, (long long)total_k,
+               Hq, Hkv);
+  return UNET_OK;
+}
+template <typename T>
+int check_matrix(const char *name, const char *what, const T *p, i64 ld, i64 rows, i64 cols) {
+  UNET_REQUIRE(p || rows == 0, "%s: %s is NULL", name, what);
+  UNET_REQUIRE(ld >= cols, "%s: the stride of %s (%lld) is smaller than its %lld columns", name, what, (long long)ld,
+               (long long)cols);
+  UNET_REQUIRE(aligned<T>(p), "%s: %s is misaligned", name, what);
+  return UNET_OK;
+}
+#define TRY(call)                    \
+  do {                               \
+    const int rc_ = (call);          \
+    if (rc_ != UNET_OK) return rc_;  \
+  } while (0)
+
+template <typename T>
+int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld,
+                const int32_t *cu_q, const int32_t *cu_k, int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D,
+                float scale, int causal) {
+  TRY(check_shape(name, num_seqs, total_q, total_k, Hq, Hkv, D));
+  UNET_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale %g is not positive and finite", name, (double)scale);
+  UNET_REQUIRE(num_seqs == 0 || (cu_q && cu_k), "%s: cu_q or cu_k is NULL", name);
+  UNET_REQUIRE(aligned<int>(cu_q) && aligned<int>(cu_k), "%s: cu_q or cu_k is misaligned", name);
+  TRY(check_matrix(name, "q", q, q_ld, total_q, (i64)Hq * D));
+  TRY(check_matrix(name, "k", k, k_ld, total_k, (i64)Hkv * D));
+  TRY(check_matrix(name, "v", v, v_ld, total_k, (i64)Hkv * D));
+  a.q = q, a.k = k, a.v = v, a.q_ld = q_ld, a.k_ld = k_ld, a.v_ld = v_ld;
+  a.cu_q = cu_q, a.cu_k = cu_k, a.num_seqs = num_seqs, a.total_q = (int)total_q, a.total_k = (int)total_k;
+  a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.causal = causal != 0, a.G = make_div((uint32_t)(Hq / Hkv));
+  a.scale = scale, a.scale2 = scale * LOG2E;
+  return UNET_OK;
+}
+
+// f(DP) with the head dimension padded to the tile's.
+template <typename F>
+void with_dim(int D, F f) {
+  if (D <= 32) f(std::integral_constant<int, 32>());
+  else if (D <= 64) f(std::integral_constant<int, 64>());
+  else f(std::integral_constant<int, 128>());
+}
+
+template <typename T>
+int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T *out, i64 out_ld, float *lse,
+            const int32_t *cu_q, const int32_t *cu_k, int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D,
+            float scale, int causal, void *ws, size_t ws_bytes, hipStream_t st) {
+  const char *const name = "dot_attention";
+  Args<T> a{};
+  TRY(common_args(name, a, q, q_ld, k, k_ld, v, v_ld, cu_q, cu_k, num_seqs, total_q, total_k, Hq, Hkv, D, scale, causal));
+  TRY(check_matrix(name, "out", out, out_ld, total_q, (i64)Hq * D));
+  UNET_REQUIRE(aligned<float>(lse), "%s: lse is misaligned", name);
+  if (num_seqs == 0 || total_q == 0) return UNET_OK;
+  a.out = out, a.out_ld = out_ld, a.lse = lse;
+  a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+  with_dim(D, [&](auto dp) { attention_kernel<T, decltype(dp)::value><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a); });
+  UNET_LAUNCH_CHECK(name);
+  return UNET_OK;
+}
+
+template <typename T>
+int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, const T *out,
+             i64 out_ld, const float *lse, T *dq, i64 dq_ld, T *dk, i64 dk_ld, T *dv, i64 dv_ld, const int32_t *cu_q,
+             const int32_t *cu_k, int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, float scale, int causal,
+             void *ws, size_t ws_bytes, hipStream_t st) {
+  const char *const name = "dot_attention_backward";
+  Args<T> a{};
+  TRY(common_args(name, a, q, q_ld, k, k_ld, v, v_ld, cu_q, cu_k, num_seqs, total_q, total_k, Hq, Hkv, D, scale, causal));
+  TRY(check_matrix(name, "grad_out", dout, dout_ld, total_q, (i64)Hq * D));
+  TRY(check_matrix(name, "out", out, out_ld, total_q, (i64)Hq * D));
+  TRY(check_matrix(name, "grad_q", (const T *)dq, dq_ld, total_q, (i64)Hq * D));
+  TRY(check_matrix(name, "grad_k", (const T *)dk, dk_ld, total_k, (i64)Hkv * D));
+  TRY(check_matrix(name, "grad_v", (const T *)dv, dv_ld, total_k, (i64)Hkv * D));
+  UNET_REQUIRE((lse || total_q == 0) && aligned<float>(lse), "%s: lse is NULL or misaligned", name);
+  size_t need = 0;
+  TRY(unet_dot_attention_backward_workspace_bytes(num_seqs, total_q, total_k, Hq, Hkv, D, &need));
+  UNET_REQUIRE(ws_bytes >= need && (ws || !need), "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
+  UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
+  if (num_seqs == 0 || (total_q == 0 && total_k == 0)) return UNET_OK;
+  a.dout = dout, a.o = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = const_cast<float *>(lse), a.delta = (float *)ws;
+  a.dout_ld = dout_ld, a.o_ld = out_ld, a.dq_ld = dq_ld, a.dk_ld = dk_ld, a.dv_ld = dv_ld;
+  a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+  const unsigned key_tiles = (unsigned)(total_k / BM) + num_seqs;
+  with_dim(D, [&](auto dp) {
+    constexpr int DP = decltype(dp)::value;
+    if (total_q) attention_dq_kernel<T, DP><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
+    if (total_k) attention_dkv_kernel<T, DP><<<key_tiles * Hkv, 256, 0, st>>>(a);
+  });
+  UNET_LAUNCH_CHECK(name);
+  return UNET_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv,
+                                       int head_dim, size_t *bytes_host) {
+  UNET_REQUIRE(bytes_host, "dot_attention_workspace_bytes: NULL result");
+  TRY(check_shape("dot_attention_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
+  *bytes_host = 0;
+  return UNET_OK;
+}
+int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
+                                                int heads_kv, int head_dim, size_t *bytes_host) {
+  UNET_REQUIRE(bytes_host, "dot_attention_backward_workspace_bytes: NULL result");
+  TRY(check_shape("dot_attention_backward_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
+  *bytes_host = (size_t)total_q * heads_q * sizeof(float);  // delta
+  return UNET_OK;
+}
+
+int unet_dot_attention_f32(const float *q, int64_t q_ld, const float *k, int64_t k_ld, const float *v, int64_t v_ld,
+                           float *out, int64_t out_ld, float *lse, const int32_t *cu_q, const int32_t *cu_k,
+                           int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv, int head_dim,
+                           float scale, int causal, void *workspace, size_t workspace_bytes, unet_stream_t stream) {
+  return forward<float>(q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, cu_q, cu_k, num_seqs, total_q, total_k, heads_q,
+                        heads_kv, head_dim, scale, causal, workspace, workspace_bytes, as_stream(stream));
+}
+int unet_dot_attention_bf16(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t k_ld, const uint16_t *v,
+                            int64_t v_ld, uint16_t *out, int64_t out_ld, float *lse, const int32_t *cu_q,
+                            const int32_t *cu_k, int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
+                            int heads_kv, int head_dim, float scale, int causal, void *workspace,
+                            size_t workspace_bytes, unet_stream_t stream) {
+  return forward<bf16_t>(q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, cu_q, cu_k, num_seqs, total_q, total_k, heads_q,
+                         heads_kv, head_dim, scale, causal, workspace, workspace_bytes, as_stream(stream));
+}
+int unet_dot_attention_backward_f32(const float *grad_out, int64_t grad_out_ld, const float *q, int64_t q_ld,
+                                    const float *k, int64_t k_ld, const float *v, int64_t v_ld, const float *out,
+                                    int64_t out_ld, const float *lse, float *grad_q, int64_t grad_q_ld, float *grad_k,
+                                    int64_t grad_k_ld, float *grad_v, int64_t grad_v_ld, const int32_t *cu_q,
+                                    const int32_t *cu_k, int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
+                                    int heads_kv, int head_dim, float scale, int causal, void *workspace,
+                                    size_t workspace_bytes, unet_stream_t stream) {
+  return backward<float>(grad_out, grad_out_ld, q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, grad_q, grad_q_ld, grad_k,
+                         grad_k_ld, grad_v, grad_v_ld, cu_q, cu_k, num_seqs, total_q, total_k, heads_q, heads_kv, head_dim,
+                         scale, causal, workspace, workspace_bytes, as_stream(stream));
+}
+int unet_dot_attention_backward_bf16(const uint16_t *grad_out, int64_t grad_out_ld, const uint16_t *q, int64_t q_ld,
+                                     const uint16_t *k, int64_t k_ld, const uint16_t *v, int64_t v_ld,
+                                     const uint16_t *out, int64_t out_ld, const float *lse, uint16_t *grad_q,
+                                     int64_t grad_q_ld, uint16_t *grad_k, int64_t grad_k_ld, uint16_t *grad_v,
+                                     int64_t grad_v_ld, const int32_t *cu_q, const int32_t *cu_k, int num_seqs,
+                                     int64_t total_q, int64_t total_k, int heads_q, int heads_kv, int head_dim,
+                                     float scale, int causal, void *workspace, size_t workspace_bytes,
+                                     unet_stream_t stream) {
+  return backward<bf16_t>(grad_out, grad_out_ld, q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, grad_q, grad_q_ld, grad_k,
+                          grad_k_ld, grad_v, grad_v_ld, cu_q, cu_k, num_seqs, total_q, total_k, heads_q, heads_kv, head_dim,
+                          scale, causal, workspace, workspace_bytes, as_stream(stream));
+}
+
+}  // extern "C"
