@@ -30,7 +30,6 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 constexpr int COLS = 32;            // columns (queries or keys) per wavefront
 constexpr int WAVES = 4;
 constexpr int BM = COLS * WAVES;    // columns per workgroup
-constexpr int ROWS = 64;            // streamed rows per tile
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // The running maximum follows a score only when that exceeds it by this much (in powers of two): until then the
 // weights are at most 2^8 and nothing is rescaled.  The final division makes up for it exactly.
@@ -130,10 +129,11 @@ __device__ __forceinline__ Seq seq_of(const A &a, int s) {
 }
 
 // ---- tiles in LDS ----------------------------------------------------------------------------------------
-template <typename T, int DP>
+template <typename T, int DP, int ROWS>
 struct Tile {
   static constexpr int RB = DP * (int)sizeof(T), NC = RB / 16, CH = 16 / (int)sizeof(T);
   static constexpr int BYTES = ROWS * RB, PER = ROWS * NC / 256;
+  static_assert(ROWS % 32 == 0 && ROWS * NC % 256 == 0, "whole sub-tiles, whole chunks per thread");
   static __device__ __forceinline__ int key(int row) {
     return NC == 4 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
   }
@@ -187,26 +187,30 @@ struct Tile {
   struct Chunks {
     u32x4 c[PER];
   };
-  template <typename Row>
+  template <bool TAIL, typename Row>
   static __device__ __forceinline__ void fetch(Chunks &to, int first, int n, int D, Row row_ptr) {
-    const int chunk = threadIdx.x % NC, e = chunk * CH;
+    const int e = (threadIdx.x % NC) * CH, r0 = first + threadIdx.x / NC;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-      const int r = first + threadIdx.x / NC + i * (256 / NC);
-      u32x4 v = {0, 0, 0, 0};
-      if (r < n && e < D) {
-        const T *p = row_ptr(r) + e;
-        if (e + CH <= D) {
-          __builtin_memcpy(&v, p, 16);
+    for (int i = 0; i < PER; ++i) to.c[i] = u32x4{0, 0, 0, 0};
+    if (first >= n) return;
+    if (e < D) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) {
+        const T *p = row_ptr(min(r0 + i * (256 / NC), n - 1)) + e;
+        if (!TAIL || e + CH <= D) {
+          __builtin_memcpy(&to.c[i], p, 16);
         } else {
           T tmp[CH];
 #pragma unroll
           for (int x = 0; x < CH; ++x) tmp[x] = e + x < D ? p[x] : (T)0;
-          __builtin_memcpy(&v, tmp, 16);
+          __builtin_memcpy(&to.c[i], tmp, 16);
         }
       }
-      to.c[i] = v;
     }
+    if (first + ROWS > n)
+#pragma unroll
+      for (int i = 0; i < PER; ++i)
+        if (r0 + i * (256 / NC) >= n) to.c[i] = u32x4{0, 0, 0, 0};
   }
   static __device__ __forceinline__ void put(const Chunks &from, unsigned char *tile) {
     const int chunk = threadIdx.x % NC;
@@ -235,41 +239,43 @@ struct Tile {
     }
     return __any(top != 0);
   }
-  // acc[d][column] += sum over 32 rows of X[row][d] W[row][column]
-  static __device__ __forceinline__ void add(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const Lane &o,
-                                             const f32x16 &w) {
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const Frag<T> b = pack8<T>(w, t);
-#pragma unroll
-      for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(rows32 + 16 * t * RB, o, db), b, acc[db]);
-    }
-  }
-  // The same where some rows are hidden from some columns (their weight is 0) and hold infinities or NaN: 0 * inf
-  // must not reach a column that does not see the row.  One row at a time, the result taken only by the columns
-  // that see it.  Rare, so slow is fine.
+  // acc[d][column] += sum over 32 rows of X[row][d] W[row][column].  edge: some rows are hidden from some columns, with
+  // weight 0.  If such rows hold infinities or NaN, 0 * inf must not reach a column that does not see them: then the
+  // rows are added one at a time, the result taken by the columns that see the row, and the common product reads
+  // zeros instead.  Rare, so slow is fine; what matters is that the accumulators stay where they are.
+  static constexpr int ZEROS = 32 * RB;
   template <typename Sees>
-  static __device__ __forceinline__ void add_careful(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const Lane &o,
-                                                     const f32x16 &w, Sees sees) {
-    const int h = (threadIdx.x & 63) >> 5;
+  static __device__ __forceinline__ void add(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const unsigned char *zeros,
+                                             const Lane &o, const f32x16 &w, bool edge, Sees sees) {
     const Frag<T> b0 = pack8<T>(w, 0), b1 = pack8<T>(w, 1);
+    if (edge && not_finite(rows32, o)) {
+      const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll 1
-    for (int k = 0; k < 32; ++k) {
-      const int j = ((k >> 3) & 1) * 4 + (k & 3);
-      const bool mine = ((k >> 2) & 1) == h, seen = sees(k);
-      Frag<T> b;
+      for (int k = 0; k < 32; ++k) {
+        const int j = ((k >> 3) & 1) * 4 + (k & 3);
+        const bool mine = ((k >> 2) & 1) == h, seen = sees(k);
+        Frag<T> b;
 #pragma unroll
-      for (int x = 0; x < 8; ++x) b[x] = k < 16 ? b0[x] : b1[x];
+        for (int x = 0; x < 8; ++x) b[x] = k < 16 ? b0[x] : b1[x];
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db) {
-        Frag<T> f = down(rows32 + (k & 16) * RB, o, db);
+        for (int db = 0; db < DP / 32; ++db) {
+          Frag<T> f = down(rows32 + (k & 16) * RB, o, db);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) f[x] = mine && x == j ? f[x] : 0;
-        const f32x16 r = mma(f, b, zero16());
+          for (int x = 0; x < 8; ++x) f[x] = mine && x == j ? f[x] : 0;
+          const f32x16 r = mma(f, b, zero16());
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[db][i] = seen ? acc[db][i] + r[i] : acc[db][i];
+          for (int i = 0; i < 16; ++i) acc[db][i] += seen ? r[i] : 0.f;
+        }
       }
+      rows32 = zeros;
     }
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(rows32, o, db), b0, acc[db]);
+#pragma unroll
+    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(rows32 + 16 * RB, o, db), b1, acc[db]);
+  }
+  static __device__ __forceinline__ void clear(unsigned char *zeros) {
+    for (int i = threadIdx.x * 16; i < ZEROS; i += 256 * 16) *reinterpret_cast<u32x4 *>(zeros + i) = u32x4{0, 0, 0, 0};
   }
 };
 
@@ -340,19 +346,66 @@ __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, Row
   return true;
 }
 
+// Streamed rows per tile: 64, or 32 where a row is 256 bytes and more (a thread then holds 16 registers of the tile that
+// is on its way; with 64 rows the kernels with two streamed matrices and 64 or 128 accumulators spill).
 template <typename T, int DP>
+constexpr int tile_rows() { return DP * sizeof(T) >= 256 ? 32 : 64; }
+
+// Runs step(tile, buffer) for the tiles [0, n) with the next tile on its way to the other buffer: fetch(t) loads tile t to
+// registers, put(buffer) writes them to LDS.  One barrier per tile: behind it every wavefront has left the buffer
+// that is written next, and sees the one that is read next.
+template <typename Fetch, typename Put, typename Step>
+__device__ __forceinline__ void stream(int n, Fetch fetch, Put put, Step step) {
+  if (n <= 0) return;
+  fetch(0);
+  put(0);
+  fetch(1);
+#pragma unroll 1
+  for (int t = 0; t < n; ++t) {
+    __syncthreads();
+    if (t + 1 < n) {
+      put((t + 1) & 1);
+      fetch(t + 2);
+    }
+    step(t, t & 1);
+  }
+}
+
+// Which keys the queries of a workgroup and of this wavefront see (all of them / at least one of them).
+struct Span {
+  int kend;                 // keys [0, kend) are seen by the workgroup
+  int all;                  // keys [0, all] by every query of the workgroup
+  int wave_all, wave_some;  // keys [0, wave_all] by every, [0, wave_some] by some query of the wavefront
+};
+template <typename T>
+__device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row0) {
+  const int wave = threadIdx.x >> 6, last = r.s.nk - 1;
+  if (!a.causal) return Span{r.s.nk, last, last, last};
+  auto sees = [&](int row) __attribute__((always_inline)) { return min(div_by(min(row, r.nrows - 1), a.G) + r.off, last); };
+  Span s;
+  s.kend = max(sees(row0 + BM - 1) + 1, 0);
+  s.all = sees(row0);
+  s.wave_all = sees(row0 + wave * COLS);
+  s.wave_some = row0 + wave * COLS < r.nrows ? sees(row0 + wave * COLS + COLS - 1) : -1;
+  return s;
+}
+
+template <typename T, int DP, bool TAIL>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(const Args<T> a) {
-  typedef Tile<T, DP> TL;
-  __shared__ __align__(16) unsigned char lds[2 * TL::BYTES];
-  unsigned char *const ldsK = lds, *const ldsV = lds + TL::BYTES;
+  constexpr int ROWS = 64;
+  typedef Tile<T, DP, ROWS> TL;
+  __shared__ __align__(16) unsigned char lds[4 * TL::BYTES + TL::ZEROS];
+  unsigned char *const zeros = lds + 4 * TL::BYTES;
   const int kvh = blockIdx.x % a.Hkv;
   const int t0 = blockIdx.x / a.Hkv;
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;  // the queries with the most keys first
   Rows r;
   int row0;
   if (!rows_of(a, tile, kvh, r, row0)) return;
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  TL::clear(zeros);
+  const int lane = threadIdx.x & 63, h = lane >> 5;
   const auto lo = TL::lane_offsets(lane);
+  const Span span = span_of(a, r, row0);
 
   Frag<T> q[DP / 16];
   {
@@ -360,76 +413,73 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) q[t] = load_frag<T>(p + 16 * t + 8 * h, r.live ? a.D - 16 * t - 8 * h : 0);
   }
-  // key range of the workgroup, and which tiles of the wavefront lie under its first / behind its last query
-
-  const int last = min(row0 + BM, r.nrows) - 1;
-  const int kend = a.causal ? min(max(div_by(last, a.G) + r.off + 1, 0), r.s.nk) : r.s.nk;
-  const int wfirst = min(row0 + wave * COLS, r.nrows - 1), wlast = min(row0 + wave * COLS + COLS, r.nrows) - 1;
-  const int all_see = a.causal ? min(div_by(wfirst, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
-  const int some_see = a.causal ? min(div_by(wlast, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
-
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
   float m = -INFINITY, l = 0.f;  // of the scores times scale2 (base 2); l over this lane's rows only
 
   const T *const kp = a.k + (i64)r.s.k0 * a.k_ld + kvh * a.D, *const vp = a.v + (i64)r.s.k0 * a.v_ld + kvh * a.D;
-  auto k_row = [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; };
-  auto v_row = [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; };
   typename TL::Chunks ck, cv;
-  TL::fetch(ck, 0, kend, a.D, k_row);
-  TL::fetch(cv, 0, kend, a.D, v_row);
-  for (int key0 = 0; key0 < kend; key0 += ROWS) {
-    __syncthreads();
-    TL::put(ck, ldsK);
-    TL::put(cv, ldsV);
-    __syncthreads();
-    if (key0 + ROWS < kend) {
-      TL::fetch(ck, key0 + ROWS, kend, a.D, k_row);
-      TL::fetch(cv, key0 + ROWS, kend, a.D, v_row);
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    TL::template fetch<TAIL>(ck, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; });
+    TL::template fetch<TAIL>(cv, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; });
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    TL::put(ck, lds + buf * 2 * TL::BYTES);
+    TL::put(cv, lds + buf * 2 * TL::BYTES + TL::BYTES);
+  };
+  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+    const unsigned char *const ldsK = lds + buf * 2 * TL::BYTES, *const ldsV = ldsK + TL::BYTES;
+    const bool edge_tile = t * ROWS + ROWS - 1 > span.all;
+    f32x16 s[ROWS / 32];
+#pragma unroll
+    for (int u = 0; u < ROWS / 32; ++u) {
+      s[u] = zero16();
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x) s[u] = mma(TL::along(ldsK + u * 32 * TL::RB, lo, x), q[x], s[u]);
     }
+    if (edge_tile) {
 #pragma unroll
-    for (int sub = 0; sub < ROWS; sub += 32) {
-      const int kb = key0 + sub;
-      if (kb > some_see) break;
-      f32x16 s = zero16();
+      for (int u = 0; u < ROWS / 32; ++u) {
+        const int rel = r.lim - (t * ROWS + u * 32) - 4 * h;
 #pragma unroll
-      for (int t = 0; t < DP / 16; ++t) s = mma(TL::along(ldsK + sub * TL::RB, lo, t), q[t], s);
-      const bool edge = kb + 31 > all_see;
-      if (edge) {
-        const int rel = r.lim - kb - 4 * h;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 <= rel ? s[i] : -INFINITY;
+        for (int i = 0; i < 16; ++i) s[u][i] = 8 * (i / 4) + i % 4 <= rel ? s[u][i] : -INFINITY;
       }
-      float top = s[0];
+    }
+    float top = s[0][0];
 #pragma unroll
-      for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
-      top *= a.scale2;
-      if (__any(top > m + LAZY)) {
-        const float m_new = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
-        const float f = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
-        m = m_new;
-        l *= f;
+    for (int u = 0; u < ROWS / 32; ++u)
 #pragma unroll
-        for (int db = 0; db < DP / 32; ++db)
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
+    top *= a.scale2;
+    if (__any(top > m + LAZY)) {
+      const float m_new = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
+      const float f = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
+      m = m_new;
+      l *= f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) acc[db][i] *= f;
-      }
-      const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: every weight is 0
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int db = 0; db < DP / 32; ++db)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] *= f;
+    }
+    const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: every weight is 0
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < ROWS / 32; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale2 - base);
-        sum[i & 3] += s[i];
+        s[u][i] = __builtin_amdgcn_exp2f(s[u][i] * a.scale2 - base);
+        sum[i & 3] += s[u][i];
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      const unsigned char *const v32 = ldsV + sub * TL::RB;
-      if (edge && TL::not_finite(v32, lo))
-        TL::add_careful(acc, v32, lo, s, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
-      else
-        TL::add(acc, v32, lo, s);
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+#pragma unroll
+    for (int u = 0; u < ROWS / 32; ++u) {
+      const int kb = t * ROWS + u * 32;
+      TL::add(acc, ldsV + u * 32 * TL::RB, zeros, lo, s[u], edge_tile && kb + 31 > span.wave_all,
+              [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
-  }
+  };
+  stream((span.kend + ROWS - 1) / ROWS, fetch, put, step);
   l += __shfl_xor(l, 32, 64);
   if (!r.live) return;
   const float f = r.lim < 0 ? 0.f : 1.f / l;
@@ -437,21 +487,23 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(
   if (a.lse && h == 0)
     a.lse[(i64)(r.s.q0 + r.query) * a.Hq + r.head] = r.lim < 0 ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
-
 // dQ, and delta for the kernel below.
-template <typename T, int DP>
+template <typename T, int DP, bool TAIL>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(const Args<T> a) {
-  typedef Tile<T, DP> TL;
-  __shared__ __align__(16) unsigned char lds[2 * TL::BYTES];
-  unsigned char *const ldsK = lds, *const ldsV = lds + TL::BYTES;
+  constexpr int ROWS = tile_rows<T, DP>();
+  typedef Tile<T, DP, ROWS> TL;
+  __shared__ __align__(16) unsigned char lds[4 * TL::BYTES + TL::ZEROS];
+  unsigned char *const zeros = lds + 4 * TL::BYTES;
   const int kvh = blockIdx.x % a.Hkv;
   const int t0 = blockIdx.x / a.Hkv;
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;
   Rows r;
   int row0;
   if (!rows_of(a, tile, kvh, r, row0)) return;
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
+  TL::clear(zeros);
+  const int lane = threadIdx.x & 63, h = lane >> 5;
   const auto lo = TL::lane_offsets(lane);
+  const Span span = span_of(a, r, row0);
 
   Frag<T> q[DP / 16], dout[DP / 16];
   float delta = 0.f;
@@ -471,74 +523,77 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
     delta += __shfl_xor(delta, 32, 64);
   }
   const i64 at = (i64)(r.s.q0 + r.query) * a.Hq + r.head;
-  float lse2 = INFINITY;  // a row that does not exist has no weight anywhere
-  if (r.live) {
-    lse2 = a.lse[at] * LOG2E;
-    if (h == 0) a.delta[at] = delta;
-  }
-  const int last = min(row0 + BM, r.nrows) - 1;
-  const int kend = a.causal ? min(max(div_by(last, a.G) + r.off + 1, 0), r.s.nk) : r.s.nk;
-  const int wfirst = min(row0 + wave * COLS, r.nrows - 1), wlast = min(row0 + wave * COLS + COLS, r.nrows) - 1;
-  const int all_see = a.causal ? min(div_by(wfirst, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
-  const int some_see = a.causal ? min(div_by(wlast, a.G) + r.off, r.s.nk - 1) : r.s.nk - 1;
+  const float lse2 = r.live ? a.lse[at] * LOG2E : INFINITY;  // a row that does not exist has no weight anywhere
 
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
   const T *const kp = a.k + (i64)r.s.k0 * a.k_ld + kvh * a.D, *const vp = a.v + (i64)r.s.k0 * a.v_ld + kvh * a.D;
-  auto k_row = [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; };
-  auto v_row = [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; };
   typename TL::Chunks ck, cv;
-  TL::fetch(ck, 0, kend, a.D, k_row);
-  TL::fetch(cv, 0, kend, a.D, v_row);
-  for (int key0 = 0; key0 < kend; key0 += ROWS) {
-    __syncthreads();
-    TL::put(ck, ldsK);
-    TL::put(cv, ldsV);
-    __syncthreads();
-    if (key0 + ROWS < kend) {
-      TL::fetch(ck, key0 + ROWS, kend, a.D, k_row);
-      TL::fetch(cv, key0 + ROWS, kend, a.D, v_row);
-    }
-#pragma unroll
-    for (int sub = 0; sub < ROWS; sub += 32) {
-      const int kb = key0 + sub;
-      if (kb > some_see) break;
-      const unsigned char *const k32 = ldsK + sub * TL::RB;
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    TL::template fetch<TAIL>(ck, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; });
+    TL::template fetch<TAIL>(cv, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; });
+  };
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    TL::put(ck, lds + buf * 2 * TL::BYTES);
+    TL::put(cv, lds + buf * 2 * TL::BYTES + TL::BYTES);
+  };
+  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+    const unsigned char *const ldsK = lds + buf * 2 * TL::BYTES, *const ldsV = ldsK + TL::BYTES;
+#pragma unroll 1
+    for (int u = 0; u < ROWS / 32; ++u) {
+      const int kb = t * ROWS + u * 32;
+      if (kb > span.wave_some) break;
+      const unsigned char *const k32 = ldsK + u * 32 * TL::RB, *const v32 = ldsV + u * 32 * TL::RB;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int t = 0; t < DP / 16; ++t) {
-        s = mma(TL::along(k32, lo, t), q[t], s);
-        dp = mma(TL::along(ldsV + sub * TL::RB, lo, t), dout[t], dp);
-      }
+      for (int x = 0; x < DP / 16; ++x) s = mma(TL::along(k32, lo, x), q[x], s);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale2 - lse2) * (dp[i] - delta);
-      const bool edge = kb + 31 > all_see;
+      for (int x = 0; x < DP / 16; ++x) dp = mma(TL::along(v32, lo, x), dout[x], dp);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale2 - lse2);
+      const bool edge = kb + 31 > span.wave_all;
       if (edge) {
         const int rel = r.lim - kb - 4 * h;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[i] = 8 * (i / 4) + i % 4 <= rel ? s[i] : 0.f;
+        for (int i = 0; i < 16; ++i) {
+          s[i] = 8 * (i / 4) + i % 4 <= rel ? s[i] : 0.f;
+          dp[i] = 8 * (i / 4) + i % 4 <= rel ? dp[i] : 0.f;
+        }
+        if (kb == 0) {
+          // A query whose keys all lie here has its delta from the weights themselves: dout * out takes out as it was
+          // stored, rounded, and with few keys, where out is large, that would be the largest error of dS.
+          float d = 0.f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) d += s[i] * dp[i];
+          d += __shfl_xor(d, 32, 64);
+          delta = r.lim < 32 ? d : delta;
+        }
       }
-      if (edge && TL::not_finite(k32, lo))
-        TL::add_careful(acc, k32, lo, s, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
-      else
-        TL::add(acc, k32, lo, s);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
+      TL::add(acc, k32, zeros, lo, s, edge, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
-  }
-  if (r.live) store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale);
+  };
+  stream((span.kend + ROWS - 1) / ROWS, fetch, put, step);
+  if (!r.live) return;
+  if (h == 0) a.delta[at] = delta;
+  store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale);
 }
 
 // dK and dV: keys in registers, the packed queries of the group streamed.
-template <typename T, int DP>
+template <typename T, int DP, bool TAIL>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(const Args<T> a) {
-  typedef Tile<T, DP> TL;
-  __shared__ __align__(16) unsigned char lds[2 * TL::BYTES + 2 * ROWS * 4];
-  unsigned char *const ldsQ = lds, *const ldsD = lds + TL::BYTES;
-  float *const ldsL = reinterpret_cast<float *>(lds + 2 * TL::BYTES), *const ldsDelta = ldsL + ROWS;
+  constexpr int ROWS = tile_rows<T, DP>();
+  typedef Tile<T, DP, ROWS> TL;
+  constexpr int STAGE = 2 * TL::BYTES + 2 * ROWS * 4;  // Q, dout, lse (base 2), delta
+  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS];
+  unsigned char *const zeros = lds + 2 * STAGE;
   const int kvh = blockIdx.x % a.Hkv;
   const Where w = find_tile<BM>(a.cu_k, a.num_seqs, a.total_k, 1, blockIdx.x / a.Hkv);
   const Seq s = seq_of(a, w.seq);
   if (w.row0 < 0 || w.row0 >= s.nk) return;
+  TL::clear(zeros);
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
   const auto lo = TL::lane_offsets(lane);
   const int g = (int)a.G.by, nrows = s.nq * g, off = s.nk - s.nq;
@@ -560,19 +615,21 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = zero16();
 
-  // the first query that sees the workgroup's first key
+  // the rows that see a key: from the first query that sees the first key of the workgroup / the last one of the wavefront
   const int first = a.causal ? min(max(w.row0 - off, 0), s.nq) * g : 0;
+  const int wave_some = a.causal ? min(max(wkey - off, 0), s.nq) * g : 0;      // rows before it see none of the wavefront's keys
+  const int wave_all = a.causal ? min(max(wkey + 31 - off, 0), s.nq) * g : 0;  // rows from it on see all of them
+  const int lim = a.causal ? min(max(key - off, 0), s.nq) * g : 0;             // rows from it on see the lane's key
   auto row_of = [&](const T *base, i64 ld, int r) __attribute__((always_inline)) {
     const int query = div_by(r, a.G);
     return base + (i64)(s.q0 + query) * ld + (kvh * g + (r - query * g)) * a.D;
   };
-  auto q_row = [&](int r) __attribute__((always_inline)) { return row_of(a.q, a.q_ld, r); };
-  auto d_row = [&](int r) __attribute__((always_inline)) { return row_of(a.dout, a.dout_ld, r); };
   typename TL::Chunks cq, cd;
   float fl, fd;
-  auto fetch_all = [&](int r0) __attribute__((always_inline)) {
-    TL::fetch(cq, r0, nrows, a.D, q_row);
-    TL::fetch(cd, r0, nrows, a.D, d_row);
+  auto fetch = [&](int t) __attribute__((always_inline)) {
+    const int r0 = first + t * ROWS;
+    TL::template fetch<TAIL>(cq, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.q, a.q_ld, r); });
+    TL::template fetch<TAIL>(cd, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.dout, a.dout_ld, r); });
     fl = INFINITY, fd = 0.f;  // rows that do not exist have no weight
     const int r = r0 + (int)threadIdx.x;
     if (threadIdx.x < ROWS && r < nrows) {
@@ -582,58 +639,55 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
       fd = a.delta[at];
     }
   };
-  fetch_all(first);
-  for (int r0 = first; r0 < nrows; r0 += ROWS) {
-    __syncthreads();
-    TL::put(cq, ldsQ);
-    TL::put(cd, ldsD);
+  auto put = [&](int buf) __attribute__((always_inline)) {
+    unsigned char *const st = lds + buf * STAGE;
+    TL::put(cq, st);
+    TL::put(cd, st + TL::BYTES);
     if (threadIdx.x < ROWS) {
-      ldsL[threadIdx.x] = fl;
-      ldsDelta[threadIdx.x] = fd;
+      float *const f = reinterpret_cast<float *>(st + 2 * TL::BYTES) + threadIdx.x;
+      f[0] = fl;
+      f[ROWS] = fd;
     }
-    __syncthreads();
-    if (r0 + ROWS < nrows) fetch_all(r0 + ROWS);
-#pragma unroll
-    for (int sub = 0; sub < ROWS; sub += 32) {
-      const int rb = r0 + sub;
+  };
+  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+    const unsigned char *const ldsQ = lds + buf * STAGE, *const ldsD = ldsQ + TL::BYTES;
+    const float *const ldsL = reinterpret_cast<const float *>(ldsD + TL::BYTES), *const ldsDelta = ldsL + ROWS;
+#pragma unroll 1
+    for (int u = 0; u < ROWS / 32; ++u) {
+      const int rb = first + t * ROWS + u * 32;
       if (rb >= nrows) break;
-      if (a.causal && div_by(min(rb + 31, nrows - 1), a.G) + off < wkey) continue;  // no row sees the wavefront's keys
-      const unsigned char *const q32 = ldsQ + sub * TL::RB, *const d32 = ldsD + sub * TL::RB;
+      if (rb + 31 < wave_some) continue;
+      const unsigned char *const q32 = ldsQ + u * 32 * TL::RB, *const d32 = ldsD + u * 32 * TL::RB;
       f32x16 p = zero16(), ds = zero16();
 #pragma unroll
-      for (int t = 0; t < DP / 16; ++t) {
-        p = mma(TL::along(q32, lo, t), k[t], p);
-        ds = mma(TL::along(d32, lo, t), v[t], ds);
-      }
+      for (int x = 0; x < DP / 16; ++x) p = mma(TL::along(q32, lo, x), k[x], p);
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x) ds = mma(TL::along(d32, lo, x), v[x], ds);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
-        const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(ldsL + sub + 8 * b + 4 * h);
-        const f32x4 delta = *reinterpret_cast<const f32x4 *>(ldsDelta + sub + 8 * b + 4 * h);
+        const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(ldsL + u * 32 + 8 * b + 4 * h);
+        const f32x4 delta = *reinterpret_cast<const f32x4 *>(ldsDelta + u * 32 + 8 * b + 4 * h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           p[4 * b + i] = __builtin_amdgcn_exp2f(p[4 * b + i] * a.scale2 - lse2[i]);
           ds[4 * b + i] = p[4 * b + i] * (ds[4 * b + i] - delta[i]);
         }
       }
-      const bool edge = a.causal && div_by(rb, a.G) + off < wkey + 31;
+      const bool edge = rb < wave_all;
       if (edge) {
+        const int rel = lim - rb - 4 * h;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const bool sees = div_by(rb + 8 * (i / 4) + 4 * h + i % 4, a.G) + off >= key;
-          p[i] = sees ? p[i] : 0.f;
-          ds[i] = sees ? ds[i] : 0.f;
+          p[i] = 8 * (i / 4) + i % 4 >= rel ? p[i] : 0.f;
+          ds[i] = 8 * (i / 4) + i % 4 >= rel ? ds[i] : 0.f;
         }
       }
-      if (edge && (TL::not_finite(q32, lo) || TL::not_finite(d32, lo))) {
-        auto sees = [&](int i) __attribute__((always_inline)) { return div_by(rb + i, a.G) + off >= key; };
-        TL::add_careful(dv, d32, lo, p, sees);
-        TL::add_careful(dk, q32, lo, ds, sees);
-      } else {
-        TL::add(dv, d32, lo, p);
-        TL::add(dk, q32, lo, ds);
-      }
+      auto sees = [&](int i) __attribute__((always_inline)) { return rb + i >= lim; };
+      TL::add(dv, d32, zeros, lo, p, edge, sees);
+      TL::add(dk, q32, zeros, lo, ds, edge, sees);
     }
-  }
+  };
+  stream((nrows - first + ROWS - 1) / ROWS, fetch, put, step);
   if (!live) return;
   store_column<T, DP>(a.dk + (i64)(s.k0 + key) * a.dk_ld + kvh * a.D, a.D, dk, a.scale);
   store_column<T, DP>(a.dv + (i64)(s.k0 + key) * a.dv_ld + kvh * a.D, a.D, dv, 1.f);
@@ -689,12 +743,17 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
   return UNET_OK;
 }
 
-// f(DP) with the head dimension padded to the tile's.
-template <typename F>
+// f(DP, TAIL) with the head dimension padded to the tile's, and whether a row ends inside a 16-byte chunk.
+template <typename T, typename F>
 void with_dim(int D, F f) {
-  if (D <= 32) f(std::integral_constant<int, 32>());
-  else if (D <= 64) f(std::integral_constant<int, 64>());
-  else f(std::integral_constant<int, 128>());
+  const bool tail = D * sizeof(T) % 16 != 0;
+  auto padded = [&](auto dp) {
+    if (tail) f(dp, std::true_type());
+    else f(dp, std::false_type());
+  };
+  if (D <= 32) padded(std::integral_constant<int, 32>());
+  else if (D <= 64) padded(std::integral_constant<int, 64>());
+  else padded(std::integral_constant<int, 128>());
 }
 
 template <typename T>
@@ -709,7 +768,9 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   if (num_seqs == 0 || total_q == 0) return UNET_OK;
   a.out = out, a.out_ld = out_ld, a.lse = lse;
   a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
-  with_dim(D, [&](auto dp) { attention_kernel<T, decltype(dp)::value><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a); });
+  with_dim<T>(D, [&](auto dp, auto tail) {
+    attention_kernel<T, decltype(dp)::value, decltype(tail)::value><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
+  });
   UNET_LAUNCH_CHECK(name);
   return UNET_OK;
 }
@@ -737,10 +798,11 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   a.dout_ld = dout_ld, a.o_ld = out_ld, a.dq_ld = dq_ld, a.dk_ld = dk_ld, a.dv_ld = dv_ld;
   a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   const unsigned key_tiles = (unsigned)(total_k / BM) + num_seqs;
-  with_dim(D, [&](auto dp) {
+  with_dim<T>(D, [&](auto dp, auto tail) {
     constexpr int DP = decltype(dp)::value;
-    if (total_q) attention_dq_kernel<T, DP><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
-    if (total_k) attention_dkv_kernel<T, DP><<<key_tiles * Hkv, 256, 0, st>>>(a);
+    constexpr bool TAIL = decltype(tail)::value;
+    if (total_q) attention_dq_kernel<T, DP, TAIL><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
+    if (total_k) attention_dkv_kernel<T, DP, TAIL><<<key_tiles * Hkv, 256, 0, st>>>(a);
   });
   UNET_LAUNCH_CHECK(name);
   return UNET_OK;
