@@ -90,9 +90,9 @@ struct Args {
   const T *q, *k, *v, *o, *dout;
   T *out, *dq, *dk, *dv;
   i64 q_ld, k_ld, v_ld, o_ld, dout_ld, out_ld, dq_ld, dk_ld, dv_ld;
-  float *lse, *delta;
+  float *lse, *delta, *partials;
   const int *cu_q, *cu_k;
-  int num_seqs, total_q, total_k, Hq, Hkv, D, causal, tiles;
+  int num_seqs, total_q, total_k, Hq, Hkv, D, causal, tiles, splits;
   Div G;
   float scale, scale2;  // scale * log2(e)
 };
@@ -587,20 +587,25 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
   constexpr int ROWS = tile_rows<T, DP>();
   typedef Tile<T, DP, ROWS> TL;
   constexpr int STAGE = 2 * TL::BYTES + 2 * ROWS * 4;  // Q, dout, lse (base 2), delta
-  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS];
+  // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands stay in
+  // LDS, each wavefront's own, in the order in which the lanes read them.
+  constexpr bool V_LDS = DP == 128;
+  constexpr int V_BYTES = V_LDS ? BM * TL::RB : 0;
+  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS + V_BYTES];
   unsigned char *const zeros = lds + 2 * STAGE;
-  const int kvh = blockIdx.x % a.Hkv;
-  const Where w = find_tile<BM>(a.cu_k, a.num_seqs, a.total_k, 1, blockIdx.x / a.Hkv);
+  const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits;
+  const Where w = find_tile<BM>(a.cu_k, a.num_seqs, a.total_k, 1, bs / a.splits);
   const Seq s = seq_of(a, w.seq);
   if (w.row0 < 0 || w.row0 >= s.nk) return;
   TL::clear(zeros);
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
   const auto lo = TL::lane_offsets(lane);
-  const int g = (int)a.G.by, nrows = s.nq * g, off = s.nk - s.nq;
+  const int g = (int)a.G.by, off = s.nk - s.nq;
   const int wkey = w.row0 + wave * COLS, key = wkey + (lane & 31);
   const bool live = key < s.nk;
 
-  Frag<T> k[DP / 16], v[DP / 16];
+  Frag<T> k[DP / 16], vr[V_LDS ? 1 : DP / 16];
+  Frag<T> *const vl = reinterpret_cast<Frag<T> *>(lds + 2 * STAGE + TL::ZEROS + wave * (V_BYTES / WAVES)) + lane;
   {
     const i64 token = s.k0 + min(key, s.nk - 1);
     const T *pk = a.k + token * a.k_ld + kvh * a.D, *pv = a.v + token * a.v_ld + kvh * a.D;
@@ -608,7 +613,8 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
     for (int t = 0; t < DP / 16; ++t) {
       const int e = 16 * t + 8 * h, n = live ? a.D - e : 0;
       k[t] = load_frag<T>(pk + e, n);
-      v[t] = load_frag<T>(pv + e, n);
+      if constexpr (V_LDS) vl[64 * t] = load_frag<T>(pv + e, n);
+      else vr[t] = load_frag<T>(pv + e, n);
     }
   }
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -616,7 +622,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
   for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = zero16();
 
   // the rows that see a key: from the first query that sees the first key of the workgroup / the last one of the wavefront
-  const int first = a.causal ? min(max(w.row0 - off, 0), s.nq) * g : 0;
+  int first = a.causal ? min(max(w.row0 - off, 0), s.nq) * g : 0, nrows = s.nq * g;
+  if (a.splits > 1) {  // this workgroup's share of them
+    const int per = (((nrows - first + ROWS - 1) / ROWS + a.splits - 1) / a.splits) * ROWS;
+    first = (int)min((i64)nrows, first + (i64)split * per);
+    nrows = (int)min((i64)nrows, (i64)first + per);
+  }
   const int wave_some = a.causal ? min(max(wkey - off, 0), s.nq) * g : 0;      // rows before it see none of the wavefront's keys
   const int wave_all = a.causal ? min(max(wkey + 31 - off, 0), s.nq) * g : 0;  // rows from it on see all of them
   const int lim = a.causal ? min(max(key - off, 0), s.nq) * g : 0;             // rows from it on see the lane's key
@@ -662,7 +673,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
 #pragma unroll
       for (int x = 0; x < DP / 16; ++x) p = mma(TL::along(q32, lo, x), k[x], p);
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) ds = mma(TL::along(d32, lo, x), v[x], ds);
+      for (int x = 0; x < DP / 16; ++x) {
+        if constexpr (V_LDS) ds = mma(TL::along(d32, lo, x), vl[64 * x], ds);
+        else ds = mma(TL::along(d32, lo, x), vr[x], ds);
+      }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(ldsL + u * 32 + 8 * b + 4 * h);
@@ -689,8 +703,32 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
   };
   stream((nrows - first + ROWS - 1) / ROWS, fetch, put, step);
   if (!live) return;
+  if (a.splits > 1) {
+    const i64 at = ((i64)(s.k0 + key) * a.Hkv + kvh) * a.D, plane = (i64)a.total_k * a.Hkv * a.D;
+    store_column<float, DP>(a.partials + (2 * split) * plane + at, a.D, dk, a.scale);
+    store_column<float, DP>(a.partials + (2 * split + 1) * plane + at, a.D, dv, 1.f);
+    return;
+  }
   store_column<T, DP>(a.dk + (i64)(s.k0 + key) * a.dk_ld + kvh * a.D, a.D, dk, a.scale);
   store_column<T, DP>(a.dv + (i64)(s.k0 + key) * a.dv_ld + kvh * a.D, a.D, dv, 1.f);
+}
+
+// dK and dV from the partial sums of attention_dkv_kernel, in the order of the splits.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_dkv_join_kernel(const Args<T> a) {
+  const int k0 = bound_of(a.cu_k, 0, a.total_k), k1 = max(bound_of(a.cu_k, a.num_seqs, a.total_k), k0);
+  const int cols = a.Hkv * a.D;
+  const i64 plane = (i64)a.total_k * cols, end = (i64)k1 * cols;
+  for (i64 i = (i64)k0 * cols + (i64)blockIdx.x * 256 + threadIdx.x; i < end; i += (i64)gridDim.x * 256) {
+    float dk = 0.f, dv = 0.f;
+    for (int s = 0; s < a.splits; ++s) {
+      dk += a.partials[2 * s * plane + i];
+      dv += a.partials[(2 * s + 1) * plane + i];
+    }
+    const i64 key = i / cols, c = i - key * cols;
+    from_f32(dk, a.dk[key * a.dk_ld + c]);
+    from_f32(dv, a.dv[key * a.dv_ld + c]);
+  }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
@@ -742,6 +780,17 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
   a.scale = scale, a.scale2 = scale * LOG2E;
   return UNET_OK;
 }
+
+// Row ranges into which the dK/dV kernel's sums are split when there are few key tiles: workgroups of very different
+// lengths (causal) fill 256 CUs evenly once there are several times 512 of them (two fit a CU).  Each range costs a
+// pass over fp32 dK and dV, so it should have 512 rows at least on the average.
+int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv) {
+  const i64 tiles = (total_k / BM + num_seqs) * Hkv, rows = num_seqs ? total_q * (Hq / Hkv) / num_seqs : 0;
+  i64 s = tiles > 0 ? 1024 / tiles : 1;
+  if (s > rows / 512) s = rows / 512;
+  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
+size_t delta_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * sizeof(float) + 15) / 16 * 16; }
 
 // f(DP, TAIL) with the head dimension padded to the tile's, and whether a row ends inside a 16-byte chunk.
 template <typename T, typename F>
@@ -798,12 +847,15 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   a.dout_ld = dout_ld, a.o_ld = out_ld, a.dq_ld = dq_ld, a.dk_ld = dk_ld, a.dv_ld = dv_ld;
   a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   const unsigned key_tiles = (unsigned)(total_k / BM) + num_seqs;
+  a.splits = dkv_splits(num_seqs, total_q, total_k, Hq, Hkv);
+  a.partials = (float *)((char *)ws + delta_bytes(total_q, Hq));
   with_dim<T>(D, [&](auto dp, auto tail) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool TAIL = decltype(tail)::value;
     if (total_q) attention_dq_kernel<T, DP, TAIL><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
-    if (total_k) attention_dkv_kernel<T, DP, TAIL><<<key_tiles * Hkv, 256, 0, st>>>(a);
+    if (total_k) attention_dkv_kernel<T, DP, TAIL><<<key_tiles * Hkv * a.splits, 256, 0, st>>>(a);
   });
+  if (total_k && a.splits > 1) attention_dkv_join_kernel<T><<<ew_grid(total_k * Hkv * D), 256, 0, st>>>(a);
   UNET_LAUNCH_CHECK(name);
   return UNET_OK;
 }
@@ -823,7 +875,9 @@ int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, i
                                                 int heads_kv, int head_dim, size_t *bytes_host) {
   UNET_REQUIRE(bytes_host, "dot_attention_backward_workspace_bytes: NULL result");
   TRY(check_shape("dot_attention_backward_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  *bytes_host = (size_t)total_q * heads_q * sizeof(float);  // delta
+  const int splits = dkv_splits(num_seqs, total_q, total_k, heads_q, heads_kv);
+  *bytes_host = delta_bytes(total_q, heads_q) +
+                (splits > 1 ? (size_t)splits * 2 * total_k * heads_kv * head_dim * sizeof(float) : 0);
   return UNET_OK;
 }
 
