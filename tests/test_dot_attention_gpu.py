@@ -121,6 +121,39 @@ def test_against_the_definition(name, causal, pad, behind, shape):
         assert torch.equal(a, b)  # equal calls, equal bits
 
 
+# long key sequences and few queries: the keys are split over workgroups and joined; and row counts for which the
+# gradient of the keys is summed in parts
+SPLIT = [([1, 1], [2500, 4100], 8, 1, 128), ([3, 0, 1], [5000, 600, 10], 6, 2, 40), ([5], [1999], 2, 2, 64), ([700, 1, 1300], [700, 1, 1300], 4, 1, 64),
+         ([1100], [1500], 2, 1, 104), ([40], [20], 32, 1, 16), ([2, 300], [9000, 3], 3, 3, 32)]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("shape", SPLIT, ids=lambda s: "x".join(map(str, [max(s[0]), max(s[1]), *s[2:]])))
+def test_split_sums(name, causal, shape):
+    c = Call(name, *shape, causal, pad=1, behind=3)
+    c.forward()
+    c.backward()
+    c.verify()
+    first = [t.clone() for t in (c.out, c.lse, c.dq, c.dk, c.dv)]
+    c.forward()
+    c.backward()
+    for a, b in zip(first, (c.out, c.lse, c.dq, c.dk, c.dv)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
+def test_split_sums_keep_bad_keys_to_the_queries_that_see_them(bad):
+    c = Call("bf16", [2, 1], [4000, 3500], 4, 2, 64, True)
+    val, bnd = c.exact()
+    c.k[3999] = bad  # seen by the second query alone
+    c.v[3999] = bad
+    c.forward()
+    for n in ("out", "lse"):
+        seq_ref.check(getattr(c, n)[[0, 2]], val[n][[0, 2]], bnd[n][[0, 2]], n)
+    assert not torch.isfinite(c.out[1].float()).any()
+
+
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 def test_large_scores(name):
     """Scores of several hundred: the running maximum moves often, most weights underflow."""

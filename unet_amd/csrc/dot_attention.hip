@@ -311,15 +311,17 @@ __device__ __forceinline__ void store4(T *p, int n, float a, float b, float c, f
 }
 // acc[d][column] * f -> p[d] of the lane's column
 template <typename T, int DP>
-__device__ __forceinline__ void store_column(T *p, int D, const f32x16 (&acc)[DP / 32], float f) {
+__device__ __forceinline__ void store_column(T *p, int D, const f32x16 (&acc)[DP / 32], float f, int db0 = 0,
+                                             int db1 = DP / 32) {
   const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db)
+    if (db >= db0 && db < db1)
 #pragma unroll
-    for (int b = 0; b < 4; ++b) {
-      const int d = 32 * db + 8 * b + 4 * h;
-      store4(p + d, D - d, acc[db][4 * b] * f, acc[db][4 * b + 1] * f, acc[db][4 * b + 2] * f, acc[db][4 * b + 3] * f);
-    }
+      for (int b = 0; b < 4; ++b) {
+        const int d = 32 * db + 8 * b + 4 * h;
+        store4(p + d, D - d, acc[db][4 * b] * f, acc[db][4 * b + 1] * f, acc[db][4 * b + 2] * f, acc[db][4 * b + 3] * f);
+      }
 }
 
 // The queries of a workgroup: what the forward and the dQ kernel share.
@@ -328,16 +330,16 @@ struct Rows {
   int nrows, off, row, query, head, lim;  // lim: last visible key of the lane's query, negative: none
   bool live;
 };
-template <typename T>
-__device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, Rows &r, int &row0) {
+template <int BQ, typename T>
+__device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int wave, Rows &r, int &row0) {
   const int g = (int)a.G.by;
-  const Where w = find_tile<BM>(a.cu_q, a.num_seqs, a.total_q, g, tile);
+  const Where w = find_tile<BQ>(a.cu_q, a.num_seqs, a.total_q, g, tile);
   r.s = seq_of(a, w.seq);
   r.nrows = r.s.nq * g;
   row0 = w.row0;
   if (row0 < 0 || row0 >= r.nrows) return false;
   r.off = r.s.nk - r.s.nq;
-  r.row = row0 + (threadIdx.x >> 6) * COLS + (threadIdx.x & 31);
+  r.row = row0 + wave * COLS + (threadIdx.x & 31);
   r.live = r.row < r.nrows;
   const int rr = min(r.row, r.nrows - 1);
   r.query = div_by(rr, a.G);
@@ -377,35 +379,39 @@ struct Span {
   int all;                  // keys [0, all] by every query of the workgroup
   int wave_all, wave_some;  // keys [0, wave_all] by every, [0, wave_some] by some query of the wavefront
 };
-template <typename T>
-__device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row0) {
-  const int wave = threadIdx.x >> 6, last = r.s.nk - 1;
+template <int BQ, typename T>
+__device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row0, int wave) {
+  const int last = r.s.nk - 1;
   if (!a.causal) return Span{r.s.nk, last, last, last};
   auto sees = [&](int row) __attribute__((always_inline)) { return min(div_by(min(row, r.nrows - 1), a.G) + r.off, last); };
   Span s;
-  s.kend = max(sees(row0 + BM - 1) + 1, 0);
+  s.kend = max(sees(row0 + BQ - 1) + 1, 0);
   s.all = sees(row0);
   s.wave_all = sees(row0 + wave * COLS);
   s.wave_some = row0 + wave * COLS < r.nrows ? sees(row0 + wave * COLS + COLS - 1) : -1;
   return s;
 }
 
-template <typename T, int DP, bool TAIL>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(const Args<T> a) {
-  constexpr int ROWS = 64;
+// The forward.  WK wavefronts share the same 32 queries and take the 32-row pieces of a tile in turn: with WK = 1 a
+// workgroup has 128 queries (every tile serves four times 32), with WK > 1 it has fewer, for calls that have too few
+// queries to fill the GPU.  splits > 1: the workgroup takes a share of the key tiles and leaves its sums to
+// attention_join_kernel.
+template <typename T, int DP, bool TAIL, int WK>
+__global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 1) void attention_kernel(const Args<T> a) {
+  constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS> TL;
-  __shared__ __align__(16) unsigned char lds[4 * TL::BYTES + TL::ZEROS];
-  unsigned char *const zeros = lds + 4 * TL::BYTES;
-  const int kvh = blockIdx.x % a.Hkv;
-  const int t0 = blockIdx.x / a.Hkv;
+  constexpr int STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
+  __shared__ __align__(16) unsigned char lds[(2 * STAGE > MERGE ? 2 * STAGE : MERGE) + TL::ZEROS];
+  unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ;
+  const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits, t0 = bs / a.splits;
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;  // the queries with the most keys first
   Rows r;
   int row0;
-  if (!rows_of(a, tile, kvh, r, row0)) return;
+  if (!rows_of<BQ>(a, tile, kvh, wq, r, row0)) return;
   TL::clear(zeros);
-  const int lane = threadIdx.x & 63, h = lane >> 5;
   const auto lo = TL::lane_offsets(lane);
-  const Span span = span_of(a, r, row0);
+  const Span span = span_of<BQ>(a, r, row0, wq);
 
   Frag<T> q[DP / 16];
   {
@@ -413,42 +419,51 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) q[t] = load_frag<T>(p + 16 * t + 8 * h, r.live ? a.D - 16 * t - 8 * h : 0);
   }
-  f32x16 acc[DP / 32];
+  f32x16 acc[DB];
 #pragma unroll
-  for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
+  for (int db = 0; db < DB; ++db) acc[db] = zero16();
   float m = -INFINITY, l = 0.f;  // of the scores times scale2 (base 2); l over this lane's rows only
 
+  int first = 0, n = (span.kend + ROWS - 1) / ROWS;  // key tiles
+  if (a.splits > 1) {
+    const int per = (n + a.splits - 1) / a.splits;
+    first = min(split * per, n);
+    n = min(per, n - first);
+  }
   const T *const kp = a.k + (i64)r.s.k0 * a.k_ld + kvh * a.D, *const vp = a.v + (i64)r.s.k0 * a.v_ld + kvh * a.D;
   typename TL::Chunks ck, cv;
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    TL::template fetch<TAIL>(ck, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; });
-    TL::template fetch<TAIL>(cv, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; });
+    const int end = min(span.kend, (first + n) * ROWS);
+    TL::template fetch<TAIL>(ck, (first + t) * ROWS, end, a.D, [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; });
+    TL::template fetch<TAIL>(cv, (first + t) * ROWS, end, a.D, [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; });
   };
   auto put = [&](int buf) __attribute__((always_inline)) {
-    TL::put(ck, lds + buf * 2 * TL::BYTES);
-    TL::put(cv, lds + buf * 2 * TL::BYTES + TL::BYTES);
+    TL::put(ck, lds + buf * STAGE);
+    TL::put(cv, lds + buf * STAGE + TL::BYTES);
   };
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
-    const unsigned char *const ldsK = lds + buf * 2 * TL::BYTES, *const ldsV = ldsK + TL::BYTES;
-    const bool edge_tile = t * ROWS + ROWS - 1 > span.all;
-    f32x16 s[ROWS / 32];
+    const int key0 = (first + t) * ROWS + wk * 32;
+    if (key0 > span.wave_some) return;
+    const unsigned char *const ldsK = lds + buf * STAGE + wk * 32 * TL::RB, *const ldsV = ldsK + TL::BYTES;
+    const bool edge = key0 + NU * 32 - 1 > span.wave_all;
+    f32x16 s[NU];
 #pragma unroll
-    for (int u = 0; u < ROWS / 32; ++u) {
+    for (int u = 0; u < NU; ++u) {
       s[u] = zero16();
 #pragma unroll
       for (int x = 0; x < DP / 16; ++x) s[u] = mma(TL::along(ldsK + u * 32 * TL::RB, lo, x), q[x], s[u]);
     }
-    if (edge_tile) {
+    if (edge) {
 #pragma unroll
-      for (int u = 0; u < ROWS / 32; ++u) {
-        const int rel = r.lim - (t * ROWS + u * 32) - 4 * h;
+      for (int u = 0; u < NU; ++u) {
+        const int rel = r.lim - (key0 + u * 32) - 4 * h;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s[u][i] = 8 * (i / 4) + i % 4 <= rel ? s[u][i] : -INFINITY;
       }
     }
     float top = s[0][0];
 #pragma unroll
-    for (int u = 0; u < ROWS / 32; ++u)
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
     top *= a.scale2;
@@ -458,14 +473,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(
       m = m_new;
       l *= f;
 #pragma unroll
-      for (int db = 0; db < DP / 32; ++db)
+      for (int db = 0; db < DB; ++db)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[db][i] *= f;
     }
     const float base = m == -INFINITY ? 0.f : m;  // nothing but -inf so far: every weight is 0
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int u = 0; u < ROWS / 32; ++u)
+    for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         s[u][i] = __builtin_amdgcn_exp2f(s[u][i] * a.scale2 - base);
@@ -473,20 +488,95 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_kernel(
       }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 #pragma unroll
-    for (int u = 0; u < ROWS / 32; ++u) {
-      const int kb = t * ROWS + u * 32;
-      TL::add(acc, ldsV + u * 32 * TL::RB, zeros, lo, s[u], edge_tile && kb + 31 > span.wave_all,
+    for (int u = 0; u < NU; ++u) {
+      const int kb = key0 + u * 32;
+      TL::add(acc, ldsV + u * 32 * TL::RB, zeros, lo, s[u], edge && kb + 31 > span.wave_all,
               [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
-  stream((span.kend + ROWS - 1) / ROWS, fetch, put, step);
+  stream(n, fetch, put, step);
   l += __shfl_xor(l, 32, 64);
+  int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
+  if constexpr (WK > 1) {
+    // Join the sums of the wavefronts that share queries; wavefront wk takes the blocks wk, wk + WK, ...
+    __syncthreads();
+    float *const mine = reinterpret_cast<float *>(lds) + threadIdx.x;
+    mine[0] = m;
+    mine[256] = l;
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) mine[(2 + db * 16 + i) * 256] = acc[db][i];
+    __syncthreads();
+    const float *const all = reinterpret_cast<const float *>(lds) + wq * 64 + lane;
+    float f[WK];
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) m = fmaxf(m, all[w * WQ * 64]);
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      f[w] = __builtin_amdgcn_exp2f(all[w * WQ * 64] - (m == -INFINITY ? 0.f : m));
+      l += f[w] * all[256 + w * WQ * 64];
+    }
+    db0 = min(wk * ((DB + WK - 1) / WK), DB);
+    db1 = min(db0 + (DB + WK - 1) / WK, DB);
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+      if (db >= db0 && db < db1)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float v = 0.f;
+#pragma unroll
+          for (int w = 0; w < WK; ++w) v += f[w] * all[(2 + db * 16 + i) * 256 + w * WQ * 64];
+          acc[db][i] = v;
+        }
+  }
   if (!r.live) return;
-  const float f = r.lim < 0 ? 0.f : 1.f / l;
-  store_column<T, DP>(a.out + (i64)(r.s.q0 + r.query) * a.out_ld + r.head * a.D, a.D, acc, f);
-  if (a.lse && h == 0)
-    a.lse[(i64)(r.s.q0 + r.query) * a.Hq + r.head] = r.lim < 0 ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+  const i64 at = (i64)(r.s.q0 + r.query) * a.Hq + r.head;
+  if (a.splits > 1) {
+    const i64 plane = (i64)a.total_q * a.Hq;
+    store_column<float, DP>(a.partials + (split * plane + at) * a.D, a.D, acc, 1.f, db0, db1);
+    if (h == 0 && wk == 0) {
+      float *const ml = a.partials + a.splits * plane * a.D + 2 * (split * plane + at);
+      ml[0] = m;
+      ml[1] = r.lim < 0 ? -1.f : l;  // a sum cannot be negative: the mark of a query that sees no key
+    }
+    return;
+  }
+  store_column<T, DP>(a.out + (i64)(r.s.q0 + r.query) * a.out_ld + r.head * a.D, a.D, acc, r.lim < 0 ? 0.f : 1.f / l, db0, db1);
+  if (a.lse && h == 0 && wk == 0) a.lse[at] = r.lim < 0 ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
+
+// out and lse from the sums over the shares of the keys: one wavefront per query and head.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_join_kernel(const Args<T> a) {
+  const int q0 = bound_of(a.cu_q, 0, a.total_q), q1 = bound_of(a.cu_q, a.num_seqs, a.total_q), lane = threadIdx.x & 63;
+  const i64 at = (i64)q0 * a.Hq + (i64)blockIdx.x * WAVES + (threadIdx.x >> 6), plane = (i64)a.total_q * a.Hq;
+  if (at >= (i64)q1 * a.Hq) return;
+  const float *const ml = a.partials + a.splits * plane * a.D + 2 * at;
+  // lanes take the shares in turn for the weights, then the elements
+  float m = -INFINITY;
+  for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[2 * s * plane]);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f, v0 = 0.f, v1 = 0.f;
+  const bool none = ml[1] < 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const float f = __builtin_amdgcn_exp2f(ml[2 * s * plane] - base);
+    l += f * ml[2 * s * plane + 1];
+    const float *const p = a.partials + (s * plane + at) * a.D;
+    if (lane < a.D) v0 += f * p[lane];
+    if (lane + 64 < a.D) v1 += f * p[lane + 64];
+  }
+  const i64 token = at / a.Hq, head = at - token * a.Hq;
+  T *const o = a.out + token * a.out_ld + head * a.D;
+  const float r = none ? 0.f : 1.f / l;
+  if (lane < a.D) from_f32(none ? 0.f : v0 * r, o[lane]);
+  if (lane + 64 < a.D) from_f32(none ? 0.f : v1 * r, o[lane + 64]);
+  if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
+}
+
 // dQ, and delta for the kernel below.
 template <typename T, int DP, bool TAIL>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(const Args<T> a) {
@@ -499,11 +589,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;
   Rows r;
   int row0;
-  if (!rows_of(a, tile, kvh, r, row0)) return;
+  const int wave = threadIdx.x >> 6;
+  if (!rows_of<BM>(a, tile, kvh, wave, r, row0)) return;
   TL::clear(zeros);
   const int lane = threadIdx.x & 63, h = lane >> 5;
   const auto lo = TL::lane_offsets(lane);
-  const Span span = span_of(a, r, row0);
+  const Span span = span_of<BM>(a, r, row0, wave);
 
   Frag<T> q[DP / 16], dout[DP / 16];
   float delta = 0.f;
@@ -781,6 +872,33 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
   return UNET_OK;
 }
 
+// How the forward shares its work.  wide: wavefronts of a workgroup share queries (see attention_kernel), when
+// workgroups of 128 would not give every CU one; splits: ranges of the keys, when that is still too few, each of at
+// least 512 keys on the average (what a join costs more would not be won back).
+struct Plan {
+  bool shared;
+  int splits, tiles;  // tiles: an upper bound
+};
+template <typename T>
+constexpr int shared_waves(int DP) { return DP * sizeof(T) > 256 ? 2 : 4; }  // the tiles of 4 would not fit the LDS
+Plan forward_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int wk) {
+  const i64 rows = total_q * (Hq / Hkv);
+  auto groups = [&](int bq) { const i64 t = (rows + bq - 1) / bq; return (t > num_seqs ? t : num_seqs) * Hkv; };
+  Plan p;
+  p.shared = groups(BM) < 256;
+  const int bq = p.shared ? BM / wk : BM;
+  i64 s = 1;
+  if (p.shared && num_seqs > 0) {
+    s = 256 / groups(bq);
+    if (s > total_k / num_seqs / 512) s = total_k / num_seqs / 512;
+  }
+  p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  p.tiles = (int)(rows / bq) + num_seqs;
+  return p;
+}
+template <typename T>
+int wk_of(int D) { return shared_waves<T>(D <= 32 ? 32 : D <= 64 ? 64 : 128); }
+
 // Row ranges into which the dK/dV kernel's sums are split when there are few key tiles: workgroups of very different
 // lengths (causal) fill 256 CUs evenly once there are several times 512 of them (two fit a CU).  Each range costs a
 // pass over fp32 dK and dV, so it should have 512 rows at least on the average.
@@ -789,6 +907,9 @@ int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv) {
   i64 s = tiles > 0 ? 1024 / tiles : 1;
   if (s > rows / 512) s = rows / 512;
   return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+}
+size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
+  return splits > 1 ? (size_t)splits * total_q * Hq * (D + 2) * sizeof(float) : 0;
 }
 size_t delta_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * sizeof(float) + 15) / 16 * 16; }
 
@@ -816,10 +937,21 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   UNET_REQUIRE(aligned<float>(lse), "%s: lse is misaligned", name);
   if (num_seqs == 0 || total_q == 0) return UNET_OK;
   a.out = out, a.out_ld = out_ld, a.lse = lse;
-  a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+  const Plan plan = forward_plan(num_seqs, total_q, total_k, Hq, Hkv, wk_of<T>(D));
+  a.tiles = plan.tiles, a.splits = plan.splits, a.partials = (float *)ws;
+  if (plan.splits > 1) {
+    const size_t need = forward_bytes(total_q, Hq, D, plan.splits);
+    UNET_REQUIRE(ws && ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
+    UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
+  }
   with_dim<T>(D, [&](auto dp, auto tail) {
-    attention_kernel<T, decltype(dp)::value, decltype(tail)::value><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
+    constexpr int DP = decltype(dp)::value;
+    constexpr bool TAIL = decltype(tail)::value;
+    const unsigned grid = (unsigned)a.tiles * Hkv * a.splits;
+    if (plan.shared) attention_kernel<T, DP, TAIL, shared_waves<T>(DP)><<<grid, 256, 0, st>>>(a);
+    else attention_kernel<T, DP, TAIL, 1><<<grid, 256, 0, st>>>(a);
   });
+  if (a.splits > 1) attention_join_kernel<T><<<cdiv_u(total_q * Hq, WAVES), 256, 0, st>>>(a);
   UNET_LAUNCH_CHECK(name);
   return UNET_OK;
 }
@@ -868,7 +1000,13 @@ int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t to
                                        int head_dim, size_t *bytes_host) {
   UNET_REQUIRE(bytes_host, "dot_attention_workspace_bytes: NULL result");
   TRY(check_shape("dot_attention_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  *bytes_host = 0;
+  // the larger of the two types' plans
+  size_t need = 0;
+  for (const int wk : {wk_of<float>(head_dim), wk_of<bf16_t>(head_dim)}) {
+    const size_t n = forward_bytes(total_q, heads_q, head_dim, forward_plan(num_seqs, total_q, total_k, heads_q, heads_kv, wk).splits);
+    if (n > need) need = n;
+  }
+  *bytes_host = need;
   return UNET_OK;
 }
 int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
