@@ -26,6 +26,9 @@
 namespace {
 
 typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int COLS = 32;            // columns (queries or keys) per wavefront
 constexpr int WAVES = 4;
@@ -34,6 +37,7 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // The running maximum follows a score only when that exceeds it by this much (in powers of two): until then the
 // weights are at most 2^8 and nothing is rescaled.  The final division makes up for it exactly.
 constexpr float LAZY = 8.f;
+constexpr unsigned NOWHERE = 0x80000000u;  // a byte offset behind the end of every buffer (a tile spans less than 2 GiB)
 
 template <typename T>
 struct FragOf;
@@ -64,9 +68,13 @@ template <typename T>
 __device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
   Frag<T> f;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    if constexpr (sizeof(T) == 2) f[j] = (__bf16)w[8 * t + j];
-    else f[j] = w[8 * t + j];
+  for (int j = 0; j < 8; j += 2) {
+    if constexpr (sizeof(T) == 2) {  // as pairs: one conversion instruction for two
+      const bf16x2 p = __builtin_convertvector((f32x2{w[8 * t + j], w[8 * t + j + 1]}), bf16x2);
+      f[j] = p[0], f[j + 1] = p[1];
+    } else {
+      f[j] = w[8 * t + j], f[j + 1] = w[8 * t + j + 1];
+    }
   }
   return f;
 }
@@ -182,12 +190,36 @@ struct Tile {
       return f;
     }
   }
-  // This thread's chunks of a tile, on their way from memory to LDS.  Row r of the tile is row first + r of a
-  // sequence of n rows; rows and elements that do not exist become zeros.
+  // ---- memory -> LDS, whole 16-byte chunks (FAST): direct loads, a wavefront moves 1 KB per instruction.  The swizzle is on
+  // the side of the memory address: lane l of a wavefront's instruction i fills chunk `slot` of the tile.
+  static constexpr int MOVES = BYTES / 1024 / WAVES;
+  static __device__ __forceinline__ int slot(int i) { return ((int)(threadIdx.x >> 6) * MOVES + i) * 64 + (int)(threadIdx.x & 63); }
+  static __device__ __forceinline__ int slot_row(int i) { return slot(i) / NC; }
+  // byte offset of the slot's chunk in its row, or beyond any buffer where the head has no such elements
+  static __device__ __forceinline__ unsigned slot_chunk(int i, int D) {
+    const int c = (slot(i) % NC) ^ key(slot_row(i));
+    return c * CH < D ? (unsigned)c * 16u : NOWHERE;
+  }
+  // offset[i]: the byte offsets of this lane's chunks from `base`; chunks at or beyond `bytes` become zeros.
+  static __device__ __forceinline__ void move(const T *base, i64 bytes, const unsigned (&offset)[MOVES], unsigned lds_tile) {
+    const uint64_t b = (uint64_t)base;
+    const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)b), __builtin_amdgcn_readfirstlane((int)(b >> 32)),
+                        __builtin_amdgcn_readfirstlane((int)(unsigned)max(min(bytes, (i64)NOWHERE), (i64)0)), 0x00020000};
+#pragma unroll
+    for (int i = 0; i < MOVES; ++i) {
+      const unsigned at = __builtin_amdgcn_readfirstlane(lds_tile + ((threadIdx.x >> 6) * MOVES + i) * 1024u);
+      asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+                   :
+                   : "s"(at), "v"(offset[i]), "s"(rsrc));
+    }
+  }
+
+  // ---- memory -> registers -> LDS, any alignment and head dimension.  This thread's chunks of a tile on their way; row r of
+  // the tile is row first + r of a sequence of n rows.  Rows and elements that do not exist become zeros.
   struct Chunks {
     u32x4 c[PER];
   };
-  template <bool TAIL, typename Row>
+  template <typename Row>
   static __device__ __forceinline__ void fetch(Chunks &to, int first, int n, int D, Row row_ptr) {
     const int e = (threadIdx.x % NC) * CH, r0 = first + threadIdx.x / NC;
 #pragma unroll
@@ -197,7 +229,7 @@ struct Tile {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const T *p = row_ptr(min(r0 + i * (256 / NC), n - 1)) + e;
-        if (!TAIL || e + CH <= D) {
+        if (e + CH <= D) {
           __builtin_memcpy(&to.c[i], p, 16);
         } else {
           T tmp[CH];
@@ -222,22 +254,19 @@ struct Tile {
   }
   // Whether any of 32 rows of the tile holds an infinity or NaN.
   static __device__ __forceinline__ bool not_finite(const unsigned char *rows32, const Lane &o) {
-    uint32_t top = 0;
+    typedef typename std::conditional<sizeof(T) == 2, u16x2, uint32_t>::type Word;  // magnitudes: 16 bits twice, or 32
+    Word top = {};
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
       const Frag<T> f = along(rows32, o, t);
       uint32_t w[sizeof(f) / 4];
       __builtin_memcpy(w, &f, sizeof(f));
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(f) / 4); ++i) {
-        if constexpr (sizeof(T) == 2) {
-          top |= ((w[i] & 0x7f80u) == 0x7f80u) | ((w[i] & 0x7f800000u) == 0x7f800000u);
-        } else {
-          top |= (w[i] & 0x7f800000u) == 0x7f800000u;
-        }
-      }
+      for (int i = 0; i < (int)(sizeof(f) / 4); ++i)
+        top = __builtin_elementwise_max(top, __builtin_bit_cast(Word, w[i] & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu)));
     }
-    return __any(top != 0);
+    if constexpr (sizeof(T) == 2) return __any(top[0] >= 0x7f80u || top[1] >= 0x7f80u);
+    else return __any(top >= 0x7f800000u);
   }
   // acc[d][column] += sum over 32 rows of X[row][d] W[row][column].  edge: some rows are hidden from some columns, with
   // weight 0.  If such rows hold infinities or NaN, 0 * inf must not reach a column that does not see them: then the
@@ -353,25 +382,79 @@ __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int
 template <typename T, int DP>
 constexpr int tile_rows() { return DP * sizeof(T) >= 256 ? 32 : 64; }
 
-// Runs step(tile, buffer) for the tiles [0, n) with the next tile on its way to the other buffer: fetch(t) loads tile t to
-// registers, put(buffer) writes them to LDS.  One barrier per tile: behind it every wavefront has left the buffer
-// that is written next, and sees the one that is read next.
-template <typename Fetch, typename Put, typename Step>
-__device__ __forceinline__ void stream(int n, Fetch fetch, Put put, Step step) {
+// Runs step(tile, buffer) for the tiles [0, n) with the next tile on its way to the other buffer.  One barrier per tile:
+// behind it every wavefront has left the buffer that is written next, and sees the one that is read next.
+//   FAST: move(t, buffer) starts the direct loads of tile t, which are waited for in front of tile t's barrier;
+//         put(buffer) writes what the tile needs besides them.
+//   else: fetch(t) loads tile t to registers, put(buffer) writes them to LDS.
+template <bool FAST, typename Move, typename Fetch, typename Put, typename Step>
+__device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, Step step) {
   if (n <= 0) return;
   fetch(0);
-  put(0);
-  fetch(1);
+  if constexpr (FAST) {
+    move(0, 0);
 #pragma unroll 1
-  for (int t = 0; t < n; ++t) {
-    __syncthreads();
-    if (t + 1 < n) {
-      put((t + 1) & 1);
-      fetch(t + 2);
+    for (int t = 0; t < n; ++t) {
+      put(t & 1);
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (t + 1 < n) {
+        move(t + 1, (t + 1) & 1);
+        fetch(t + 1);
+      }
+      step(t, t & 1);
     }
-    step(t, t & 1);
+  } else {
+    put(0);
+    fetch(1);
+#pragma unroll 1
+    for (int t = 0; t < n; ++t) {
+      __syncthreads();
+      if (t + 1 < n) {
+        put((t + 1) & 1);
+        fetch(t + 2);
+      }
+      step(t, t & 1);
+    }
   }
 }
+// Where a workgroup's LDS array begins, as the direct loads want it.
+__device__ __forceinline__ unsigned lds_address(unsigned char *lds) {
+  return (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds;
+}
+
+// Keys and values of a sequence, tile by tile, for the kernels that stream them.
+template <typename T, typename TL, bool FAST>
+struct KeyTiles {
+  const T *k, *v;
+  i64 k_ld, v_ld;
+  int D;
+  unsigned ko[TL::MOVES], vo[TL::MOVES];
+  typename TL::Chunks ck, cv;
+  __device__ __forceinline__ KeyTiles(const Args<T> &a, const Seq &s, int kvh)
+      : k(a.k + (i64)s.k0 * a.k_ld + kvh * a.D), v(a.v + (i64)s.k0 * a.v_ld + kvh * a.D), k_ld(a.k_ld), v_ld(a.v_ld), D(a.D) {
+    if constexpr (FAST)
+#pragma unroll
+      for (int i = 0; i < TL::MOVES; ++i) {
+        const unsigned c = TL::slot_chunk(i, D);
+        ko[i] = c == NOWHERE ? c : TL::slot_row(i) * (unsigned)k_ld * (unsigned)sizeof(T) + c;
+        vo[i] = c == NOWHERE ? c : TL::slot_row(i) * (unsigned)v_ld * (unsigned)sizeof(T) + c;
+      }
+  }
+  // the tile whose first key is `first`, keys [0, end)
+  __device__ __forceinline__ void move(int first, int end, unsigned lds_k, unsigned lds_v) {
+    const i64 rows = end - first - 1;  // behind the last row's elements, in front of the next row's
+    TL::move(k + first * k_ld, rows < 0 ? 0 : (rows * k_ld + D) * (i64)sizeof(T), ko, lds_k);
+    TL::move(v + first * v_ld, rows < 0 ? 0 : (rows * v_ld + D) * (i64)sizeof(T), vo, lds_v);
+  }
+  __device__ __forceinline__ void fetch(int first, int end) {
+    TL::fetch(ck, first, end, D, [&](int j) __attribute__((always_inline)) { return k + j * k_ld; });
+    TL::fetch(cv, first, end, D, [&](int j) __attribute__((always_inline)) { return v + j * v_ld; });
+  }
+  __device__ __forceinline__ void put(unsigned char *lds_k, unsigned char *lds_v) {
+    TL::put(ck, lds_k);
+    TL::put(cv, lds_v);
+  }
+};
 
 // Which keys the queries of a workgroup and of this wavefront see (all of them / at least one of them).
 struct Span {
@@ -396,7 +479,7 @@ __device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row
 // workgroup has 128 queries (every tile serves four times 32), with WK > 1 it has fewer, for calls that have too few
 // queries to fill the GPU.  splits > 1: the workgroup takes a share of the key tiles and leaves its sums to
 // attention_join_kernel.
-template <typename T, int DP, bool TAIL, int WK>
+template <typename T, int DP, bool FAST, int WK>
 __global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 1) void attention_kernel(const Args<T> a) {
   constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS> TL;
@@ -430,16 +513,17 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 
     first = min(split * per, n);
     n = min(per, n - first);
   }
-  const T *const kp = a.k + (i64)r.s.k0 * a.k_ld + kvh * a.D, *const vp = a.v + (i64)r.s.k0 * a.v_ld + kvh * a.D;
-  typename TL::Chunks ck, cv;
+  KeyTiles<T, TL, FAST> keys(a, r.s, kvh);
+  const unsigned lds0 = lds_address(lds);
+  const int end = min(span.kend, (first + n) * ROWS);
+  auto move = [&](int t, int buf) __attribute__((always_inline)) {
+    keys.move((first + t) * ROWS, end, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
+  };
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    const int end = min(span.kend, (first + n) * ROWS);
-    TL::template fetch<TAIL>(ck, (first + t) * ROWS, end, a.D, [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; });
-    TL::template fetch<TAIL>(cv, (first + t) * ROWS, end, a.D, [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; });
+    if (!FAST) keys.fetch((first + t) * ROWS, end);
   };
   auto put = [&](int buf) __attribute__((always_inline)) {
-    TL::put(ck, lds + buf * STAGE);
-    TL::put(cv, lds + buf * STAGE + TL::BYTES);
+    if (!FAST) keys.put(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
   };
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const int key0 = (first + t) * ROWS + wk * 32;
@@ -494,7 +578,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 
               [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
-  stream(n, fetch, put, step);
+  stream<FAST>(n, move, fetch, put, step);
   l += __shfl_xor(l, 32, 64);
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
@@ -554,21 +638,26 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args<T> a) {
   const i64 at = (i64)q0 * a.Hq + (i64)blockIdx.x * WAVES + (threadIdx.x >> 6), plane = (i64)a.total_q * a.Hq;
   if (at >= (i64)q1 * a.Hq) return;
   const float *const ml = a.partials + a.splits * plane * a.D + 2 * at;
-  // lanes take the shares in turn for the weights, then the elements
-  float m = -INFINITY;
-  for (int s = lane; s < a.splits; s += 64) m = fmaxf(m, ml[2 * s * plane]);
+  // lane s: the weight of share s (there are at most 64); then the lanes take the elements
+  const float m_s = lane < a.splits ? ml[2 * lane * plane] : -INFINITY, l_s = lane < a.splits ? ml[2 * lane * plane + 1] : 0.f;
+  const bool none = ml[1] < 0.f;
+  float m = m_s;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f, v0 = 0.f, v1 = 0.f;
-  const bool none = ml[1] < 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float f = __builtin_amdgcn_exp2f(ml[2 * s * plane] - base);
-    l += f * ml[2 * s * plane + 1];
-    const float *const p = a.partials + (s * plane + at) * a.D;
-    if (lane < a.D) v0 += f * p[lane];
-    if (lane + 64 < a.D) v1 += f * p[lane + 64];
-  }
+  const float f_s = __builtin_amdgcn_exp2f(m_s - (m == -INFINITY ? 0.f : m));
+  const float l = wave_sum(f_s * l_s);
+  float v0 = 0.f, v1 = 0.f;
+  const float *p = a.partials + at * a.D;
+  const int e0 = min(lane, a.D - 1), e1 = min(lane + 64, a.D - 1);
+  for (int s0 = 0; s0 < a.splits; s0 += 8)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(f_s), s0 + j));
+      const float *const ps = p + min(s0 + j, a.splits - 1) * (plane * a.D);
+      const float x0 = f * ps[e0], x1 = f * ps[e1];
+      v0 += s0 + j < a.splits ? x0 : 0.f;
+      v1 += s0 + j < a.splits ? x1 : 0.f;
+    }
   const i64 token = at / a.Hq, head = at - token * a.Hq;
   T *const o = a.out + token * a.out_ld + head * a.D;
   const float r = none ? 0.f : 1.f / l;
@@ -578,7 +667,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args<T> a) {
 }
 
 // dQ, and delta for the kernel below.
-template <typename T, int DP, bool TAIL>
+template <typename T, int DP, bool FAST>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(const Args<T> a) {
   constexpr int ROWS = tile_rows<T, DP>();
   typedef Tile<T, DP, ROWS> TL;
@@ -619,15 +708,16 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
   f32x16 acc[DP / 32];
 #pragma unroll
   for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
-  const T *const kp = a.k + (i64)r.s.k0 * a.k_ld + kvh * a.D, *const vp = a.v + (i64)r.s.k0 * a.v_ld + kvh * a.D;
-  typename TL::Chunks ck, cv;
+  KeyTiles<T, TL, FAST> keys(a, r.s, kvh);
+  const unsigned lds0 = lds_address(lds);
+  auto move = [&](int t, int buf) __attribute__((always_inline)) {
+    keys.move(t * ROWS, span.kend, lds0 + buf * 2 * TL::BYTES, lds0 + buf * 2 * TL::BYTES + TL::BYTES);
+  };
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    TL::template fetch<TAIL>(ck, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return kp + (i64)j * a.k_ld; });
-    TL::template fetch<TAIL>(cv, t * ROWS, span.kend, a.D, [&](int j) __attribute__((always_inline)) { return vp + (i64)j * a.v_ld; });
+    if (!FAST) keys.fetch(t * ROWS, span.kend);
   };
   auto put = [&](int buf) __attribute__((always_inline)) {
-    TL::put(ck, lds + buf * 2 * TL::BYTES);
-    TL::put(cv, lds + buf * 2 * TL::BYTES + TL::BYTES);
+    if (!FAST) keys.put(lds + buf * 2 * TL::BYTES, lds + buf * 2 * TL::BYTES + TL::BYTES);
   };
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const unsigned char *const ldsK = lds + buf * 2 * TL::BYTES, *const ldsV = ldsK + TL::BYTES;
@@ -666,14 +756,14 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
       TL::add(acc, k32, zeros, lo, s, edge, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
-  stream((span.kend + ROWS - 1) / ROWS, fetch, put, step);
+  stream<FAST>((span.kend + ROWS - 1) / ROWS, move, fetch, put, step);
   if (!r.live) return;
   if (h == 0) a.delta[at] = delta;
   store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale);
 }
 
 // dK and dV: keys in registers, the packed queries of the group streamed.
-template <typename T, int DP, bool TAIL>
+template <typename T, int DP, bool FAST>
 __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(const Args<T> a) {
   constexpr int ROWS = tile_rows<T, DP>();
   typedef Tile<T, DP, ROWS> TL;
@@ -728,10 +818,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
   };
   typename TL::Chunks cq, cd;
   float fl, fd;
+  const unsigned lds0 = lds_address(lds);
+  auto move = [&](int t, int buf) __attribute__((always_inline)) {
+    const int r0 = first + t * ROWS, query0 = div_by(r0, a.G);
+    unsigned qo[TL::MOVES], dof[TL::MOVES];
+#pragma unroll
+    for (int i = 0; i < TL::MOVES; ++i) {
+      const int r = r0 + TL::slot_row(i), query = div_by(r, a.G);
+      const unsigned c = r < nrows ? TL::slot_chunk(i, a.D) : NOWHERE;
+      const unsigned in_row = c + (unsigned)((r - query * g) * a.D * (int)sizeof(T)), by = (unsigned)(query - query0) * (unsigned)sizeof(T);
+      qo[i] = c == NOWHERE ? c : by * (unsigned)a.q_ld + in_row;
+      dof[i] = c == NOWHERE ? c : by * (unsigned)a.dout_ld + in_row;
+    }
+    const i64 token = s.q0 + query0;
+    TL::move(a.q + token * a.q_ld + kvh * g * a.D, NOWHERE, qo, lds0 + buf * STAGE);
+    TL::move(a.dout + token * a.dout_ld + kvh * g * a.D, NOWHERE, dof, lds0 + buf * STAGE + TL::BYTES);
+  };
   auto fetch = [&](int t) __attribute__((always_inline)) {
     const int r0 = first + t * ROWS;
-    TL::template fetch<TAIL>(cq, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.q, a.q_ld, r); });
-    TL::template fetch<TAIL>(cd, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.dout, a.dout_ld, r); });
+    if (!FAST) {
+      TL::fetch(cq, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.q, a.q_ld, r); });
+      TL::fetch(cd, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.dout, a.dout_ld, r); });
+    }
     fl = INFINITY, fd = 0.f;  // rows that do not exist have no weight
     const int r = r0 + (int)threadIdx.x;
     if (threadIdx.x < ROWS && r < nrows) {
@@ -743,8 +851,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
   };
   auto put = [&](int buf) __attribute__((always_inline)) {
     unsigned char *const st = lds + buf * STAGE;
-    TL::put(cq, st);
-    TL::put(cd, st + TL::BYTES);
+    if (!FAST) {
+      TL::put(cq, st);
+      TL::put(cd, st + TL::BYTES);
+    }
     if (threadIdx.x < ROWS) {
       float *const f = reinterpret_cast<float *>(st + 2 * TL::BYTES) + threadIdx.x;
       f[0] = fl;
@@ -792,7 +902,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
       TL::add(dk, q32, zeros, lo, ds, edge, sees);
     }
   };
-  stream((nrows - first + ROWS - 1) / ROWS, fetch, put, step);
+  stream<FAST>((nrows - first + ROWS - 1) / ROWS, move, fetch, put, step);
   if (!live) return;
   if (a.splits > 1) {
     const i64 at = ((i64)(s.k0 + key) * a.Hkv + kvh) * a.D, plane = (i64)a.total_k * a.Hkv * a.D;
@@ -872,8 +982,10 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
   return UNET_OK;
 }
 
-// How the forward shares its work.  wide: wavefronts of a workgroup share queries (see attention_kernel), when
-// workgroups of 128 would not give every CU one; splits: ranges of the keys, when that is still too few, each of at
+// How the forward shares its work.  shared: wavefronts of a workgroup share queries (see attention_kernel), when
+// workgroups of 128 would give at most half of the CUs one.  A quarter of the queries is then a quarter of the time and a
+// third more, for tiles that serve one wavefront each: 224 workgroups of 128 took 89 us, 896 of 32 117 us (fp32, head
+// dimension 64), 16 against 64 10.0 and 6.6 us (bf16, 64).  splits: ranges of the keys, when that is still too few, each of at
 // least 512 keys on the average (what a join costs more would not be won back).
 struct Plan {
   bool shared;
@@ -885,7 +997,7 @@ Plan forward_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int w
   const i64 rows = total_q * (Hq / Hkv);
   auto groups = [&](int bq) { const i64 t = (rows + bq - 1) / bq; return (t > num_seqs ? t : num_seqs) * Hkv; };
   Plan p;
-  p.shared = groups(BM) < 256;
+  p.shared = groups(BM) <= 128;
   const int bq = p.shared ? BM / wk : BM;
   i64 s = 1;
   if (p.shared && num_seqs > 0) {
@@ -913,17 +1025,21 @@ size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
 }
 size_t delta_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * sizeof(float) + 15) / 16 * 16; }
 
-// f(DP, TAIL) with the head dimension padded to the tile's, and whether a row ends inside a 16-byte chunk.
+// f(DP, FAST) with the head dimension padded to the tile's, and whether the streamed rows are whole aligned chunks.
 template <typename T, typename F>
-void with_dim(int D, F f) {
-  const bool tail = D * sizeof(T) % 16 != 0;
+void with_dim(int D, bool fast, F f) {
   auto padded = [&](auto dp) {
-    if (tail) f(dp, std::true_type());
+    if (fast) f(dp, std::true_type());
     else f(dp, std::false_type());
   };
   if (D <= 32) padded(std::integral_constant<int, 32>());
   else if (D <= 64) padded(std::integral_constant<int, 64>());
   else padded(std::integral_constant<int, 128>());
+}
+template <typename T>
+bool whole_chunks(const T *p, i64 ld, int D) {
+  // and a tile's span (at most 128 rows) stays below 2 GiB, the reach of the direct loads' offsets
+  return ((uintptr_t)p & 15) == 0 && ld * sizeof(T) % 16 == 0 && D * sizeof(T) % 16 == 0 && ld <= (1 << 24) / (i64)sizeof(T);
 }
 
 template <typename T>
@@ -944,12 +1060,12 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
     UNET_REQUIRE(ws && ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
     UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
   }
-  with_dim<T>(D, [&](auto dp, auto tail) {
+  with_dim<T>(D, whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D), [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value;
-    constexpr bool TAIL = decltype(tail)::value;
+    constexpr bool FAST = decltype(fast)::value;
     const unsigned grid = (unsigned)a.tiles * Hkv * a.splits;
-    if (plan.shared) attention_kernel<T, DP, TAIL, shared_waves<T>(DP)><<<grid, 256, 0, st>>>(a);
-    else attention_kernel<T, DP, TAIL, 1><<<grid, 256, 0, st>>>(a);
+    if (plan.shared) attention_kernel<T, DP, FAST, shared_waves<T>(DP)><<<grid, 256, 0, st>>>(a);
+    else attention_kernel<T, DP, FAST, 1><<<grid, 256, 0, st>>>(a);
   });
   if (a.splits > 1) attention_join_kernel<T><<<cdiv_u(total_q * Hq, WAVES), 256, 0, st>>>(a);
   UNET_LAUNCH_CHECK(name);
@@ -981,11 +1097,13 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   const unsigned key_tiles = (unsigned)(total_k / BM) + num_seqs;
   a.splits = dkv_splits(num_seqs, total_q, total_k, Hq, Hkv);
   a.partials = (float *)((char *)ws + delta_bytes(total_q, Hq));
-  with_dim<T>(D, [&](auto dp, auto tail) {
+  const bool whole =
+      whole_chunks(q, q_ld, D) && whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D) && whole_chunks(dout, dout_ld, D);
+  with_dim<T>(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value;
-    constexpr bool TAIL = decltype(tail)::value;
-    if (total_q) attention_dq_kernel<T, DP, TAIL><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
-    if (total_k) attention_dkv_kernel<T, DP, TAIL><<<key_tiles * Hkv * a.splits, 256, 0, st>>>(a);
+    constexpr bool FAST = decltype(fast)::value;
+    if (total_q) attention_dq_kernel<T, DP, FAST><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
+    if (total_k) attention_dkv_kernel<T, DP, FAST><<<key_tiles * Hkv * a.splits, 256, 0, st>>>(a);
   });
   if (total_k && a.splits > 1) attention_dkv_join_kernel<T><<<ew_grid(total_k * Hkv * D), 256, 0, st>>>(a);
   UNET_LAUNCH_CHECK(name);
