@@ -92,6 +92,9 @@ __device__ __forceinline__ int div_by(int r, const Div &d) {  // r < 2^31
   return (int)((__umulhi((uint32_t)r, d.mul) + (uint32_t)r) >> d.shift);
 }
 
+// The wavefront's number in its workgroup, in a scalar register.
+__device__ __forceinline__ int wave_index() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
 // ---- arguments ------------------------------------------------------------------------------------------
 template <typename T>
 struct Args {
@@ -113,15 +116,21 @@ __device__ __forceinline__ int bound_of(const int *cu, int s, int total) { retur
 struct Where {
   int seq, row0;
 };
+// The lanes look at 64 sequences at once: one load's latency for up to 64 sequences, two for up to 4096.
 template <int TILE>
 __device__ __forceinline__ Where find_tile(const int *cu, int num_seqs, int total, int g, int tile) {
-  int lo = 0, hi = num_seqs;
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if ((bound_of(cu, mid, total) * g) / TILE + mid <= tile) lo = mid;
-    else hi = mid;
+  auto first_tile = [&](int s) __attribute__((always_inline)) { return (bound_of(cu, s, total) * g) / TILE + s; };
+  int lo = 0, n = num_seqs;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, s = lo + (int)(threadIdx.x & 63) * step;
+    const bool before = (threadIdx.x & 63) == 0 || (s < lo + n && first_tile(s) <= tile);
+    const int count = __popcll(__ballot(before));  // bounds do not decrease: these are the first lanes
+    const int skip = (count - 1) * step;
+    n = min(step, n - skip);
+    lo += skip;
   }
-  return Where{lo, (tile - ((bound_of(cu, lo, total) * g) / TILE + lo)) * TILE};
+  lo = __builtin_amdgcn_readfirstlane(lo);
+  return Where{lo, (tile - first_tile(lo)) * TILE};
 }
 struct Seq {
   int q0, nq, k0, nk;  // first query / key and their numbers
@@ -142,38 +151,55 @@ struct Tile {
   static constexpr int RB = DP * (int)sizeof(T), NC = RB / 16, CH = 16 / (int)sizeof(T);
   static constexpr int BYTES = ROWS * RB, PER = ROWS * NC / 256;
   static_assert(ROWS % 32 == 0 && ROWS * NC % 256 == 0, "whole sub-tiles, whole chunks per thread");
+  // 16 rows at one chunk (the reads along rows, 16 lanes at a time) and 4 rows of 64 bytes (the transposing reads, 32
+  // lanes at a time) both cover the 256 bytes of a bank line.
   static __device__ __forceinline__ int key(int row) {
-    return NC == 4 ? (row & 2) | ((row >> 2) & 1) : ((row & 3) << 1) | ((row >> 2) & 1);
+    if constexpr (RB == 64) return (row >> 2) & 3;
+    else if constexpr (RB == 128) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return ((row & 3) << 2) | ((row >> 2) & 3);
   }
   // Lane offsets: reads along a row (lane l: row l % 32, elements 16 t + 8 (l / 32) + j) and down 16 rows (lane l:
-  // element 32 db + l % 32 of the rows 4 (l / 32) + j and 8 + 4 (l / 32) + j, j < 4).
+  // element 32 db + l % 32 of the rows 4 (l / 32) + j and 8 + 4 (l / 32) + j, j < 4).  t and db change bits of the chunk
+  // number alone, so they are exclusive-ored into the offset.
   struct Lane {
-    int row[4], down[4];
+    int row, down[sizeof(T) == 2 ? 2 : 8];
   };
   static __device__ __forceinline__ Lane lane_offsets(int lane) {
     Lane o;
     const int h = lane >> 5, l = lane & 31;
+    if constexpr (sizeof(T) == 2) {
+      o.row = l * RB + (h ^ key(l)) * 16;
+      const int q = (lane & 15) >> 2, p = lane & 3;  // a 16-lane group transposes 4 rows x 16 elements
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (sizeof(T) == 2) {
-        o.row[i] = l * RB + ((2 * i + h) ^ key(l)) * 16;
-        const int q = (lane & 15) >> 2, p = lane & 3, r = 4 * h + q;  // a 16-lane group transposes 4 rows x 16 elements
-        o.down[i] = r * RB + (((4 * (i & 1) + 2 * ((lane >> 4) & 1) + (p >> 1)) ^ key(r)) * 16) + (p & 1) * 8;
-      } else {
-        o.row[i] = l * RB + ((4 * (i >> 1) + 2 * h + (i & 1)) ^ key(l)) * 16;
-        const int r = 4 * h + i;
-        o.down[i] = r * RB + (((l >> 2) ^ key(r)) * 16) + (l & 3) * 4;
+      for (int i = 0; i < 2; ++i) {
+        const int r = 8 * i + 4 * h + q;
+        o.down[i] = r * RB + ((2 * ((lane >> 4) & 1) + (p >> 1)) ^ key(r)) * 16 + (p & 1) * 8;
+      }
+    } else {
+      o.row = l * RB + ((2 * h) ^ key(l)) * 16;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int r = 8 * (i >> 2) + 4 * h + (i & 3);
+        o.down[i] = r * RB + ((l >> 2) ^ key(r)) * 16 + (l & 3) * 4;
       }
     }
+    return o;
+  }
+  // The same offsets, but not known to be the same as before: the exclusive-ors are then taken again where they are used
+  // instead of being kept in registers over the whole loop.
+  static __device__ __forceinline__ Lane forget(Lane o) {
+    asm volatile("" : "+v"(o.row));
+#pragma unroll
+    for (int &d : o.down) asm volatile("" : "+v"(d));
     return o;
   }
   static __device__ __forceinline__ Frag<T> along(const unsigned char *rows32, const Lane &o, int t) {
     Frag<T> f;
     if constexpr (sizeof(T) == 2) {
-      f = *reinterpret_cast<const bf16x8 *>(rows32 + o.row[t & 3] + (t >> 2) * 128);
+      f = *reinterpret_cast<const bf16x8 *>(rows32 + (o.row ^ (t * 32)));
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4 *>(rows32 + o.row[(t & 1) * 2] + (t >> 1) * 128);
-      const f32x4 b = *reinterpret_cast<const f32x4 *>(rows32 + o.row[(t & 1) * 2 + 1] + (t >> 1) * 128);
+      const f32x4 a = *reinterpret_cast<const f32x4 *>(rows32 + (o.row ^ (t * 64)));
+      const f32x4 b = *reinterpret_cast<const f32x4 *>(rows32 + (o.row ^ (t * 64 + 16)));
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
     }
@@ -181,12 +207,11 @@ struct Tile {
   }
   static __device__ __forceinline__ Frag<T> down(const unsigned char *rows16, const Lane &o, int db) {
     if constexpr (sizeof(T) == 2) {
-      const unsigned char *p = rows16 + o.down[db & 1] + (db >> 1) * 128;
-      return tr_read_pair(p, p + 8 * RB);
+      return tr_read_pair(rows16 + (o.down[0] ^ (db * 64)), rows16 + (o.down[1] ^ (db * 64)));
     } else {
       Frag<T> f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float *>(rows16 + o.down[j & 3] + (j >> 2) * 8 * RB + db * 128);
+      for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float *>(rows16 + (o.down[j] ^ (db * 128)));
       return f;
     }
   }
@@ -272,11 +297,12 @@ struct Tile {
   // weight 0.  If such rows hold infinities or NaN, 0 * inf must not reach a column that does not see them: then the
   // rows are added one at a time, the result taken by the columns that see the row, and the common product reads
   // zeros instead.  Rare, so slow is fine; what matters is that the accumulators stay where they are.
-  static constexpr int ZEROS = 32 * RB;
+  static constexpr int ZEROS = 16 * RB;
   template <typename Sees>
   static __device__ __forceinline__ void add(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const unsigned char *zeros,
                                              const Lane &o, const f32x16 &w, bool edge, Sees sees) {
     const Frag<T> b0 = pack8<T>(w, 0), b1 = pack8<T>(w, 1);
+    const unsigned char *low = rows32, *high = rows32 + 16 * RB;
     if (edge && not_finite(rows32, o)) {
       const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll 1
@@ -296,12 +322,12 @@ struct Tile {
           for (int i = 0; i < 16; ++i) acc[db][i] += seen ? r[i] : 0.f;
         }
       }
-      rows32 = zeros;
+      low = high = zeros;
     }
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(rows32, o, db), b0, acc[db]);
+    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(low, o, db), b0, acc[db]);
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(rows32 + 16 * RB, o, db), b1, acc[db]);
+    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(high, o, db), b1, acc[db]);
   }
   static __device__ __forceinline__ void clear(unsigned char *zeros) {
     for (int i = threadIdx.x * 16; i < ZEROS; i += 256 * 16) *reinterpret_cast<u32x4 *>(zeros + i) = u32x4{0, 0, 0, 0};
@@ -486,7 +512,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 
   constexpr int STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
   __shared__ __align__(16) unsigned char lds[(2 * STAGE > MERGE ? 2 * STAGE : MERGE) + TL::ZEROS];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6, wq = wave % WQ, wk = wave / WQ;
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits, t0 = bs / a.splits;
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;  // the queries with the most keys first
   Rows r;
@@ -678,7 +704,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;
   Rows r;
   int row0;
-  const int wave = threadIdx.x >> 6;
+  const int wave = wave_index();
   if (!rows_of<BM>(a, tile, kvh, wave, r, row0)) return;
   TL::clear(zeros);
   const int lane = threadIdx.x & 63, h = lane >> 5;
@@ -768,34 +794,37 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
   constexpr int ROWS = tile_rows<T, DP>();
   typedef Tile<T, DP, ROWS> TL;
   constexpr int STAGE = 2 * TL::BYTES + 2 * ROWS * 4;  // Q, dout, lse (base 2), delta
-  // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands stay in
-  // LDS, each wavefront's own, in the order in which the lanes read them.
-  constexpr bool V_LDS = DP == 128;
-  constexpr int V_BYTES = V_LDS ? BM * TL::RB : 0;
-  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS + V_BYTES];
+  // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands, and the last
+  // two of K, stay in LDS, each wavefront's own, in the order in which the lanes read them.  (With six more registers
+  // in use one operand was reloaded from scratch memory in every step, behind the direct loads in flight: 1004 us
+  // instead of 805-830, 8192 tokens, 16/4 heads, causal.)
+  constexpr int KT = DP / 16, K_REG = DP < 128 ? KT : KT - 2, V_REG = DP < 128 ? KT : 0;
+  constexpr int OWN = (2 * KT - K_REG - V_REG) * 64 * (int)sizeof(Frag<T>);
+  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS + WAVES * OWN];
   unsigned char *const zeros = lds + 2 * STAGE;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits;
   const Where w = find_tile<BM>(a.cu_k, a.num_seqs, a.total_k, 1, bs / a.splits);
   const Seq s = seq_of(a, w.seq);
   if (w.row0 < 0 || w.row0 >= s.nk) return;
   TL::clear(zeros);
-  const int lane = threadIdx.x & 63, h = lane >> 5, wave = threadIdx.x >> 6;
-  const auto lo = TL::lane_offsets(lane);
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index();
+  const auto lane_at = TL::lane_offsets(lane);
   const int g = (int)a.G.by, off = s.nk - s.nq;
   const int wkey = w.row0 + wave * COLS, key = wkey + (lane & 31);
   const bool live = key < s.nk;
 
-  Frag<T> k[DP / 16], vr[V_LDS ? 1 : DP / 16];
-  Frag<T> *const vl = reinterpret_cast<Frag<T> *>(lds + 2 * STAGE + TL::ZEROS + wave * (V_BYTES / WAVES)) + lane;
+  Frag<T> kr[K_REG], vr[V_REG ? V_REG : 1];
+  Frag<T> *const own = reinterpret_cast<Frag<T> *>(lds + 2 * STAGE + TL::ZEROS + wave * OWN) + lane;
   {
     const i64 token = s.k0 + min(key, s.nk - 1);
     const T *pk = a.k + token * a.k_ld + kvh * a.D, *pv = a.v + token * a.v_ld + kvh * a.D;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) {
+    for (int t = 0; t < KT; ++t) {
       const int e = 16 * t + 8 * h, n = live ? a.D - e : 0;
-      k[t] = load_frag<T>(pk + e, n);
-      if constexpr (V_LDS) vl[64 * t] = load_frag<T>(pv + e, n);
-      else vr[t] = load_frag<T>(pv + e, n);
+      if (t < K_REG) kr[t] = load_frag<T>(pk + e, n);
+      else own[64 * (KT - V_REG + t - K_REG)] = load_frag<T>(pk + e, n);
+      if (t < V_REG) vr[t] = load_frag<T>(pv + e, n);
+      else own[64 * (t - V_REG)] = load_frag<T>(pv + e, n);
     }
   }
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -870,14 +899,13 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
       if (rb >= nrows) break;
       if (rb + 31 < wave_some) continue;
       const unsigned char *const q32 = ldsQ + u * 32 * TL::RB, *const d32 = ldsD + u * 32 * TL::RB;
+      const auto lo = DP < 128 ? lane_at : TL::forget(lane_at);  // at 128 elements every register counts
       f32x16 p = zero16(), ds = zero16();
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) p = mma(TL::along(q32, lo, x), k[x], p);
+      for (int x = 0; x < DP / 16; ++x) p = mma(TL::along(q32, lo, x), x < K_REG ? kr[x < K_REG ? x : 0] : own[64 * (KT - V_REG + x - K_REG)], p);
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) {
-        if constexpr (V_LDS) ds = mma(TL::along(d32, lo, x), vl[64 * x], ds);
-        else ds = mma(TL::along(d32, lo, x), vr[x], ds);
-      }
+      for (int x = 0; x < DP / 16; ++x) 
+        ds = mma(TL::along(d32, lo, x), x < V_REG ? vr[x < V_REG ? x : 0] : own[64 * (x - V_REG)], ds);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(ldsL + u * 32 + 8 * b + 4 * h);
