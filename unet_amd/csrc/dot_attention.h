@@ -81,7 +81,7 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
 struct Div {
   uint32_t mul, shift, by;
 };
-Div make_div(uint32_t by) {
+inline Div make_div(uint32_t by) {
   uint32_t s = 0;
   while ((1ull << s) < by) ++s;
   return Div{(uint32_t)((((1ull << s) - by) << 32) / by + 1), s, by};
@@ -144,11 +144,12 @@ __device__ __forceinline__ Seq seq_of(const A &a, int s) {
 }
 
 // ---- tiles in LDS ----------------------------------------------------------------------------------------
-template <typename T, int DP, int ROWS>
+// DP: elements that are computed with, a multiple of 32 (rows of 96 are stored like rows of 128); NW: wavefronts of the workgroup.
+template <typename T, int DP, int ROWS, int NW = WAVES>
 struct Tile {
-  static constexpr int RB = DP * (int)sizeof(T), NC = RB / 16, CH = 16 / (int)sizeof(T);
-  static constexpr int BYTES = ROWS * RB, PER = ROWS * NC / 256;
-  static_assert(ROWS % 32 == 0 && ROWS * NC % 256 == 0, "whole sub-tiles, whole chunks per thread");
+  static constexpr int RB = (DP == 96 ? 128 : DP) * (int)sizeof(T), NC = RB / 16, CH = 16 / (int)sizeof(T);
+  static constexpr int BYTES = ROWS * RB, NT = 64 * NW, PER = ROWS * NC / NT;
+  static_assert(ROWS % 32 == 0 && ROWS * NC % NT == 0, "whole sub-tiles, whole chunks per thread");
   // 16 rows at one chunk (the reads along rows, 16 lanes at a time) and 4 rows of 64 bytes (the transposing reads, 32
   // lanes at a time) both cover the 256 bytes of a bank line.
   static __device__ __forceinline__ int key(int row) {
@@ -215,7 +216,7 @@ struct Tile {
   }
   // ---- memory -> LDS, whole 16-byte chunks (FAST): direct loads, a wavefront moves 1 KB per instruction.  The swizzle is on
   // the side of the memory address: lane l of a wavefront's instruction i fills chunk `slot` of the tile.
-  static constexpr int MOVES = BYTES / 1024 / WAVES;
+  static constexpr int MOVES = BYTES / 1024 / NW;
   static __device__ __forceinline__ int slot(int i) { return ((int)(threadIdx.x >> 6) * MOVES + i) * 64 + (int)(threadIdx.x & 63); }
   static __device__ __forceinline__ int slot_row(int i) { return slot(i) / NC; }
   // byte offset of the slot's chunk in its row, or beyond any buffer where the head has no such elements
@@ -251,7 +252,7 @@ struct Tile {
     if (e < D) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
-        const T *p = row_ptr(min(r0 + i * (256 / NC), n - 1)) + e;
+        const T *p = row_ptr(min(r0 + i * (NT / NC), n - 1)) + e;
         if (e + CH <= D) {
           __builtin_memcpy(&to.c[i], p, 16);
         } else {
@@ -265,13 +266,13 @@ struct Tile {
     if (first + ROWS > n)
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (r0 + i * (256 / NC) >= n) to.c[i] = u32x4{0, 0, 0, 0};
+        if (r0 + i * (NT / NC) >= n) to.c[i] = u32x4{0, 0, 0, 0};
   }
   static __device__ __forceinline__ void put(const Chunks &from, unsigned char *tile) {
     const int chunk = threadIdx.x % NC;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-      const int r = threadIdx.x / NC + i * (256 / NC);
+      const int r = threadIdx.x / NC + i * (NT / NC);
       *reinterpret_cast<u32x4 *>(tile + r * RB + ((chunk ^ key(r)) * 16)) = from.c[i];
     }
   }
@@ -328,7 +329,7 @@ struct Tile {
     for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(high, o, db), b1, acc[db]);
   }
   static __device__ __forceinline__ void clear(unsigned char *zeros) {
-    for (int i = threadIdx.x * 16; i < ZEROS; i += 256 * 16) *reinterpret_cast<u32x4 *>(zeros + i) = u32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x * 16; i < ZEROS; i += NT * 16) *reinterpret_cast<u32x4 *>(zeros + i) = u32x4{0, 0, 0, 0};
   }
 };
 
@@ -401,10 +402,12 @@ __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int
   return true;
 }
 
-// Streamed rows per tile: 64, or 32 where a row is 256 bytes and more (a thread then holds 16 registers of the tile that
-// is on its way; with 64 rows the kernels with two streamed matrices and 64 or 128 accumulators spill).
-template <typename T, int DP>
-constexpr int tile_rows() { return DP * sizeof(T) >= 256 ? 32 : 64; }
+// Streamed rows per tile of the gradient kernels.  WK wavefronts that share queries take 32 rows each; else 64, or 32 where
+// long rows go through registers (a thread then holds 16 of them for the tile that is on its way; with 64 rows the kernels
+// with two streamed matrices and 64 or 128 accumulators spill), and in fp32, where the matrix cores take long enough per tile
+// (dQ and dK/dV of 3525 tokens, 8 heads of 64: 124 and 183 us with 32 rows, 138 and 208 with 64).
+template <typename T, int DP, bool FAST, int WK>
+constexpr int tile_rows() { return WK > 1 ? 32 * WK : DP * sizeof(T) >= (FAST && sizeof(T) == 2 ? 257 : 192) ? 32 : 64; }
 
 // Runs step(tile, buffer) for the tiles [0, n) with the next tile on its way to the other buffer.  One barrier per tile:
 // behind it every wavefront has left the buffer that is written next, and sees the one that is read next.
@@ -441,6 +444,34 @@ __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, S
     }
   }
 }
+// Whether the registers are to be limited so that two workgroups fit a CU (the LDS of WK = 4 at 96 elements and more, and the
+// operands of fp32, allow one).
+template <typename T, int DP, int WK>
+constexpr bool two_fit() { return sizeof(T) == 2 && (WK < 4 || DP <= 64); }
+
+// The sums of the wavefronts that share queries, each times its factor, for the blocks [db0, db1) of 32 elements: `all` holds
+// value i of block db of thread t at [(first + db * 16 + i) * 256 + t].
+template <int WK, int DB>
+__device__ __forceinline__ void leave_sums(float *mine, const f32x16 (&acc)[DB], int first) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mine[(first + db * 16 + i) * 256] = acc[db][i];
+}
+template <int WK, int DB>
+__device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], const float *all, int first, const float (&f)[WK], int db0, int db1) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+    if (db >= db0 && db < db1)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) v += f[w] * all[(first + db * 16 + i) * 256 + w * (WAVES / WK) * 64];
+        acc[db][i] = v;
+      }
+}
+
 // Where a workgroup's LDS array begins, as the direct loads want it.
 __device__ __forceinline__ unsigned lds_address(unsigned char *lds) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds;
@@ -504,7 +535,7 @@ __device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row
 // queries to fill the GPU.  splits > 1: the workgroup takes a share of the key tiles and leaves its sums to
 // attention_join_kernel.
 template <typename T, int DP, bool FAST, int WK>
-__global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 1) void attention_kernel(const Args<T> a) {
+__global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_kernel(const Args<T> a) {
   constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS> TL;
   constexpr int STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
@@ -606,15 +637,12 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 
   l += __shfl_xor(l, 32, 64);
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
-    // Join the sums of the wavefronts that share queries; wavefront wk takes the blocks wk, wk + WK, ...
+    // Join the sums of the wavefronts that share queries; each takes a part of the blocks.
     __syncthreads();
     float *const mine = reinterpret_cast<float *>(lds) + threadIdx.x;
     mine[0] = m;
     mine[256] = l;
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mine[(2 + db * 16 + i) * 256] = acc[db][i];
+    leave_sums<WK>(mine, acc, 2);
     __syncthreads();
     const float *const all = reinterpret_cast<const float *>(lds) + wq * 64 + lane;
     float f[WK];
@@ -628,16 +656,7 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 && (WK == 1 || DP < 128) ? 2 : 
     }
     db0 = min(wk * ((DB + WK - 1) / WK), DB);
     db1 = min(db0 + (DB + WK - 1) / WK, DB);
-#pragma unroll
-    for (int db = 0; db < DB; ++db)
-      if (db >= db0 && db < db1)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float v = 0.f;
-#pragma unroll
-          for (int w = 0; w < WK; ++w) v += f[w] * all[(2 + db * 16 + i) * 256 + w * WQ * 64];
-          acc[db][i] = v;
-        }
+    join_sums<WK>(acc, all, 2, f, db0, db1);
   }
   if (!r.live) return;
   const i64 at = (i64)(r.s.q0 + r.query) * a.Hq + r.head;
@@ -690,24 +709,24 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args<T> a) {
   if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// dQ, and delta for the kernel below.
-template <typename T, int DP, bool FAST>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kernel(const Args<T> a) {
-  constexpr int ROWS = tile_rows<T, DP>();
+// dQ, and delta for the kernel below.  WK as in the forward.
+template <typename T, int DP, bool FAST, int WK>
+__global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_dq_kernel(const Args<T> a) {
+  constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = tile_rows<T, DP, FAST, WK>(), NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS> TL;
-  __shared__ __align__(16) unsigned char lds[4 * TL::BYTES + TL::ZEROS];
-  unsigned char *const zeros = lds + 4 * TL::BYTES;
+  constexpr int STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * DB * 16 * 4;
+  __shared__ __align__(16) unsigned char lds[(2 * STAGE > MERGE ? 2 * STAGE : MERGE) + TL::ZEROS];
+  unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
+  const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
   const int kvh = blockIdx.x % a.Hkv;
   const int t0 = blockIdx.x / a.Hkv;
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;
   Rows r;
   int row0;
-  const int wave = wave_index();
-  if (!rows_of<BM>(a, tile, kvh, wave, r, row0)) return;
+  if (!rows_of<BQ>(a, tile, kvh, wq, r, row0)) return;
   TL::clear(zeros);
-  const int lane = threadIdx.x & 63, h = lane >> 5;
   const auto lo = TL::lane_offsets(lane);
-  const Span span = span_of<BM>(a, r, row0, wave);
+  const Span span = span_of<BQ>(a, r, row0, wq);
 
   Frag<T> q[DP / 16], dout[DP / 16];
   float delta = 0.f;
@@ -735,19 +754,19 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
   KeyTiles<T, TL, FAST> keys(a, r.s, kvh);
   const unsigned lds0 = lds_address(lds);
   auto move = [&](int t, int buf) __attribute__((always_inline)) {
-    keys.move(t * ROWS, span.kend, lds0 + buf * 2 * TL::BYTES, lds0 + buf * 2 * TL::BYTES + TL::BYTES);
+    keys.move(t * ROWS, span.kend, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
     if (!FAST) keys.fetch(t * ROWS, span.kend);
   };
   auto put = [&](int buf) __attribute__((always_inline)) {
-    if (!FAST) keys.put(lds + buf * 2 * TL::BYTES, lds + buf * 2 * TL::BYTES + TL::BYTES);
+    if (!FAST) keys.put(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
   };
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
-    const unsigned char *const ldsK = lds + buf * 2 * TL::BYTES, *const ldsV = ldsK + TL::BYTES;
+    const unsigned char *const ldsK = lds + buf * STAGE + wk * 32 * TL::RB, *const ldsV = ldsK + TL::BYTES;
 #pragma unroll 1
-    for (int u = 0; u < ROWS / 32; ++u) {
-      const int kb = t * ROWS + u * 32;
+    for (int u = 0; u < NU; ++u) {
+      const int kb = t * ROWS + (wk + u) * 32;
       if (kb > span.wave_some) break;
       const unsigned char *const k32 = ldsK + u * 32 * TL::RB, *const v32 = ldsV + u * 32 * TL::RB;
       f32x16 s = zero16(), dp = zero16();
@@ -781,16 +800,28 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dq_kern
     }
   };
   stream<FAST>((span.kend + ROWS - 1) / ROWS, move, fetch, put, step);
+  int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
+  if constexpr (WK > 1) {
+    __syncthreads();
+    leave_sums<WK>(reinterpret_cast<float *>(lds) + threadIdx.x, acc, 0);
+    __syncthreads();
+    float f[WK];
+#pragma unroll
+    for (int w = 0; w < WK; ++w) f[w] = 1.f;
+    db0 = min(wk * ((DB + WK - 1) / WK), DB);
+    db1 = min(db0 + (DB + WK - 1) / WK, DB);
+    join_sums<WK>(acc, reinterpret_cast<const float *>(lds) + wq * 64 + lane, 0, f, db0, db1);
+  }
   if (!r.live) return;
-  if (h == 0) a.delta[at] = delta;
-  store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale);
+  if (h == 0 && wk == 0) a.delta[at] = delta;  // the wavefront that has seen the first keys
+  store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale, db0, db1);
 }
 
 // dK and dV: keys in registers, the packed queries of the group streamed.
-template <typename T, int DP, bool FAST>
-__global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(const Args<T> a) {
-  constexpr int ROWS = tile_rows<T, DP>();
-  typedef Tile<T, DP, ROWS> TL;
+template <typename T, int DP, bool FAST, int NW>
+__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(const Args<T> a) {
+  constexpr int ROWS = tile_rows<T, DP, FAST, 1>();
+  typedef Tile<T, DP, ROWS, NW> TL;
   constexpr int STAGE = 2 * TL::BYTES + 2 * ROWS * 4;  // Q, dout, lse (base 2), delta
   // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands, and the last
   // two of K, stay in LDS, each wavefront's own, in the order in which the lanes read them.  (With six more registers
@@ -798,10 +829,10 @@ __global__ __launch_bounds__(256, sizeof(T) == 2 ? 2 : 1) void attention_dkv_ker
   // instead of 805-830, 8192 tokens, 16/4 heads, causal.)
   constexpr int KT = DP / 16, K_REG = DP < 128 ? KT : KT - 2, V_REG = DP < 128 ? KT : 0;
   constexpr int OWN = (2 * KT - K_REG - V_REG) * 64 * (int)sizeof(Frag<T>);
-  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS + WAVES * OWN];
+  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS + NW * OWN];
   unsigned char *const zeros = lds + 2 * STAGE;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits;
-  const Where w = find_tile<BM>(a.cu_k, a.num_seqs, a.total_k, 1, bs / a.splits);
+  const Where w = find_tile<COLS * NW>(a.cu_k, a.num_seqs, a.total_k, 1, bs / a.splits);
   const Seq s = seq_of(a, w.seq);
   if (w.row0 < 0 || w.row0 >= s.nk) return;
   TL::clear(zeros);
@@ -962,7 +993,7 @@ __global__ __launch_bounds__(256) void attention_dkv_join_kernel(const Args<T> a
 template <typename T>
 bool aligned(const void *p) { return ((uintptr_t)p & (sizeof(T) - 1)) == 0; }
 
-int check_shape(const char *name, int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
+inline int check_shape(const char *name, int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
   UNET_REQUIRE(num_seqs >= 0 && total_q >= 0 && total_k >= 0, "%s: num_seqs %d, total_q %lld, total_k %lld", name, num_seqs,
                (long long)total_q, (long long)total_k);
   UNET_REQUIRE(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "%s: %d query heads are no multiple of %d key/value heads", name, Hq, Hkv);
@@ -1008,51 +1039,63 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
   return UNET_OK;
 }
 
-// How the forward shares its work.  shared: wavefronts of a workgroup share queries (see attention_kernel), when
-// workgroups of 128 would give at most half of the CUs one.  A quarter of the queries is then a quarter of the time and a
-// third more, for tiles that serve one wavefront each: 224 workgroups of 128 took 89 us, 896 of 32 117 us (fp32, head
-// dimension 64), 16 against 64 10.0 and 6.6 us (bf16, 64).  splits: ranges of the keys, when that is still too few, each of at
-// least 512 keys on the average (what a join costs more would not be won back).
+// How the kernels that keep queries share their work.  wk (see attention_kernel): 128 queries a workgroup when that fills
+// three quarters of the places (two a CU, one in fp32), else 64, and 32 when it is a quarter or less: shorter workgroups fill
+// the GPU evenly, but their tiles serve fewer wavefronts.  Measured, forward in us with 128 / 64 / 32 queries: 512 workgroups of 128
+// (16 x 256 tokens, 16 heads of 64, bf16) 12.6 / 17.4 / 23.6; 332 (8 sequences of up to 2049, 8/2 heads of 80, causal)
+// 52.7 / 42.4 / 73; 224 (fp32, 3525 tokens, 8 heads of 64) 89 / 84 / 117, dQ 124 / 130 / -; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
+// splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average (what a join costs
+// more would not be won back).
 struct Plan {
-  bool shared;
-  int splits, tiles;  // tiles: an upper bound
+  int wk, splits, tiles;  // tiles of queries: an upper bound
 };
 template <typename T>
-constexpr int shared_waves(int DP) { return DP * sizeof(T) > 256 ? 2 : 4; }  // the tiles of 4 would not fit the LDS
-Plan forward_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int wk) {
+constexpr int most_shared(int DP) { return DP * sizeof(T) > 256 ? 2 : 4; }  // the tiles of 4 would not fit the LDS
+constexpr int padded_dim(int D) { return (D + 31) / 32 * 32; }
+template <typename T>
+Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
+  const int most = most_shared<T>(padded_dim(D)), places = sizeof(T) == 2 ? 512 : 256;
   const i64 rows = total_q * (Hq / Hkv);
   auto groups = [&](int bq) { const i64 t = (rows + bq - 1) / bq; return (t > num_seqs ? t : num_seqs) * Hkv; };
   Plan p;
-  p.shared = groups(BM) <= 128;
-  const int bq = p.shared ? BM / wk : BM;
+  const i64 n = groups(BM);
+  p.wk = n >= places * 3 / 4 ? 1 : n > places / 4 || most == 2 ? 2 : 4;
   i64 s = 1;
-  if (p.shared && num_seqs > 0) {
-    s = 256 / groups(bq);
+  if (p.wk == most && num_seqs > 0) {
+    s = 256 / groups(BM / p.wk);
     if (s > total_k / num_seqs / 512) s = total_k / num_seqs / 512;
   }
   p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
-  p.tiles = (int)(rows / bq) + num_seqs;
+  p.tiles = (int)(rows / (BM / p.wk)) + num_seqs;
   return p;
 }
-template <typename T>
-int wk_of(int D) { return shared_waves<T>(D <= 32 ? 32 : D <= 64 ? 64 : 128); }
 
-// Row ranges into which the dK/dV kernel's sums are split when there are few key tiles: workgroups of very different
-// lengths (causal) fill 256 CUs evenly once there are several times 512 of them (two fit a CU).  Each range costs a
-// pass over fp32 dK and dV, so it should have 512 rows at least on the average.
-int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv) {
-  const i64 tiles = (total_k / BM + num_seqs) * Hkv, rows = num_seqs ? total_q * (Hq / Hkv) / num_seqs : 0;
-  i64 s = tiles > 0 ? 1024 / tiles : 1;
-  if (s > rows / 512) s = rows / 512;
-  return (int)(s < 1 ? 1 : s > 8 ? 8 : s);
+// Wavefronts of a dK/dV workgroup.  bf16 rows of 96 elements and more: 8 wavefronts, 256 keys, share a tile of queries,
+// because two workgroups of 4 would ask for 16 bytes of direct loads per clock and CU, which is all there is (8192 tokens,
+// 16/4 heads of 128, causal: 805 us with 4, 600 with 8).
+template <typename T>
+constexpr int dkv_waves(int DP) { return sizeof(T) == 2 && DP >= 96 ? 8 : WAVES; }
+// Row ranges into which their sums are split when there are few key tiles: `fit` workgroups run at once (one of 8 wavefronts
+// a CU, one of fp32, else two), and where lengths differ as much as under a causal mask it takes twice as many to fill the GPU
+// evenly.  Each range costs a pass over fp32 dK and dV, so it should have 256 rows at least on the average.  A power of
+// two, so that workgroups of one range and head keep to one XCD and its L2 (workgroups go round over the 8 XCDs): with 5 or
+// 7 ranges the case above is 6 % slower than with 4; with one range it takes 1.9 ms.
+template <typename T>
+int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, bool causal) {
+  const int nw = dkv_waves<T>(padded_dim(D)), fit = sizeof(T) == 2 && nw == 4 ? 512 : 256;
+  const i64 t = (total_k + COLS * nw - 1) / (COLS * nw), tiles = (t > num_seqs ? t : num_seqs) * Hkv;
+  const i64 rows = num_seqs ? total_q * (Hq / Hkv) / num_seqs : 0;
+  int s = 1;
+  while (s < 8 && s * tiles < fit * (causal ? 6 : 3) / 4 && 2 * s * 256 <= rows) s *= 2;
+  return s;
 }
-size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
+inline size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
   return splits > 1 ? (size_t)splits * total_q * Hq * (D + 2) * sizeof(float) : 0;
 }
-size_t delta_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * sizeof(float) + 15) / 16 * 16; }
+inline size_t delta_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * sizeof(float) + 15) / 16 * 16; }
 
 // f(DP, FAST) with the head dimension padded to the tile's, and whether the streamed rows are whole aligned chunks.
-template <typename T, typename F>
+template <typename F>
 void with_dim(int D, bool fast, F f) {
   auto padded = [&](auto dp) {
     if (fast) f(dp, std::true_type());
@@ -1060,7 +1103,18 @@ void with_dim(int D, bool fast, F f) {
   };
   if (D <= 32) padded(std::integral_constant<int, 32>());
   else if (D <= 64) padded(std::integral_constant<int, 64>());
+  else if (D <= 96) padded(std::integral_constant<int, 96>());
   else padded(std::integral_constant<int, 128>());
+}
+// f(WK): the shared kernels exist for whole chunks; other inputs take workgroups of 128 queries whatever their number.
+template <typename T, int DP, bool FAST, typename F>
+void with_shared(int wk, F f) {
+  if constexpr (FAST) {
+    if constexpr (most_shared<T>(DP) == 4)
+      if (wk == 4) return f(std::integral_constant<int, 4>());
+    if (wk >= 2) return f(std::integral_constant<int, 2>());
+  }
+  f(std::integral_constant<int, 1>());
 }
 template <typename T>
 bool whole_chunks(const T *p, i64 ld, int D) {
@@ -1079,19 +1133,21 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   UNET_REQUIRE(aligned<float>(lse), "%s: lse is misaligned", name);
   if (num_seqs == 0 || total_q == 0) return UNET_OK;
   a.out = out, a.out_ld = out_ld, a.lse = lse;
-  const Plan plan = forward_plan(num_seqs, total_q, total_k, Hq, Hkv, wk_of<T>(D));
-  a.tiles = plan.tiles, a.splits = plan.splits, a.partials = (float *)ws;
+  const bool whole = whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D);
+  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D);
+  a.tiles = whole ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+  a.splits = plan.splits, a.partials = (float *)ws;
   if (plan.splits > 1) {
     const size_t need = forward_bytes(total_q, Hq, D, plan.splits);
     UNET_REQUIRE(ws && ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
     UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
   }
-  with_dim<T>(D, whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D), [&](auto dp, auto fast) {
+  with_dim(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool FAST = decltype(fast)::value;
-    const unsigned grid = (unsigned)a.tiles * Hkv * a.splits;
-    if (plan.shared) attention_kernel<T, DP, FAST, shared_waves<T>(DP)><<<grid, 256, 0, st>>>(a);
-    else attention_kernel<T, DP, FAST, 1><<<grid, 256, 0, st>>>(a);
+    with_shared<T, DP, FAST>(plan.wk, [&](auto wk) {
+      attention_kernel<T, DP, FAST, decltype(wk)::value><<<(unsigned)a.tiles * Hkv * a.splits, 256, 0, st>>>(a);
+    });
   });
   if (a.splits > 1) attention_join_kernel<T><<<cdiv_u(total_q * Hq, WAVES), 256, 0, st>>>(a);
   UNET_LAUNCH_CHECK(name);
@@ -1119,17 +1175,22 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   if (num_seqs == 0 || (total_q == 0 && total_k == 0)) return UNET_OK;
   a.dout = dout, a.o = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = const_cast<float *>(lse), a.delta = (float *)ws;
   a.dout_ld = dout_ld, a.o_ld = out_ld, a.dq_ld = dq_ld, a.dk_ld = dk_ld, a.dv_ld = dv_ld;
-  a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
-  const unsigned key_tiles = (unsigned)(total_k / BM) + num_seqs;
-  a.splits = dkv_splits(num_seqs, total_q, total_k, Hq, Hkv);
-  a.partials = (float *)((char *)ws + delta_bytes(total_q, Hq));
   const bool whole =
       whole_chunks(q, q_ld, D) && whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D) && whole_chunks(dout, dout_ld, D);
-  with_dim<T>(D, whole, [&](auto dp, auto fast) {
-    constexpr int DP = decltype(dp)::value;
+  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D);
+  a.tiles = whole ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+  const int nw = dkv_waves<T>(padded_dim(D));
+  const unsigned key_tiles = (unsigned)(total_k / (COLS * nw)) + num_seqs;
+  a.splits = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
+  a.partials = (float *)((char *)ws + delta_bytes(total_q, Hq));
+  with_dim(D, whole, [&](auto dp, auto fast) {
+    constexpr int DP = decltype(dp)::value, NW = dkv_waves<T>(DP);
     constexpr bool FAST = decltype(fast)::value;
-    if (total_q) attention_dq_kernel<T, DP, FAST><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
-    if (total_k) attention_dkv_kernel<T, DP, FAST><<<key_tiles * Hkv * a.splits, 256, 0, st>>>(a);
+    if (total_q)
+      with_shared<T, DP, FAST>(plan.wk, [&](auto wk) {
+        attention_dq_kernel<T, DP, FAST, decltype(wk)::value><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
+      });
+    if (total_k) attention_dkv_kernel<T, DP, FAST, NW><<<key_tiles * Hkv * a.splits, 64 * NW, 0, st>>>(a);
   });
   if (total_k && a.splits > 1) attention_dkv_join_kernel<T><<<ew_grid(total_k * Hkv * D), 256, 0, st>>>(a);
   UNET_LAUNCH_CHECK(name);
@@ -1137,69 +1198,3 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
 }
 
 }  // namespace
-
-extern "C" {
-
-int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv,
-                                       int head_dim, size_t *bytes_host) {
-  UNET_REQUIRE(bytes_host, "dot_attention_workspace_bytes: NULL result");
-  TRY(check_shape("dot_attention_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  // the larger of the two types' plans
-  size_t need = 0;
-  for (const int wk : {wk_of<float>(head_dim), wk_of<bf16_t>(head_dim)}) {
-    const size_t n = forward_bytes(total_q, heads_q, head_dim, forward_plan(num_seqs, total_q, total_k, heads_q, heads_kv, wk).splits);
-    if (n > need) need = n;
-  }
-  *bytes_host = need;
-  return UNET_OK;
-}
-int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
-                                                int heads_kv, int head_dim, size_t *bytes_host) {
-  UNET_REQUIRE(bytes_host, "dot_attention_backward_workspace_bytes: NULL result");
-  TRY(check_shape("dot_attention_backward_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  const int splits = dkv_splits(num_seqs, total_q, total_k, heads_q, heads_kv);
-  *bytes_host = delta_bytes(total_q, heads_q) +
-                (splits > 1 ? (size_t)splits * 2 * total_k * heads_kv * head_dim * sizeof(float) : 0);
-  return UNET_OK;
-}
-
-int unet_dot_attention_f32(const float *q, int64_t q_ld, const float *k, int64_t k_ld, const float *v, int64_t v_ld,
-                           float *out, int64_t out_ld, float *lse, const int32_t *cu_q, const int32_t *cu_k,
-                           int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv, int head_dim,
-                           float scale, int causal, void *workspace, size_t workspace_bytes, unet_stream_t stream) {
-  return forward<float>(q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, cu_q, cu_k, num_seqs, total_q, total_k, heads_q,
-                        heads_kv, head_dim, scale, causal, workspace, workspace_bytes, as_stream(stream));
-}
-int unet_dot_attention_bf16(const uint16_t *q, int64_t q_ld, const uint16_t *k, int64_t k_ld, const uint16_t *v,
-                            int64_t v_ld, uint16_t *out, int64_t out_ld, float *lse, const int32_t *cu_q,
-                            const int32_t *cu_k, int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
-                            int heads_kv, int head_dim, float scale, int causal, void *workspace,
-                            size_t workspace_bytes, unet_stream_t stream) {
-  return forward<bf16_t>(q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, cu_q, cu_k, num_seqs, total_q, total_k, heads_q,
-                         heads_kv, head_dim, scale, causal, workspace, workspace_bytes, as_stream(stream));
-}
-int unet_dot_attention_backward_f32(const float *grad_out, int64_t grad_out_ld, const float *q, int64_t q_ld,
-                                    const float *k, int64_t k_ld, const float *v, int64_t v_ld, const float *out,
-                                    int64_t out_ld, const float *lse, float *grad_q, int64_t grad_q_ld, float *grad_k,
-                                    int64_t grad_k_ld, float *grad_v, int64_t grad_v_ld, const int32_t *cu_q,
-                                    const int32_t *cu_k, int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
-                                    int heads_kv, int head_dim, float scale, int causal, void *workspace,
-                                    size_t workspace_bytes, unet_stream_t stream) {
-  return backward<float>(grad_out, grad_out_ld, q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, grad_q, grad_q_ld, grad_k,
-                         grad_k_ld, grad_v, grad_v_ld, cu_q, cu_k, num_seqs, total_q, total_k, heads_q, heads_kv, head_dim,
-                         scale, causal, workspace, workspace_bytes, as_stream(stream));
-}
-int unet_dot_attention_backward_bf16(const uint16_t *grad_out, int64_t grad_out_ld, const uint16_t *q, int64_t q_ld,
-                                     const uint16_t *k, int64_t k_ld, const uint16_t *v, int64_t v_ld,
-                                     const uint16_t *out, int64_t out_ld, const float *lse, uint16_t *grad_q,
-                                     int64_t grad_q_ld, uint16_t *grad_k, int64_t grad_k_ld, uint16_t *grad_v,
-                                     int64_t grad_v_ld, const int32_t *cu_q, const int32_t *cu_k, int num_seqs,
-                                     int64_t total_q, int64_t total_k, int heads_q, int heads_kv, int head_dim,
-                                     float scale, int causal, void *workspace, size_t workspace_bytes,
-                                     unet_stream_t stream) {
-  return backward<bf16_t>(grad_out, grad_out_ld, q, q_ld, k, k_ld, v, v_ld, out, out_ld, lse, grad_q, grad_q_ld, grad_k,
-                          grad_k_ld, grad_v, grad_v_ld, cu_q, cu_k, num_seqs, total_q, total_k, heads_q, heads_kv, head_dim,
-                          scale, causal, workspace, workspace_bytes, as_stream(stream));
-}
-
-}  // extern "C"
