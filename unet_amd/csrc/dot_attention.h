@@ -99,7 +99,8 @@ struct Args {
   const T *q, *k, *v, *o, *dout;
   T *out, *dq, *dk, *dv;
   i64 q_ld, k_ld, v_ld, o_ld, dout_ld, out_ld, dq_ld, dk_ld, dv_ld;
-  float *lse, *delta, *partials;
+  float *lse, *partials;
+  float *rows;  // for the dK/dV kernel: lse in base 2, then delta, [total_q][Hq] each
   const int *cu_q, *cu_k;
   int num_seqs, total_q, total_k, Hq, Hkv, D, causal, tiles, splits;
   Div G;
@@ -109,38 +110,38 @@ struct Args {
 // Bounds of a sequence, inside [0, total] whatever the array holds.
 __device__ __forceinline__ int bound_of(const int *cu, int s, int total) { return min(max(cu[s], 0), total); }
 
-// The sequence and first row of tile `tile` where sequence s owns the tiles from floor(start(s) * g / BM) + s on: at
-// least ceil(len * g / BM) of them, without a prefix sum over the lengths.  Tiles behind the last row are empty.
-struct Where {
-  int seq, row0;
-};
-// The lanes look at 64 sequences at once: one load's latency for up to 64 sequences, two for up to 4096.
-template <int TILE>
-__device__ __forceinline__ Where find_tile(const int *cu, int num_seqs, int total, int g, int tile) {
-  auto first_tile = [&](int s) __attribute__((always_inline)) { return (bound_of(cu, s, total) * g) / TILE + s; };
-  int lo = 0, n = num_seqs;
-  while (n > 1) {
-    const int step = (n + 63) >> 6, s = lo + (int)(threadIdx.x & 63) * step;
-    const bool before = (threadIdx.x & 63) == 0 || (s < lo + n && first_tile(s) <= tile);
-    const int count = __popcll(__ballot(before));  // bounds do not decrease: these are the first lanes
-    const int skip = (count - 1) * step;
-    n = min(step, n - skip);
-    lo += skip;
-  }
-  lo = __builtin_amdgcn_readfirstlane(lo);
-  return Where{lo, (tile - first_tile(lo)) * TILE};
-}
 struct Seq {
   int q0, nq, k0, nk;  // first query / key and their numbers
 };
-template <typename A>
-__device__ __forceinline__ Seq seq_of(const A &a, int s) {
-  Seq r;
-  r.q0 = bound_of(a.cu_q, s, a.total_q);
-  r.nq = max(bound_of(a.cu_q, s + 1, a.total_q) - r.q0, 0);
-  r.k0 = bound_of(a.cu_k, s, a.total_k);
-  r.nk = max(bound_of(a.cu_k, s + 1, a.total_k) - r.k0, 0);
-  return r;
+// The sequence of tile `tile` and the tile's first row in it, where sequence s owns the tiles from floor(start(s) * g / TILE) + s
+// on (start in queries, or in keys where KEYS): at least ceil(len * g / TILE) of them, without a prefix sum over the
+// lengths.  Tiles in front of the first or behind the last row of their sequence are empty.  The lanes look at 64
+// sequences at once: up to 63 sequences cost the latency of one load.
+template <int TILE, bool KEYS, typename A>
+__device__ __forceinline__ Seq locate(const A &a, int g, int tile, int &row0) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0, q0, q1, k0, k1;
+  if (a.num_seqs < 64) {
+    const int s = min(lane, a.num_seqs), vq = bound_of(a.cu_q, s, a.total_q), vk = bound_of(a.cu_k, s, a.total_k);
+    // bounds do not decrease: the sequences that begin at or before the tile are the first lanes
+    lo = __popcll(__ballot(lane == 0 || (lane < a.num_seqs && ((KEYS ? vk : vq) * g) / TILE + lane <= tile))) - 1;
+    q0 = __builtin_amdgcn_readlane(vq, lo), q1 = __builtin_amdgcn_readlane(vq, lo + 1);
+    k0 = __builtin_amdgcn_readlane(vk, lo), k1 = __builtin_amdgcn_readlane(vk, lo + 1);
+  } else {
+    const int *const cu = KEYS ? a.cu_k : a.cu_q, total = KEYS ? a.total_k : a.total_q;
+    for (int n = a.num_seqs; n > 1;) {
+      const int step = (n + 63) >> 6, s = lo + lane * step;
+      const bool before = lane == 0 || (s < lo + n && (bound_of(cu, s, total) * g) / TILE + s <= tile);
+      const int skip = (__popcll(__ballot(before)) - 1) * step;
+      n = min(step, n - skip);
+      lo += skip;
+    }
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    q0 = bound_of(a.cu_q, lo, a.total_q), q1 = bound_of(a.cu_q, lo + 1, a.total_q);
+    k0 = bound_of(a.cu_k, lo, a.total_k), k1 = bound_of(a.cu_k, lo + 1, a.total_k);
+  }
+  row0 = (tile - (((KEYS ? k0 : q0) * g) / TILE + lo)) * TILE;
+  return Seq{q0, max(q1 - q0, 0), k0, max(k1 - k0, 0)};
 }
 
 // ---- tiles in LDS ----------------------------------------------------------------------------------------
@@ -333,17 +334,28 @@ struct Tile {
   }
 };
 
-// Eight consecutive elements p[0..8), zero from element n on, as (half of) a B operand.
-template <typename T>
-__device__ __forceinline__ Frag<T> load_frag(const T *p, int n) {
+// Eight consecutive elements p[e..e+8) of a row of D, zero from element D on, as (half of) a B operand.  WHOLE: D is a
+// multiple of the elements in 16 bytes; then without branches, from the row's first elements where there are none.
+template <typename T, bool WHOLE>
+__device__ __forceinline__ Frag<T> load_frag(const T *p, int e, int D) {
   Frag<T> f;
-  if (n >= 8) {
-    __builtin_memcpy(&f, p, sizeof(f));
-  } else {
-    T e[8];
+  const int n = D - e;
+  if constexpr (WHOLE) {
+    constexpr int N = 16 / (int)sizeof(T);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = i < n ? p[i] : (T)0;
-    __builtin_memcpy(&f, e, sizeof(f));
+    for (int i = 0; i < 8; i += N) {
+      u32x4 v;
+      __builtin_memcpy(&v, p + (i < n ? e + i : 0), 16);
+      if (i >= n) v = u32x4{0, 0, 0, 0};
+      __builtin_memcpy((char *)&f + i * sizeof(T), &v, 16);
+    }
+  } else if (n >= 8) {
+    __builtin_memcpy(&f, p + e, sizeof(f));
+  } else {
+    T x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < n ? p[e + i] : (T)0;
+    __builtin_memcpy(&f, x, sizeof(f));
   }
   return f;
 }
@@ -387,10 +399,8 @@ struct Rows {
 template <int BQ, typename T>
 __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int wave, Rows &r, int &row0) {
   const int g = (int)a.G.by;
-  const Where w = find_tile<BQ>(a.cu_q, a.num_seqs, a.total_q, g, tile);
-  r.s = seq_of(a, w.seq);
+  r.s = locate<BQ, false>(a, g, tile, row0);
   r.nrows = r.s.nq * g;
-  row0 = w.row0;
   if (row0 < 0 || row0 >= r.nrows) return false;
   r.off = r.s.nk - r.s.nq;
   r.row = row0 + wave * COLS + (threadIdx.x & 31);
@@ -409,28 +419,31 @@ __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int
 template <typename T, int DP, bool FAST, int WK>
 constexpr int tile_rows() { return WK > 1 ? 32 * WK : DP * sizeof(T) >= (FAST && sizeof(T) == 2 ? 257 : 192) ? 32 : 64; }
 
-// Runs step(tile, buffer) for the tiles [0, n) with the next tile on its way to the other buffer.  One barrier per tile:
-// behind it every wavefront has left the buffer that is written next, and sees the one that is read next.
-//   FAST: move(t, buffer) starts the direct loads of tile t, which are waited for in front of tile t's barrier;
-//         put(buffer) writes what the tile needs besides them.
-//   else: fetch(t) loads tile t to registers, put(buffer) writes them to LDS.
-template <bool FAST, typename Move, typename Fetch, typename Put, typename Step>
+// Runs step(tile, buffer) for the tiles [0, n), the next tiles on their way to other buffers.  One barrier per tile: behind
+// it every wavefront has left the buffer that is written next, and sees the one that is read next.
+//   FAST: move(t, buffer) starts the direct loads of tile t, at least PER of them per wavefront, into one of NB buffers; tile t
+//         is waited for in front of its barrier, while the NB - 2 tiles behind it may be in flight.  The loop has no
+//         other vector memory instructions: a wait of the compiler's for one of those would be for all direct loads as well.
+//   else: fetch(t) loads tile t to registers, put(buffer) writes them to one of two buffers.
+template <bool FAST, int NB, int PER, typename Move, typename Fetch, typename Put, typename Step>
 __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, Step step) {
+  static_assert(NB == 2 || (FAST && NB == 3), "two or three buffers");
   if (n <= 0) return;
-  fetch(0);
   if constexpr (FAST) {
     move(0, 0);
+    if (NB == 3 && n > 1) move(1, 1);
+    int buf = 0;
 #pragma unroll 1
     for (int t = 0; t < n; ++t) {
-      put(t & 1);
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (t + 1 < n) {
-        move(t + 1, (t + 1) & 1);
-        fetch(t + 1);
-      }
-      step(t, t & 1);
+      if (NB == 3 && t + 1 < n) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(PER) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      const int free = buf == 0 ? NB - 1 : buf - 1;
+      if (t + NB - 1 < n) move(t + NB - 1, free);
+      step(t, buf);
+      buf = buf == NB - 1 ? 0 : buf + 1;
     }
   } else {
+    fetch(0);
     put(0);
     fetch(1);
 #pragma unroll 1
@@ -444,6 +457,11 @@ __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, S
     }
   }
 }
+// Buffers: three where the LDS of two or three workgroups a CU has room for them (short sequences spend their time waiting for the first
+// tiles: 16 x 256 tokens, 16 heads of 64, TODO).
+template <typename T, int DP, bool FAST, int WK>
+constexpr int buffers() { return FAST && sizeof(T) == 2 && DP <= 64 && WK < 4 ? 3 : 2; }
+
 // Whether the registers are to be limited so that two workgroups fit a CU (the LDS of WK = 4 at 96 elements and more, and the
 // operands of fp32, allow one).
 template <typename T, int DP, int WK>
@@ -472,6 +490,15 @@ __device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], const float *all, i
       }
 }
 
+// LDS[lds + 4 * lane] = the number at byte offset `at` from base, 0 at NOWHERE.
+__device__ __forceinline__ void direct_load_dword(const float *base, unsigned at, unsigned lds) {
+  const uint64_t b = (uint64_t)base;
+  const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)b), __builtin_amdgcn_readfirstlane((int)(b >> 32)), (int)NOWHERE,
+                      0x00020000};
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at), "s"(rsrc));
+}
 // Where a workgroup's LDS array begins, as the direct loads want it.
 __device__ __forceinline__ unsigned lds_address(unsigned char *lds) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds;
@@ -538,8 +565,8 @@ template <typename T, int DP, bool FAST, int WK>
 __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_kernel(const Args<T> a) {
   constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS> TL;
-  constexpr int STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
-  __shared__ __align__(16) unsigned char lds[(2 * STAGE > MERGE ? 2 * STAGE : MERGE) + TL::ZEROS];
+  constexpr int NB = buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
+  __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits, t0 = bs / a.splits;
@@ -555,7 +582,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   {
     const T *p = a.q + (i64)(r.s.q0 + r.query) * a.q_ld + r.head * a.D;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) q[t] = load_frag<T>(p + 16 * t + 8 * h, r.live ? a.D - 16 * t - 8 * h : 0);
+    for (int t = 0; t < DP / 16; ++t) q[t] = load_frag<T, FAST>(p, 16 * t + 8 * h, a.D);
   }
   f32x16 acc[DB];
 #pragma unroll
@@ -633,7 +660,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
               [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
-  stream<FAST>(n, move, fetch, put, step);
+  stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step);
   l += __shfl_xor(l, 32, 64);
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
@@ -709,13 +736,13 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args<T> a) {
   if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// dQ, and delta for the kernel below.  WK as in the forward.
+// dQ, and lse and delta for the kernel below.  WK as in the forward.
 template <typename T, int DP, bool FAST, int WK>
 __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_dq_kernel(const Args<T> a) {
   constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = tile_rows<T, DP, FAST, WK>(), NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS> TL;
-  constexpr int STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * DB * 16 * 4;
-  __shared__ __align__(16) unsigned char lds[(2 * STAGE > MERGE ? 2 * STAGE : MERGE) + TL::ZEROS];
+  constexpr int NB = buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * DB * 16 * 4;
+  __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
   const int kvh = blockIdx.x % a.Hkv;
@@ -736,17 +763,17 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
             *po = a.o + token * a.o_ld + r.head * a.D;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
-      const int e = 16 * t + 8 * h, n = r.live ? a.D - e : 0;
-      q[t] = load_frag<T>(p + e, n);
-      dout[t] = load_frag<T>(pd + e, n);
-      const Frag<T> o = load_frag<T>(po + e, n);
+      const int e = 16 * t + 8 * h;
+      q[t] = load_frag<T, FAST>(p, e, a.D);
+      dout[t] = load_frag<T, FAST>(pd, e, a.D);
+      const Frag<T> o = load_frag<T, FAST>(po, e, a.D);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta += (float)dout[t][j] * (float)o[j];
     }
     delta += __shfl_xor(delta, 32, 64);
   }
   const i64 at = (i64)(r.s.q0 + r.query) * a.Hq + r.head;
-  const float lse2 = r.live ? a.lse[at] * LOG2E : INFINITY;  // a row that does not exist has no weight anywhere
+  const float lse2 = a.lse[at] * LOG2E;  // (a row that does not exist repeats the last one and is not stored)
 
   f32x16 acc[DP / 32];
 #pragma unroll
@@ -799,7 +826,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
       TL::add(acc, k32, zeros, lo, s, edge, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
-  stream<FAST>((span.kend + ROWS - 1) / ROWS, move, fetch, put, step);
+  stream<FAST, NB, 2 * TL::MOVES>((span.kend + ROWS - 1) / ROWS, move, fetch, put, step);
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
     __syncthreads();
@@ -813,7 +840,10 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
     join_sums<WK>(acc, reinterpret_cast<const float *>(lds) + wq * 64 + lane, 0, f, db0, db1);
   }
   if (!r.live) return;
-  if (h == 0 && wk == 0) a.delta[at] = delta;  // the wavefront that has seen the first keys
+  if (h == 0 && wk == 0) {  // the wavefront that has seen the first keys
+    a.rows[at] = lse2;
+    a.rows[at + (i64)a.total_q * a.Hq] = delta;
+  }
   store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale, db0, db1);
 }
 
@@ -822,38 +852,39 @@ template <typename T, int DP, bool FAST, int NW>
 __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(const Args<T> a) {
   constexpr int ROWS = tile_rows<T, DP, FAST, 1>();
   typedef Tile<T, DP, ROWS, NW> TL;
-  constexpr int STAGE = 2 * TL::BYTES + 2 * ROWS * 4;  // Q, dout, lse (base 2), delta
+  constexpr int STAGE = 2 * TL::BYTES + 2 * 64 * 4;  // Q, dout, lse (base 2), delta (64 values: a wavefront's direct load)
+  constexpr int NB = buffers<T, DP, FAST, 1>();
   // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands, and the last
   // two of K, stay in LDS, each wavefront's own, in the order in which the lanes read them.  (With six more registers
   // in use one operand was reloaded from scratch memory in every step, behind the direct loads in flight: 1004 us
   // instead of 805-830, 8192 tokens, 16/4 heads, causal.)
   constexpr int KT = DP / 16, K_REG = DP < 128 ? KT : KT - 2, V_REG = DP < 128 ? KT : 0;
   constexpr int OWN = (2 * KT - K_REG - V_REG) * 64 * (int)sizeof(Frag<T>);
-  __shared__ __align__(16) unsigned char lds[2 * STAGE + TL::ZEROS + NW * OWN];
-  unsigned char *const zeros = lds + 2 * STAGE;
+  __shared__ __align__(16) unsigned char lds[NB * STAGE + TL::ZEROS + NW * OWN];
+  unsigned char *const zeros = lds + NB * STAGE;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits;
-  const Where w = find_tile<COLS * NW>(a.cu_k, a.num_seqs, a.total_k, 1, bs / a.splits);
-  const Seq s = seq_of(a, w.seq);
-  if (w.row0 < 0 || w.row0 >= s.nk) return;
+  int key0;
+  const Seq s = locate<COLS * NW, true>(a, 1, bs / a.splits, key0);
+  if (key0 < 0 || key0 >= s.nk) return;
   TL::clear(zeros);
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index();
   const auto lane_at = TL::lane_offsets(lane);
   const int g = (int)a.G.by, off = s.nk - s.nq;
-  const int wkey = w.row0 + wave * COLS, key = wkey + (lane & 31);
+  const int wkey = key0 + wave * COLS, key = wkey + (lane & 31);
   const bool live = key < s.nk;
 
   Frag<T> kr[K_REG], vr[V_REG ? V_REG : 1];
-  Frag<T> *const own = reinterpret_cast<Frag<T> *>(lds + 2 * STAGE + TL::ZEROS + wave * OWN) + lane;
+  Frag<T> *const own = reinterpret_cast<Frag<T> *>(lds + NB * STAGE + TL::ZEROS + wave * OWN) + lane;
   {
     const i64 token = s.k0 + min(key, s.nk - 1);
     const T *pk = a.k + token * a.k_ld + kvh * a.D, *pv = a.v + token * a.v_ld + kvh * a.D;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const int e = 16 * t + 8 * h, n = live ? a.D - e : 0;
-      if (t < K_REG) kr[t] = load_frag<T>(pk + e, n);
-      else own[64 * (KT - V_REG + t - K_REG)] = load_frag<T>(pk + e, n);
-      if (t < V_REG) vr[t] = load_frag<T>(pv + e, n);
-      else own[64 * (t - V_REG)] = load_frag<T>(pv + e, n);
+      const Frag<T> fk = load_frag<T, FAST>(pk, 16 * t + 8 * h, a.D), fv = load_frag<T, FAST>(pv, 16 * t + 8 * h, a.D);
+      if (t < K_REG) kr[t] = fk;
+      else own[64 * (KT - V_REG + t - K_REG)] = fk;
+      if (t < V_REG) vr[t] = fv;
+      else own[64 * (t - V_REG)] = fv;
     }
   }
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -861,7 +892,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
   for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = zero16();
 
   // the rows that see a key: from the first query that sees the first key of the workgroup / the last one of the wavefront
-  int first = a.causal ? min(max(w.row0 - off, 0), s.nq) * g : 0, nrows = s.nq * g;
+  int first = a.causal ? min(max(key0 - off, 0), s.nq) * g : 0, nrows = s.nq * g;
   if (a.splits > 1) {  // this workgroup's share of them
     const int per = (((nrows - first + ROWS - 1) / ROWS + a.splits - 1) / a.splits) * ROWS;
     first = (int)min((i64)nrows, first + (i64)split * per);
@@ -891,6 +922,11 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
     const i64 token = s.q0 + query0;
     TL::move(a.q + token * a.q_ld + kvh * g * a.D, NOWHERE, qo, lds0 + buf * STAGE);
     TL::move(a.dout + token * a.dout_ld + kvh * g * a.D, NOWHERE, dof, lds0 + buf * STAGE + TL::BYTES);
+    if (wave < 2) {  // lse, delta; zeros where there is no row: with Q and dout zero as well, it adds nothing
+      const int r = r0 + lane, query = div_by(r, a.G);
+      const unsigned at = lane < ROWS && r < nrows ? (unsigned)((query - query0) * a.Hq + (r - query * g)) * 4u : NOWHERE;
+      direct_load_dword(a.rows + ((i64)wave * a.total_q + token) * a.Hq + kvh * g, at, lds0 + buf * STAGE + 2 * TL::BYTES + wave * 256u);
+    }
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
     const int r0 = first + t * ROWS;
@@ -898,30 +934,28 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
       TL::fetch(cq, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.q, a.q_ld, r); });
       TL::fetch(cd, r0, nrows, a.D, [&](int r) __attribute__((always_inline)) { return row_of(a.dout, a.dout_ld, r); });
     }
-    fl = INFINITY, fd = 0.f;  // rows that do not exist have no weight
+    fl = fd = 0.f;
     const int r = r0 + (int)threadIdx.x;
-    if (threadIdx.x < ROWS && r < nrows) {
+    if (!FAST && threadIdx.x < ROWS && r < nrows) {
       const int query = div_by(r, a.G);
       const i64 at = (i64)(s.q0 + query) * a.Hq + kvh * g + (r - query * g);
-      fl = a.lse[at] * LOG2E;
-      fd = a.delta[at];
+      fl = a.rows[at];
+      fd = a.rows[at + (i64)a.total_q * a.Hq];
     }
   };
   auto put = [&](int buf) __attribute__((always_inline)) {
     unsigned char *const st = lds + buf * STAGE;
-    if (!FAST) {
-      TL::put(cq, st);
-      TL::put(cd, st + TL::BYTES);
-    }
+    TL::put(cq, st);
+    TL::put(cd, st + TL::BYTES);
     if (threadIdx.x < ROWS) {
       float *const f = reinterpret_cast<float *>(st + 2 * TL::BYTES) + threadIdx.x;
       f[0] = fl;
-      f[ROWS] = fd;
+      f[64] = fd;
     }
   };
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const unsigned char *const ldsQ = lds + buf * STAGE, *const ldsD = ldsQ + TL::BYTES;
-    const float *const ldsL = reinterpret_cast<const float *>(ldsD + TL::BYTES), *const ldsDelta = ldsL + ROWS;
+    const float *const ldsL = reinterpret_cast<const float *>(ldsD + TL::BYTES), *const ldsDelta = ldsL + 64;
 #pragma unroll 1
     for (int u = 0; u < ROWS / 32; ++u) {
       const int rb = first + t * ROWS + u * 32;
@@ -959,7 +993,7 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
       TL::add(dk, q32, zeros, lo, ds, edge, sees);
     }
   };
-  stream<FAST>((nrows - first + ROWS - 1) / ROWS, move, fetch, put, step);
+  stream<FAST, NB, 2 * TL::MOVES>((nrows - first + ROWS - 1) / ROWS, move, fetch, put, step);
   if (!live) return;
   if (a.splits > 1) {
     const i64 at = ((i64)(s.k0 + key) * a.Hkv + kvh) * a.D, plane = (i64)a.total_k * a.Hkv * a.D;
@@ -1092,7 +1126,7 @@ int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
 inline size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
   return splits > 1 ? (size_t)splits * total_q * Hq * (D + 2) * sizeof(float) : 0;
 }
-inline size_t delta_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * sizeof(float) + 15) / 16 * 16; }
+inline size_t rows_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * 2 * sizeof(float) + 15) / 16 * 16; }
 
 // f(DP, FAST) with the head dimension padded to the tile's, and whether the streamed rows are whole aligned chunks.
 template <typename F>
@@ -1173,7 +1207,7 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   UNET_REQUIRE(ws_bytes >= need && (ws || !need), "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
   UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
   if (num_seqs == 0 || (total_q == 0 && total_k == 0)) return UNET_OK;
-  a.dout = dout, a.o = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = const_cast<float *>(lse), a.delta = (float *)ws;
+  a.dout = dout, a.o = out, a.dq = dq, a.dk = dk, a.dv = dv, a.lse = const_cast<float *>(lse), a.rows = (float *)ws;
   a.dout_ld = dout_ld, a.o_ld = out_ld, a.dq_ld = dq_ld, a.dk_ld = dk_ld, a.dv_ld = dv_ld;
   const bool whole =
       whole_chunks(q, q_ld, D) && whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D) && whole_chunks(dout, dout_ld, D);
@@ -1182,7 +1216,7 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   const int nw = dkv_waves<T>(padded_dim(D));
   const unsigned key_tiles = (unsigned)(total_k / (COLS * nw)) + num_seqs;
   a.splits = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
-  a.partials = (float *)((char *)ws + delta_bytes(total_q, Hq));
+  a.partials = (float *)((char *)ws + rows_bytes(total_q, Hq));
   with_dim(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value, NW = dkv_waves<T>(DP);
     constexpr bool FAST = decltype(fast)::value;
