@@ -74,8 +74,13 @@ def last_error():
 
 
 def _wrap(name):
+    fn = None
+
     def call(*args):
-        rc = getattr(lib(), name)(*args)
+        nonlocal fn
+        if fn is None:
+            fn = getattr(lib(), name)
+        rc = fn(*args)
         if rc != 0:
             raise RuntimeError(f"{name}: {last_error()} (status {rc})")
         return rc

@@ -462,10 +462,11 @@ __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, S
 template <typename T, int DP, bool FAST, int WK>
 constexpr int buffers() { return FAST && sizeof(T) == 2 && DP <= 64 && WK < 4 ? 3 : 2; }
 
-// Whether the registers are to be limited so that two workgroups fit a CU (the LDS of WK = 4 at 96 elements and more, and the
-// operands of fp32, allow one).
+// Whether the registers are to be limited so that two workgroups fit a CU.  The LDS of WK = 4 at rows of 256 bytes and more,
+// and the operands of fp32 at 96 elements and more, allow one.  (fp32, 3525 tokens, 8 heads of 64: forward 88 us with one,
+// 81 with two; the dK/dV kernel is slower with two, for lack of registers: 186 and 205.)
 template <typename T, int DP, int WK>
-constexpr bool two_fit() { return sizeof(T) == 2 && (WK < 4 || DP <= 64); }
+constexpr bool two_fit() { return sizeof(T) == 2 ? WK < 4 || DP <= 64 : WK < 4 && DP <= 64; }
 
 // The sums of the wavefronts that share queries, each times its factor, for the blocks [db0, db1) of 32 elements: `all` holds
 // value i of block db of thread t at [(first + db * 16 + i) * 256 + t].
@@ -1074,10 +1075,10 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 }
 
 // How the kernels that keep queries share their work.  wk (see attention_kernel): 128 queries a workgroup when that fills
-// three quarters of the places (two a CU, one in fp32), else 64, and 32 when it is a quarter or less: shorter workgroups fill
+// three quarters of the places (two a CU, one in fp32 behind 64 elements), else 64, and 32 when it is a quarter or less: shorter workgroups fill
 // the GPU evenly, but their tiles serve fewer wavefronts.  Measured, forward in us with 128 / 64 / 32 queries: 512 workgroups of 128
 // (16 x 256 tokens, 16 heads of 64, bf16) 12.6 / 17.4 / 23.6; 332 (8 sequences of up to 2049, 8/2 heads of 80, causal)
-// 52.7 / 42.4 / 73; 224 (fp32, 3525 tokens, 8 heads of 64) 89 / 84 / 117, dQ 124 / 130 / -; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
+// 52.7 / 42.4 / 73; 224 (fp32, 3525 tokens, 8 heads of 64) 82 / 81 / 117; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
 // splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average (what a join costs
 // more would not be won back).
 struct Plan {
@@ -1088,7 +1089,7 @@ constexpr int most_shared(int DP) { return DP * sizeof(T) > 256 ? 2 : 4; }  // t
 constexpr int padded_dim(int D) { return (D + 31) / 32 * 32; }
 template <typename T>
 Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
-  const int most = most_shared<T>(padded_dim(D)), places = sizeof(T) == 2 ? 512 : 256;
+  const int most = most_shared<T>(padded_dim(D)), places = sizeof(T) == 2 || D <= 64 ? 512 : 256;
   const i64 rows = total_q * (Hq / Hkv);
   auto groups = [&](int bq) { const i64 t = (rows + bq - 1) / bq; return (t > num_seqs ? t : num_seqs) * Hkv; };
   Plan p;

@@ -59,19 +59,23 @@ __global__ __launch_bounds__(256) void dropout_kernel(const Args<T> a) {
       row = a.total <= 0xffffffffll ? (i64)((uint32_t)e0 / (uint32_t)a.C) : e0 / a.C;
       col = e0 - row * a.C;
     }
-    const bool whole = n == E && (FLAT || col + E <= a.C);
+    // the thread's elements lie in one row, or in two (C >= 8: the second begins at element `left`), or anywhere (C < 8)
+    const int left = FLAT ? E : (int)min<i64>(E, a.C - col);
+    const bool whole = n == E && left == E;
+    auto at = [&](const T *base, i64 ld, int i) __attribute__((always_inline)) {
+      if (FLAT || a.C >= E) return base + row * ld + col + i + (i >= left ? ld - a.C : 0);
+      const i64 r = (e0 + i) / a.C;
+      return base + r * ld + (e0 + i - r * a.C);
+    };
     float x[E], r[E];
     if (whole) {
       load8(a.x + row * a.x_ld + col, x);
       if (RES) load8(a.res + row * a.res_ld + col, r);
     } else {
-      i64 rr = row, cc = col;
 #pragma unroll
       for (int i = 0; i < E; ++i) {
-        x[i] = i < n ? to_f32(a.x[rr * a.x_ld + cc]) : 0.f;
-        if (RES) r[i] = i < n ? to_f32(a.res[rr * a.res_ld + cc]) : 0.f;
-        if (!FLAT && ++cc == a.C) { cc = 0; ++rr; }
-        else if (FLAT) ++cc;
+        x[i] = i < n ? to_f32(*at(a.x, a.x_ld, i)) : 0.f;
+        if (RES) r[i] = i < n ? to_f32(*at(a.res, a.res_ld, i)) : 0.f;
       }
     }
     const uint32_t b0 = (uint32_t)b, b1 = (uint32_t)((uint64_t)b >> 32);
@@ -103,13 +107,9 @@ __global__ __launch_bounds__(256) void dropout_kernel(const Args<T> a) {
     if (whole) {
       store8(a.out + row * a.out_ld + col, x);
     } else {
-      i64 rr = row, cc = col;
 #pragma unroll
-      for (int i = 0; i < E; ++i) {
-        if (i < n) from_f32(x[i], a.out[rr * a.out_ld + cc]);
-        if (!FLAT && ++cc == a.C) { cc = 0; ++rr; }
-        else if (FLAT) ++cc;
-      }
+      for (int i = 0; i < E; ++i)
+        if (i < n) from_f32(x[i], *const_cast<T *>(at(a.out, a.out_ld, i)));
     }
   }
 }

@@ -5,7 +5,7 @@
 //   dgamma = sum_rows dy * xhat,  dbeta = sum_rows dy
 //
 // Bound by HBM: a few operations per element read or written.  So every tensor is passed over once: a row lives in
-// the registers of a group of G lanes (16 lanes up to 32 pieces of 16 bytes, a wavefront up to 256, the workgroup up
+// the registers of a group of G lanes (16 lanes up to 32 pieces of 16 bytes, 32 or 64 up to 256, the workgroup up
 // to 1024; longer rows are read again by the *_long kernels), which takes the statistics from the registers in two
 // passes (mean, then squared deviations: no cancellation).  Groups walk over rows, gamma and beta stay on the CU
 // across rows (in LDS: in registers they would cost half of the wavefronts), and the next row is requested before the
@@ -307,14 +307,17 @@ __global__ __launch_bounds__(256) void layer_norm_long_columns_kernel(const BwdA
 }
 
 // f(G, NV) with the lanes per row and 16-byte pieces per lane that hold a row of `pieces` pieces; false: too long.
-// The smallest group that holds the row: the fewer lanes share a row, the fewer steps its sums take.
+// The smallest group that holds the row: the fewer lanes share a row, the fewer steps its sums take; three pieces a lane
+// where two or four would leave more than a quarter of the lanes idle.
 template <typename F>
 bool with_row_shape(i64 pieces, F f) {
   using std::integral_constant;
   if (pieces <= 16) f(integral_constant<int, 16>(), integral_constant<int, 1>());
   else if (pieces <= 32) f(integral_constant<int, 16>(), integral_constant<int, 2>());
   else if (pieces <= 64) f(integral_constant<int, 64>(), integral_constant<int, 1>());
+  else if (pieces <= 96) f(integral_constant<int, 32>(), integral_constant<int, 3>());
   else if (pieces <= 128) f(integral_constant<int, 64>(), integral_constant<int, 2>());
+  else if (pieces <= 192) f(integral_constant<int, 64>(), integral_constant<int, 3>());
   else if (pieces <= 256) f(integral_constant<int, 64>(), integral_constant<int, 4>());
   else if (pieces <= 512) f(integral_constant<int, 256>(), integral_constant<int, 2>());
   else if (pieces <= 1024) f(integral_constant<int, 256>(), integral_constant<int, 4>());

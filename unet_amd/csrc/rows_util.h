@@ -90,14 +90,15 @@ __device__ __forceinline__ float pair_sum32(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
-// Sums of NS values over a group of G lanes (16, 64, or the 256 of the workgroup); every lane gets the totals.
+// Sums of NS values over a group of G lanes (16, 32, 64, or the 256 of the workgroup); every lane gets the totals.
 // G = 256: `red` holds 2 x NS x 4 floats and `phase` alternates between its halves, one barrier per sum.
 template <int G, int NS>
 __device__ __forceinline__ void group_sum(float (&v)[NS], float *red, int &phase) {
 #pragma unroll
   for (int s = 0; s < NS; ++s) {
     v[s] = row16_sum(v[s]);
-    if (G > 16) v[s] = pair_sum32(pair_sum16(v[s]));
+    if (G > 16) v[s] = pair_sum16(v[s]);
+    if (G > 32) v[s] = pair_sum32(v[s]);
   }
   if (G == 256) {
     float *r = red + phase * NS * 4;
