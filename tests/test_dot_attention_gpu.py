@@ -142,6 +142,16 @@ def test_split_sums(name, causal, shape):
         assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dim", [96, 128])
+def test_many_queries(causal, dim):
+    """Enough queries for the widest workgroups; a sequence that ends inside one, and queries that see nothing."""
+    c = Call("bf16", [300, 700], [290, 701], 106, 53, dim, causal, behind=2)
+    c.forward()
+    c.backward()
+    c.verify()
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
 def test_split_sums_keep_bad_keys_to_the_queries_that_see_them(bad):
     c = Call("bf16", [2, 1], [4000, 3500], 4, 2, 64, True)

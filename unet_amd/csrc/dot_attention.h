@@ -427,7 +427,7 @@ constexpr int tile_rows() { return WK > 1 ? 32 * WK : DP * sizeof(T) >= (FAST &&
 //   else: fetch(t) loads tile t to registers, put(buffer) writes them to one of two buffers.
 template <bool FAST, int NB, int PER, typename Move, typename Fetch, typename Put, typename Step>
 __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, Step step) {
-  static_assert(NB == 2 || (FAST && NB == 3), "two or three buffers");
+  static_assert(NB == 2 || (FAST && NB == 3), "two buffers, three for direct loads");
   if (n <= 0) return;
   if constexpr (FAST) {
     move(0, 0);
@@ -560,13 +560,13 @@ __device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row
 
 // The forward.  WK wavefronts share the same 32 queries and take the 32-row pieces of a tile in turn: with WK = 1 a
 // workgroup has 128 queries (every tile serves four times 32), with WK > 1 it has fewer, for calls that have too few
-// queries to fill the GPU.  splits > 1: the workgroup takes a share of the key tiles and leaves its sums to
+// queries to fill the GPU.  NW = 8: 256 queries a workgroup, for long rows and many queries (see Plan).  splits > 1: the workgroup takes a share of the key tiles and leaves its sums to
 // attention_join_kernel.
-template <typename T, int DP, bool FAST, int WK>
-__global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_kernel(const Args<T> a) {
-  constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
-  typedef Tile<T, DP, ROWS> TL;
-  constexpr int NB = buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
+template <typename T, int DP, bool FAST, int WK, int NW = WAVES>
+__global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_kernel(const Args<T> a) {
+  constexpr int WQ = NW / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
+  typedef Tile<T, DP, ROWS, NW> TL;
+  constexpr int NB = NW == 8 ? 3 : buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
   __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
@@ -1081,8 +1081,12 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 // 52.7 / 42.4 / 73; 224 (fp32, 3525 tokens, 8 heads of 64) 82 / 81 / 117; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
 // splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average (what a join costs
 // more would not be won back).
+// wide: 8 wavefronts and 256 queries a workgroup (forward, bf16 rows of 96 elements and more): half the direct loads, and room for
+// a third buffer; 8192 tokens, 16/4 heads of 128, causal: 293 -> 275 us.  (dQ gains nothing by it: its two score products
+// take twice as long per tile.)
 struct Plan {
   int wk, splits, tiles;  // tiles of queries: an upper bound
+  bool wide;
 };
 template <typename T>
 constexpr int most_shared(int DP) { return DP * sizeof(T) > 256 ? 2 : 4; }  // the tiles of 4 would not fit the LDS
@@ -1095,6 +1099,7 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
   Plan p;
   const i64 n = groups(BM);
   p.wk = n >= places * 3 / 4 ? 1 : n > places / 4 || most == 2 ? 2 : 4;
+  p.wide = p.wk == 1 && groups(2 * BM) >= 384;
   i64 s = 1;
   if (p.wk == most && num_seqs > 0) {
     s = 256 / groups(BM / p.wk);
@@ -1180,6 +1185,12 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   with_dim(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool FAST = decltype(fast)::value;
+    if constexpr (FAST && sizeof(T) == 2 && DP >= 96)
+      if (plan.wide) {
+        a.tiles = (int)(total_q * (Hq / Hkv) / (2 * BM)) + num_seqs;
+        attention_kernel<T, DP, FAST, 1, 8><<<(unsigned)a.tiles * Hkv, 512, 0, st>>>(a);
+        return;
+      }
     with_shared<T, DP, FAST>(plan.wk, [&](auto wk) {
       attention_kernel<T, DP, FAST, decltype(wk)::value><<<(unsigned)a.tiles * Hkv * a.splits, 256, 0, st>>>(a);
     });
