@@ -297,11 +297,19 @@ struct Tile {
   // weight 0.  If such rows hold infinities or NaN, 0 * inf must not reach a column that does not see them: then the
   // rows are added one at a time, the result taken by the columns that see the row, and the common product reads
   // zeros instead.  Rare, so slow is fine; what matters is that the accumulators stay where they are.
+  // TWICE: a bf16 weight is taken as the sum of two bf16 numbers, its rounding and what that left over.
   static constexpr int ZEROS = 16 * RB;
-  template <typename Sees>
+  template <bool TWICE = false, typename Sees>
   static __device__ __forceinline__ void add(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const unsigned char *zeros,
                                              const Lane &o, const f32x16 &w, bool edge, Sees sees) {
     const Frag<T> b0 = pack8<T>(w, 0), b1 = pack8<T>(w, 1);
+    Frag<T> c0, c1;
+    if constexpr (TWICE) {
+      f32x16 rest;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) rest[i] = w[i] - (float)(i < 8 ? b0[i & 7] : b1[i & 7]);
+      c0 = pack8<T>(rest, 0), c1 = pack8<T>(rest, 1);
+    }
     const unsigned char *low = rows32, *high = rows32 + 16 * RB;
     if (edge && not_finite(rows32, o)) {
       const int h = (threadIdx.x & 63) >> 5;
@@ -309,15 +317,19 @@ struct Tile {
       for (int k = 0; k < 32; ++k) {
         const int j = ((k >> 3) & 1) * 4 + (k & 3);
         const bool mine = ((k >> 2) & 1) == h, seen = sees(k);
-        Frag<T> b;
+        Frag<T> b, c;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) b[x] = k < 16 ? b0[x] : b1[x];
+        for (int x = 0; x < 8; ++x) {
+          b[x] = k < 16 ? b0[x] : b1[x];
+          if constexpr (TWICE) c[x] = k < 16 ? c0[x] : c1[x];
+        }
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) {
           Frag<T> f = down(rows32 + (k & 16) * RB, o, db);
 #pragma unroll
           for (int x = 0; x < 8; ++x) f[x] = mine && x == j ? f[x] : 0;
-          const f32x16 r = mma(f, b, zero16());
+          f32x16 r = mma(f, b, zero16());
+          if constexpr (TWICE) r = mma(f, c, r);
 #pragma unroll
           for (int i = 0; i < 16; ++i) acc[db][i] += seen ? r[i] : 0.f;
         }
@@ -325,9 +337,17 @@ struct Tile {
       low = high = zeros;
     }
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(low, o, db), b0, acc[db]);
+    for (int db = 0; db < DP / 32; ++db) {
+      const Frag<T> x = down(low, o, db);
+      acc[db] = mma(x, b0, acc[db]);
+      if constexpr (TWICE) acc[db] = mma(x, c0, acc[db]);
+    }
 #pragma unroll
-    for (int db = 0; db < DP / 32; ++db) acc[db] = mma(down(high, o, db), b1, acc[db]);
+    for (int db = 0; db < DP / 32; ++db) {
+      const Frag<T> x = down(high, o, db);
+      acc[db] = mma(x, b1, acc[db]);
+      if constexpr (TWICE) acc[db] = mma(x, c1, acc[db]);
+    }
   }
   static __device__ __forceinline__ void clear(unsigned char *zeros) {
     for (int i = threadIdx.x * 16; i < ZEROS; i += NT * 16) *reinterpret_cast<u32x4 *>(zeros + i) = u32x4{0, 0, 0, 0};
@@ -824,7 +844,9 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
-      TL::add(acc, k32, zeros, lo, s, edge, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
+      // dS of a query adds up to zero, so its product with K loses the part that the keys have in common, but the roundings
+      // of dS do not: with few elements (that part is then large beside the rest) they are kept out.
+      TL::template add<sizeof(T) == 2 && DP <= 64>(acc, k32, zeros, lo, s, edge, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
   stream<FAST, NB, 2 * TL::MOVES>((span.kend + ROWS - 1) / ROWS, move, fetch, put, step);
