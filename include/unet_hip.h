@@ -201,7 +201,7 @@ int unet_batch_norm_relu_backward_f32(const float *grad_activations, const float
  *   activations = gamma * (x - mean) * rstd + beta
  * row_stats (may be NULL: inference) receives [mean, rstd] per row for the backward.  Statistics are fp32 from two
  * passes over the values; one rounding to the storage type at the end.  activations may be the inputs' own buffer
- * (same pointer, same stride).  rows = 0 is a valid empty call. */
+ * (same pointer, same stride).  rows = 0 is a valid empty call.  At most 2^26 channels. */
 int unet_layer_norm_f32(const float *inputs, int64_t in_ld, float *activations, int64_t out_ld, const float *weights,
                         float *row_stats, int64_t rows, int channels, float eps, unet_stream_t stream);
 int unet_layer_norm_bf16(const uint16_t *inputs, int64_t in_ld, uint16_t *activations, int64_t out_ld,
@@ -215,7 +215,8 @@ int unet_layer_norm_bf16(const uint16_t *inputs, int64_t in_ld, uint16_t *activa
  * grad_skip or of inputs (same pointer, same stride).  grad_weights (fp32, overwritten) or grad_inputs may be NULL to skip
  * that half.  weights NULL = gamma 1.  Sums over rows have a fixed order: equal calls give equal bits.
  * `workspace` is device memory of at least unet_layer_norm_backward_workspace_bytes() bytes, 16-byte aligned, free
- * for other use once the call's work on `stream` has finished; it may be NULL when grad_weights is.  The calls
+ * for other use once the call's work on `stream` has finished (calls that may run at the same time need one each); it
+ * may be NULL when grad_weights is.  The calls
  * allocate nothing and can be captured into a graph. */
 int unet_layer_norm_backward_workspace_bytes(int64_t rows, int channels, size_t *bytes_host);
 int unet_layer_norm_backward_f32(const float *grad_activations, int64_t grad_ld, const float *inputs, int64_t in_ld,
@@ -365,9 +366,10 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  * does not reach it, whatever it holds (NaN and infinities included).  Rows of out and lse in front of the first or behind
  * the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
  * accumulators are fp32; the bf16 form rounds the softmax weights to bf16 for their product with V.  Equal calls
- * give equal bits.  out must not overlap q, k or v.
+ * give equal bits.  out must not overlap q, k or v.  total_q * heads_q and total_k * heads_kv may be up to about 2^29.
  * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
- * do), 16-byte aligned, free for other use once the call's work on `stream` has finished.  The calls allocate
+ * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the same
+ * time need one each.  The calls allocate
  * nothing and can be captured into a graph. */
 int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv,
                                        int head_dim, size_t *bytes_host);
@@ -383,7 +385,8 @@ int unet_dot_attention_bf16(const uint16_t *q, int64_t q_ld, const uint16_t *k, 
 /* Gradients of the above from grad_out and the forward's out and lse: with P the softmax weights,
  * dP = grad_out V^T and dS = P * (dP - sum_d grad_out * out):
  *   grad_v = P^T grad_out, grad_q = scale * dS K, grad_k = scale * dS^T Q, all overwritten; grad_k and grad_v sum over the query heads that
- * share a key/value head.  The bf16 form rounds P and dS to bf16 for their products.  No atomics: every sum has a
+ * share a key/value head.  The bf16 form rounds P and dS to bf16 for their products (dS for grad_q in two parts up to head_dim
+ * 64).  No atomics: every sum has a
  * fixed order.  Rows outside the sequences are left as they were; keys that no query sees get 0.  The gradients must not
  * overlap the inputs or each other's columns (they may be column slices of one buffer). */
 int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q,

@@ -19,7 +19,7 @@ def ln(x=P, x_ld=8, y=P, y_ld=8, w=P, stats=P, rows=2, c=8, eps=1e-5, f=capi.une
 
 @pytest.mark.parametrize("f", [capi.unet_layer_norm_f32, capi.unet_layer_norm_bf16])
 @pytest.mark.parametrize("bad,match", [(dict(x=None), "NULL"), (dict(y=None), "NULL"), (dict(x_ld=7), "stride"), (dict(y_ld=7), "stride"),
-                                       (dict(rows=-1), "rows"), (dict(c=0), "channels"), (dict(eps=-1.0), "eps"),
+                                       (dict(rows=-1), "rows"), (dict(c=0), "channels"), (dict(c=2 ** 26 + 1, x_ld=2 ** 27, y_ld=2 ** 27), "channels"), (dict(eps=-1.0), "eps"),
                                        (dict(eps=float("nan")), "eps"), (dict(x=P + 1), "misaligned"), (dict(w=P + 2), "misaligned")])
 def test_layer_norm_refuses(f, bad, match):
     with pytest.raises(RuntimeError, match=match):
@@ -72,7 +72,7 @@ ATT = dict(q=P, q_ld=64, k=P, k_ld=32, v=P, v_ld=32, out=P, out_ld=64, lse=P, cu
 SHAPE = [(dict(heads_kv=3), "multiple"), (dict(heads_kv=0), "multiple"), (dict(heads_q=0), "multiple"), (dict(head_dim=0), "head_dim"),
          (dict(head_dim=129, q_ld=4096, k_ld=4096, v_ld=4096, out_ld=4096), "larger than 128"), (dict(num_seqs=-1), "num_seqs"),
          (dict(total_q=-1), "total_q"), (dict(total_k=2 ** 31), "too many"), (dict(total_q=2 ** 30), "too many"), (dict(scale=0.0), "scale"),
-         (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(cu_q=None), "cu_q"),
+         (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"), (dict(scale=3e38), "scale"), (dict(num_seqs=2 ** 30), "too many"), (dict(cu_q=None), "cu_q"),
          (dict(cu_k=None), "cu_k"), (dict(cu_k=P + 2), "misaligned"), (dict(q=None), "q is NULL"), (dict(k=None), "k is NULL"),
          (dict(v=None), "v is NULL"), (dict(q_ld=63), "stride of q"), (dict(k_ld=31), "stride of k"), (dict(v_ld=31), "stride of v"),
          (dict(q=P + 1), "misaligned")]

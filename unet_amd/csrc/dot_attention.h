@@ -580,8 +580,8 @@ __device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row
 
 // The forward.  WK wavefronts share the same 32 queries and take the 32-row pieces of a tile in turn: with WK = 1 a
 // workgroup has 128 queries (every tile serves four times 32), with WK > 1 it has fewer, for calls that have too few
-// queries to fill the GPU.  NW = 8: 256 queries a workgroup, for long rows and many queries (see Plan).  splits > 1: the workgroup takes a share of the key tiles and leaves its sums to
-// attention_join_kernel.
+// queries to fill the GPU.  NW = 8: 256 queries a workgroup, for long rows and many queries (see Plan).  splits > 1: the
+// workgroup takes a share of the key tiles and leaves its sums to attention_join_kernel.
 template <typename T, int DP, bool FAST, int WK, int NW = WAVES>
 __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_kernel(const Args<T> a) {
   constexpr int WQ = NW / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
@@ -1056,10 +1056,10 @@ inline int check_shape(const char *name, int num_seqs, i64 total_q, i64 total_k,
   UNET_REQUIRE(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "%s: %d query heads are no multiple of %d key/value heads", name, Hq, Hkv);
   UNET_REQUIRE(D >= 1, "%s: head_dim %d", name, D);
   if (D > 128) return unet_set_error(UNET_ERR_UNSUPPORTED, "%s: head_dim %d is larger than 128", name, D);
-  // rows and tiles are counted in 32 bits; a grid has fewer than 2^31 workgroups
-  const i64 most = ((i64)1 << 31) - 256, rows = total_q * (Hq / Hkv);
-  UNET_REQUIRE(total_q <= most && total_k <= most && rows <= most &&
-                   (rows / BM + num_seqs) * Hkv <= most && (total_k / BM + num_seqs) * Hkv <= most,
+  // rows are counted in 32 bits, and a launch has fewer than 2^32 threads (512 a workgroup at most, splits only for few)
+  const i64 most = ((i64)1 << 31) - 256, groups = (i64)1 << 22, rows = total_q * (Hq / Hkv);
+  UNET_REQUIRE(total_q <= most && total_k <= most && rows <= most && rows / BM + num_seqs <= groups / Hkv &&
+                   total_k / BM + num_seqs <= groups / Hkv,
                "%s: too many tokens (%lld queries, %lld keys, %d and %d heads)", name, (long long)total_q, (long long)total_k,
                Hq, Hkv);
   return UNET_OK;
@@ -1083,7 +1083,7 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
                 const int32_t *cu_q, const int32_t *cu_k, int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D,
                 float scale, int causal) {
   TRY(check_shape(name, num_seqs, total_q, total_k, Hq, Hkv, D));
-  UNET_REQUIRE(scale > 0.f && scale < INFINITY, "%s: scale %g is not positive and finite", name, (double)scale);
+  UNET_REQUIRE(scale > 0.f && scale * LOG2E < INFINITY, "%s: scale %g is not positive and finite", name, (double)scale);
   UNET_REQUIRE(num_seqs == 0 || (cu_q && cu_k), "%s: cu_q or cu_k is NULL", name);
   UNET_REQUIRE(aligned<int>(cu_q) && aligned<int>(cu_k), "%s: cu_q or cu_k is misaligned", name);
   TRY(check_matrix(name, "q", q, q_ld, total_q, (i64)Hq * D));

@@ -21,6 +21,7 @@ namespace {
 
 constexpr int FWD_BLOCKS = 2048;  // at most 8 workgroups of 4 wavefronts per CU: all resident
 constexpr int BWD_BLOCKS = 512;   // 2 per CU: fewer partial rows for the second launch to read
+constexpr int MOST_CHANNELS = 1 << 26;  // the column sums' launch has 32 threads a channel, of fewer than 2^32
 constexpr int LONG_SPLITS = 64;   // row ranges of the column sums of rows that do not fit registers
 
 template <typename T>
@@ -333,7 +334,7 @@ bool aligned(const void *p) { return ((uintptr_t)p & (sizeof(T) - 1)) == 0; }
 template <typename T>
 int layer_norm(const T *x, i64 x_ld, T *y, i64 y_ld, const float *w, float *stats, i64 rows, int C, float eps,
                hipStream_t st) {
-  UNET_REQUIRE(rows >= 0 && C >= 1, "layer_norm: rows %lld, channels %d", (long long)rows, C);
+  UNET_REQUIRE(rows >= 0 && C >= 1 && C <= MOST_CHANNELS, "layer_norm: rows %lld, channels %d", (long long)rows, C);
   UNET_REQUIRE(eps >= 0.f, "layer_norm: eps %g is negative or NaN", (double)eps);
   UNET_REQUIRE(x_ld >= C && y_ld >= C, "layer_norm: a row stride (%lld, %lld) is smaller than the %d channels",
                (long long)x_ld, (long long)y_ld, C);
@@ -355,7 +356,7 @@ template <typename T>
 int layer_norm_backward(const T *dy, i64 dy_ld, const T *x, i64 x_ld, const float *stats, const float *w, const T *skip,
                         i64 skip_ld, T *dx, i64 dx_ld, float *dw, i64 rows, int C, void *ws, size_t ws_bytes,
                         hipStream_t st) {
-  UNET_REQUIRE(rows >= 0 && C >= 1, "layer_norm_backward: rows %lld, channels %d", (long long)rows, C);
+  UNET_REQUIRE(rows >= 0 && C >= 1 && C <= MOST_CHANNELS, "layer_norm_backward: rows %lld, channels %d", (long long)rows, C);
   UNET_REQUIRE(dy_ld >= C && x_ld >= C && (!skip || skip_ld >= C) && (!dx || dx_ld >= C),
                "layer_norm_backward: a row stride is smaller than the %d channels", C);
   UNET_REQUIRE(rows == 0 || (dy && x && stats), "layer_norm_backward: NULL tensor");
@@ -399,7 +400,7 @@ extern "C" {
 
 int unet_layer_norm_backward_workspace_bytes(int64_t rows, int channels, size_t *bytes_host) {
   UNET_REQUIRE(bytes_host, "layer_norm_backward_workspace_bytes: NULL result");
-  UNET_REQUIRE(rows >= 0 && channels >= 1, "layer_norm_backward_workspace_bytes: rows %lld, channels %d", (long long)rows,
+  UNET_REQUIRE(rows >= 0 && channels >= 1 && channels <= MOST_CHANNELS, "layer_norm_backward_workspace_bytes: rows %lld, channels %d", (long long)rows,
                channels);
   *bytes_host = (size_t)(rows < BWD_BLOCKS ? rows : BWD_BLOCKS) * 2 * (size_t)channels * sizeof(float);
   return UNET_OK;
