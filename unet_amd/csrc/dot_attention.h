@@ -19,6 +19,17 @@
 // LDS holds a tile as rows of DP elements in 16-byte chunks, chunk c of row r at c ^ key(r): both the reads along a row
 // (A operands of the scores) and the transposing reads down the rows (A operands of the second product) then
 // spread over all banks.
+//
+// What bounds it, measured:
+//   - long sequences: the matrix cores.  8192 tokens, 16/4 heads of 128, causal, bf16: forward 275 us (1.0 PFLOP/s of the
+//     visible pairs), dQ 395, dK/dV 570-600, their join 23 (0.68 PFLOP/s on five products of two kernels that compute
+//     seven; a large library product reaches 1.26).
+//   - short ones: the latency of a few tiles.  16 x 256 tokens, 16 heads of 64, bf16: forward 13 us, dQ 20.5, dK/dV 21 for
+//     34 to 50 MB each.
+//   - few queries: HBM.  4 queries over 53386 keys, 32/4 heads of 128, bf16: 20 us (5.5 TB/s) and 4 for the join.
+//   - fp32: the matrix cores and an uneven last round of workgroups.  3525 tokens in 4 sequences, 8 heads of 64: forward
+//     81 us, dQ 114, dK/dV 177 (81, 87 and 75 TFLOP/s of the products that they compute; a large library product
+//     reaches 154).
 #include <math.h>
 
 #include "rows_util.h"
@@ -61,7 +72,8 @@ __device__ __forceinline__ f32x16 zero16() {
   for (int i = 0; i < 16; ++i) z[i] = 0.f;
   return z;
 }
-// Weights of 16 rows as a B operand; bf16 rounds them (relative 2^-9, half of what rounding the output costs).
+// Weights of 16 rows as a B operand; bf16 rounds them.  Each is off by at most 2^-8 of itself, so the sum by no more than
+// rounding the output once costs, and by less where many keys have a part in it.
 template <typename T>
 __device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
   Frag<T> f;
@@ -113,10 +125,10 @@ __device__ __forceinline__ int bound_of(const int *cu, int s, int total) { retur
 struct Seq {
   int q0, nq, k0, nk;  // first query / key and their numbers
 };
-// The sequence of tile `tile` and the tile's first row in it, where sequence s owns the tiles from floor(start(s) * g / TILE) + s
-// on (start in queries, or in keys where KEYS): at least ceil(len * g / TILE) of them, without a prefix sum over the
-// lengths.  Tiles in front of the first or behind the last row of their sequence are empty.  The lanes look at 64
-// sequences at once: up to 63 sequences cost the latency of one load.
+// The sequence of tile `tile` and the tile's first row in it, where sequence s owns the tiles from
+// floor(start(s) * g / TILE) + s on (start in queries, or in keys where KEYS): at least ceil(len * g / TILE) of them,
+// without a prefix sum over the lengths.  Tiles in front of the first or behind the last row of their sequence are
+// empty.  The lanes look at 64 sequences at once: up to 63 sequences cost the latency of one load.
 template <int TILE, bool KEYS, typename A>
 __device__ __forceinline__ Seq locate(const A &a, int g, int tile, int &row0) {
   const int lane = threadIdx.x & 63;
@@ -145,7 +157,8 @@ __device__ __forceinline__ Seq locate(const A &a, int g, int tile, int &row0) {
 }
 
 // ---- tiles in LDS ----------------------------------------------------------------------------------------
-// DP: elements that are computed with, a multiple of 32 (rows of 96 are stored like rows of 128); NW: wavefronts of the workgroup.
+// DP: elements that are computed with, a multiple of 32 (rows of 96 are stored like rows of 128); NW: wavefronts of the
+// workgroup.
 template <typename T, int DP, int ROWS, int NW = WAVES>
 struct Tile {
   static constexpr int RB = (DP == 96 ? 128 : DP) * (int)sizeof(T), NC = RB / 16, CH = 16 / (int)sizeof(T);
@@ -215,8 +228,8 @@ struct Tile {
       return f;
     }
   }
-  // ---- memory -> LDS, whole 16-byte chunks (FAST): direct loads, a wavefront moves 1 KB per instruction.  The swizzle is on
-  // the side of the memory address: lane l of a wavefront's instruction i fills chunk `slot` of the tile.
+  // ---- memory -> LDS, whole 16-byte chunks (FAST): direct loads, a wavefront moves 1 KB per instruction.  The swizzle is
+  // on the side of the memory address: lane l of a wavefront's instruction i fills chunk `slot` of the tile.
   static constexpr int MOVES = BYTES / 1024 / NW;
   static __device__ __forceinline__ int slot(int i) { return ((int)(threadIdx.x >> 6) * MOVES + i) * 64 + (int)(threadIdx.x & 63); }
   static __device__ __forceinline__ int slot_row(int i) { return slot(i) / NC; }
@@ -239,8 +252,8 @@ struct Tile {
     }
   }
 
-  // ---- memory -> registers -> LDS, any alignment and head dimension.  This thread's chunks of a tile on their way; row r of
-  // the tile is row first + r of a sequence of n rows.  Rows and elements that do not exist become zeros.
+  // ---- memory -> registers -> LDS, any alignment and head dimension.  This thread's chunks of a tile on their way; row r
+  // of the tile is row first + r of a sequence of n rows.  Rows and elements that do not exist become zeros.
   struct Chunks {
     u32x4 c[PER];
   };
@@ -432,18 +445,23 @@ __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int
   return true;
 }
 
-// Streamed rows per tile of the gradient kernels.  WK wavefronts that share queries take 32 rows each; else 64, or 32 where
-// long rows go through registers (a thread then holds 16 of them for the tile that is on its way; with 64 rows the kernels
-// with two streamed matrices and 64 or 128 accumulators spill), and in fp32, where the matrix cores take long enough per tile
-// (dQ and dK/dV of 3525 tokens, 8 heads of 64: 124 and 183 us with 32 rows, 138 and 208 with 64).
+// Streamed rows per tile of the gradient kernels.  WK wavefronts that share queries take 32 rows each; else 64, or 32 for
+// rows of 192 bytes and more
+//   - that go through registers: a thread then holds 16 of them for the tile that is on its way, and with 64 rows the
+//     kernels with two streamed matrices and 64 or 128 accumulators spill;
+//   - in fp32, where the matrix cores take long enough per tile (dQ and dK/dV of 3525 tokens, 8 heads of 64: 124 and 183
+//     us with 32 rows, 138 and 208 with 64, one workgroup a CU).
 template <typename T, int DP, bool FAST, int WK>
-constexpr int tile_rows() { return WK > 1 ? 32 * WK : DP * sizeof(T) >= (FAST && sizeof(T) == 2 ? 257 : 192) ? 32 : 64; }
+constexpr int tile_rows() {
+  return WK > 1 ? 32 * WK : DP * sizeof(T) >= 192 && !(FAST && sizeof(T) == 2) ? 32 : 64;
+}
 
-// Runs step(tile, buffer) for the tiles [0, n), the next tiles on their way to other buffers.  One barrier per tile: behind
-// it every wavefront has left the buffer that is written next, and sees the one that is read next.
-//   FAST: move(t, buffer) starts the direct loads of tile t, at least PER of them per wavefront, into one of NB buffers; tile t
-//         is waited for in front of its barrier, while the NB - 2 tiles behind it may be in flight.  The loop has no
-//         other vector memory instructions: a wait of the compiler's for one of those would be for all direct loads as well.
+// Runs step(tile, buffer) for the tiles [0, n), the next tiles on their way to other buffers.  One barrier per tile:
+// behind it every wavefront has left the buffer that is written next, and sees the one that is read next.
+//   FAST: move(t, buffer) starts the direct loads of tile t, at least PER of them per wavefront, into one of NB buffers;
+//         tile t is waited for in front of its barrier, while the NB - 2 tiles behind it may be in flight.  The loop has
+//         no other vector memory instructions: a wait of the compiler's for one of those would be for all direct loads
+//         as well.
 //   else: fetch(t) loads tile t to registers, put(buffer) writes them to one of two buffers.
 template <bool FAST, int NB, int PER, typename Move, typename Fetch, typename Put, typename Step>
 __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, Step step) {
@@ -477,19 +495,20 @@ __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, S
     }
   }
 }
-// Buffers: three where the LDS of two or three workgroups a CU has room for them (short sequences spend their time waiting for the first
-// tiles: 16 x 256 tokens, 16 heads of 64, TODO).
+// Buffers: three where the LDS of two or three workgroups a CU has room for them.  Short sequences spend their time
+// waiting for the first tiles: 16 x 256 tokens, 16 heads of 64, bf16, the backward's kernels together 40.7 us with three,
+// 41.7 with two, and the forward 13.0 with either.
 template <typename T, int DP, bool FAST, int WK>
 constexpr int buffers() { return FAST && sizeof(T) == 2 && DP <= 64 && WK < 4 ? 3 : 2; }
 
-// Whether the registers are to be limited so that two workgroups fit a CU.  The LDS of WK = 4 at rows of 256 bytes and more,
-// and the operands of fp32 at 96 elements and more, allow one.  (fp32, 3525 tokens, 8 heads of 64: forward 88 us with one,
-// 81 with two; the dK/dV kernel is slower with two, for lack of registers: 186 and 205.)
+// Whether the registers are to be limited so that two workgroups fit a CU.  The LDS of WK = 4 at rows of 256 bytes and
+// more, and the operands of fp32 at 96 elements and more, allow one.  (fp32, 3525 tokens, 8 heads of 64: forward 88 us
+// with one, 81 with two; the dK/dV kernel is slower with two, for lack of registers: 186 and 205.)
 template <typename T, int DP, int WK>
 constexpr bool two_fit() { return sizeof(T) == 2 ? WK < 4 || DP <= 64 : WK < 4 && DP <= 64; }
 
-// The sums of the wavefronts that share queries, each times its factor, for the blocks [db0, db1) of 32 elements: `all` holds
-// value i of block db of thread t at [(first + db * 16 + i) * 256 + t].
+// The sums of the wavefronts that share queries, each times its factor, for the blocks [db0, db1) of 32 elements: `all`
+// holds value i of block db of thread t at [(first + db * 16 + i) * 256 + t].
 template <int WK, int DB>
 __device__ __forceinline__ void leave_sums(float *mine, const f32x16 (&acc)[DB], int first) {
 #pragma unroll
@@ -514,8 +533,8 @@ __device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], const float *all, i
 // LDS[lds + 4 * lane] = the number at byte offset `at` from base, 0 at NOWHERE.
 __device__ __forceinline__ void direct_load_dword(const float *base, unsigned at, unsigned lds) {
   const uint64_t b = (uint64_t)base;
-  const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)b), __builtin_amdgcn_readfirstlane((int)(b >> 32)), (int)NOWHERE,
-                      0x00020000};
+  const i32x4 rsrc = {__builtin_amdgcn_readfirstlane((int)(unsigned)b), __builtin_amdgcn_readfirstlane((int)(b >> 32)),
+                      (int)NOWHERE, 0x00020000};
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at), "s"(rsrc));
@@ -844,9 +863,11 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
-      // dS of a query adds up to zero, so its product with K loses the part that the keys have in common, but the roundings
-      // of dS do not: with few elements (that part is then large beside the rest) they are kept out.
-      TL::template add<sizeof(T) == 2 && DP <= 64>(acc, k32, zeros, lo, s, edge, [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
+      // dS of a query adds up to zero, so its product with K loses the part that the keys have in common, but the
+      // roundings of dS do not: with few elements (that part is then large beside the rest) they are kept out.  (16 x 256
+      // tokens, 16 heads of 64: 21.2 us instead of 18.9, and an error of 1.0 instead of 1.45 output roundings.)
+      TL::template add<sizeof(T) == 2 && DP <= 64>(acc, k32, zeros, lo, s, edge,
+                                                   [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
   stream<FAST, NB, 2 * TL::MOVES>((span.kend + ROWS - 1) / ROWS, move, fetch, put, step);
@@ -877,10 +898,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
   typedef Tile<T, DP, ROWS, NW> TL;
   constexpr int STAGE = 2 * TL::BYTES + 2 * 64 * 4;  // Q, dout, lse (base 2), delta (64 values: a wavefront's direct load)
   constexpr int NB = buffers<T, DP, FAST, 1>();
-  // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands, and the last
-  // two of K, stay in LDS, each wavefront's own, in the order in which the lanes read them.  (With six more registers
-  // in use one operand was reloaded from scratch memory in every step, behind the direct loads in flight: 1004 us
-  // instead of 805-830, 8192 tokens, 16/4 heads, causal.)
+  // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands, and the
+  // last two of K, stay in LDS, each wavefront's own, in the order in which the lanes read them.  (With six more
+  // registers in use one operand is reloaded from scratch memory in every step, behind the direct loads in flight: 25 %
+  // slower.)
   constexpr int KT = DP / 16, K_REG = DP < 128 ? KT : KT - 2, V_REG = DP < 128 ? KT : 0;
   constexpr int OWN = (2 * KT - K_REG - V_REG) * 64 * (int)sizeof(Frag<T>);
   __shared__ __align__(16) unsigned char lds[NB * STAGE + TL::ZEROS + NW * OWN];
@@ -938,7 +959,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
     for (int i = 0; i < TL::MOVES; ++i) {
       const int r = r0 + TL::slot_row(i), query = div_by(r, a.G);
       const unsigned c = r < nrows ? TL::slot_chunk(i, a.D) : NOWHERE;
-      const unsigned in_row = c + (unsigned)((r - query * g) * a.D * (int)sizeof(T)), by = (unsigned)(query - query0) * (unsigned)sizeof(T);
+      const unsigned in_row = c + (unsigned)((r - query * g) * a.D * (int)sizeof(T));
+      const unsigned by = (unsigned)(query - query0) * (unsigned)sizeof(T);
       qo[i] = c == NOWHERE ? c : by * (unsigned)a.q_ld + in_row;
       dof[i] = c == NOWHERE ? c : by * (unsigned)a.dout_ld + in_row;
     }
@@ -948,7 +970,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
     if (wave < 2) {  // lse, delta; zeros where there is no row: with Q and dout zero as well, it adds nothing
       const int r = r0 + lane, query = div_by(r, a.G);
       const unsigned at = lane < ROWS && r < nrows ? (unsigned)((query - query0) * a.Hq + (r - query * g)) * 4u : NOWHERE;
-      direct_load_dword(a.rows + ((i64)wave * a.total_q + token) * a.Hq + kvh * g, at, lds0 + buf * STAGE + 2 * TL::BYTES + wave * 256u);
+      direct_load_dword(a.rows + ((i64)wave * a.total_q + token) * a.Hq + kvh * g, at,
+                        lds0 + buf * STAGE + 2 * TL::BYTES + wave * 256u);
     }
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
@@ -988,9 +1011,10 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
       const auto lo = DP < 128 ? lane_at : TL::forget(lane_at);  // at 128 elements every register counts
       f32x16 p = zero16(), ds = zero16();
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) p = mma(TL::along(q32, lo, x), x < K_REG ? kr[x < K_REG ? x : 0] : own[64 * (KT - V_REG + x - K_REG)], p);
+      for (int x = 0; x < DP / 16; ++x)
+        p = mma(TL::along(q32, lo, x), x < K_REG ? kr[x < K_REG ? x : 0] : own[64 * (KT - V_REG + x - K_REG)], p);
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) 
+      for (int x = 0; x < DP / 16; ++x)
         ds = mma(TL::along(d32, lo, x), x < V_REG ? vr[x < V_REG ? x : 0] : own[64 * (x - V_REG)], ds);
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
@@ -1096,16 +1120,17 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
   return UNET_OK;
 }
 
-// How the kernels that keep queries share their work.  wk (see attention_kernel): 128 queries a workgroup when that fills
-// three quarters of the places (two a CU, one in fp32 behind 64 elements), else 64, and 32 when it is a quarter or less: shorter workgroups fill
-// the GPU evenly, but their tiles serve fewer wavefronts.  Measured, forward in us with 128 / 64 / 32 queries: 512 workgroups of 128
-// (16 x 256 tokens, 16 heads of 64, bf16) 12.6 / 17.4 / 23.6; 332 (8 sequences of up to 2049, 8/2 heads of 80, causal)
-// 52.7 / 42.4 / 73; 224 (fp32, 3525 tokens, 8 heads of 64) 82 / 81 / 117; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
-// splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average (what a join costs
-// more would not be won back).
-// wide: 8 wavefronts and 256 queries a workgroup (forward, bf16 rows of 96 elements and more): half the direct loads, and room for
-// a third buffer; 8192 tokens, 16/4 heads of 128, causal: 293 -> 275 us.  (dQ gains nothing by it: its two score products
-// take twice as long per tile.)
+// How the kernels that keep queries share their work.
+// wk (see attention_kernel): 128 queries a workgroup when that fills three quarters of the places (two a CU, one in fp32
+// behind 64 elements), else 64, and 32 when it is a quarter or less: shorter workgroups fill the GPU evenly, but their
+// tiles serve fewer wavefronts.  Forward in us with 128 / 64 / 32 queries: 512 workgroups of 128 (16 x 256 tokens, 16
+// heads of 64, bf16) 12.6 / 17.4 / 23.6; 332 (8 sequences of up to 2049, 8/2 heads of 80, causal) 52.7 / 42.4 / 73; 224
+// (fp32, 3525 tokens, 8 heads of 64) 82 / 81 / 117; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
+// splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average (what a join
+// costs more would not be won back).
+// wide: 8 wavefronts and 256 queries a workgroup (forward, bf16 rows of 96 elements and more): half the direct loads, and
+// room for a third buffer; 8192 tokens, 16/4 heads of 128, causal: 293 -> 275 us.  (dQ gains nothing by it: its two
+// score products take twice as long per tile.)
 struct Plan {
   int wk, splits, tiles;  // tiles of queries: an upper bound
   bool wide;
@@ -1133,15 +1158,15 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
 }
 
 // Wavefronts of a dK/dV workgroup.  bf16 rows of 96 elements and more: 8 wavefronts, 256 keys, share a tile of queries,
-// because two workgroups of 4 would ask for 16 bytes of direct loads per clock and CU, which is all there is (8192 tokens,
-// 16/4 heads of 128, causal: 805 us with 4, 600 with 8).
+// because two workgroups of 4 would ask for 16 bytes of direct loads per clock and CU, which is all there is (8192
+// tokens, 16/4 heads of 128, causal: 805 us with 4, 600 with 8).
 template <typename T>
 constexpr int dkv_waves(int DP) { return sizeof(T) == 2 && DP >= 96 ? 8 : WAVES; }
-// Row ranges into which their sums are split when there are few key tiles: `fit` workgroups run at once (one of 8 wavefronts
-// a CU, one of fp32, else two), and where lengths differ as much as under a causal mask it takes twice as many to fill the GPU
-// evenly.  Each range costs a pass over fp32 dK and dV, so it should have 256 rows at least on the average.  A power of
-// two, so that workgroups of one range and head keep to one XCD and its L2 (workgroups go round over the 8 XCDs): with 5 or
-// 7 ranges the case above is 6 % slower than with 4; with one range it takes 1.9 ms.
+// Row ranges into which their sums are split when there are few key tiles: `fit` workgroups run at once (one of 8
+// wavefronts a CU, one of fp32, else two), and where lengths differ as much as under a causal mask it takes twice as many
+// to fill the GPU evenly.  Each range costs a pass over fp32 dK and dV, so it should have 256 rows at least on the
+// average.  A power of two, so that workgroups of one range and head keep to one XCD and its L2 (workgroups go round over
+// the 8 XCDs): with 5 or 7 ranges the case above is 6 % slower than with 4; with one range it takes 1.9 ms.
 template <typename T>
 int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, bool causal) {
   const int nw = dkv_waves<T>(padded_dim(D)), fit = sizeof(T) == 2 && nw == 4 ? 512 : 256;

@@ -7,7 +7,8 @@
 // Bound by HBM as long as the generator stays cheap: one Philox block (20 multiplications of 32 x 32 bits) makes the
 // upper 16 bits of eight elements' numbers.  Those decide unless they equal the threshold's upper 16 bits, which
 // happens to one element in 65536; only then the block of the lower 16 bits is computed.  So p has the resolution of
-// 2^-32 at half the multiplications.
+// 2^-32 at half the multiplications.  65536 rows of 1024 bf16 channels with a residual: 73 us, 5.5 TB/s (the 400 MB are
+// partly in the last-level cache; a large copy reaches 4.9).
 #include "rows_util.h"
 
 namespace {
