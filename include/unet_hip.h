@@ -212,12 +212,11 @@ int unet_layer_norm_bf16(const uint16_t *inputs, int64_t in_ld, uint16_t *activa
  *   grad_weights[2c] = sum_rows grad_activations * xhat, grad_weights[2c+1] = sum_rows grad_activations
  * grad_skip (may be NULL; skip_ld is then ignored) is the gradient that reaches the inputs around the layer norm
  * (the residual connection), added before the one rounding.  grad_inputs may be the buffer of grad_activations, of
- * grad_skip or of inputs (same pointer, same stride).  grad_weights (fp32, overwritten) or grad_inputs may be NULL to skip
- * that half.  weights NULL = gamma 1.  Sums over rows have a fixed order: equal calls give equal bits.
+ * grad_skip or of inputs (same pointer, same stride).  grad_weights (fp32, overwritten) or grad_inputs may be NULL to
+ * skip that half.  weights NULL = gamma 1.  Sums over rows have a fixed order: equal calls give equal bits.
  * `workspace` is device memory of at least unet_layer_norm_backward_workspace_bytes() bytes, 16-byte aligned, free
  * for other use once the call's work on `stream` has finished (calls that may run at the same time need one each); it
- * may be NULL when grad_weights is.  The calls
- * allocate nothing and can be captured into a graph. */
+ * may be NULL when grad_weights is.  The calls allocate nothing and can be captured into a graph. */
 int unet_layer_norm_backward_workspace_bytes(int64_t rows, int channels, size_t *bytes_host);
 int unet_layer_norm_backward_f32(const float *grad_activations, int64_t grad_ld, const float *inputs, int64_t in_ld,
                                  const float *row_stats, const float *weights, const float *grad_skip, int64_t skip_ld,
@@ -260,9 +259,9 @@ int unet_tanh_backward_f32(const float *grad_activations, const float *activatio
  *     16-bit number of element e is (word[j / 2] >> 16 * (j % 2)) % 2^16, j = e % 8;
  *   - u(e) = 2^16 * (number for f = 0) + (number for f = 1); kept iff u(e) >= round(p * 2^32).
  * 0 <= p <= 1; at p = 1 nothing is kept.  A dropped element contributes exactly 0, also where the input is not finite.
- * Calls that shall draw independent masks use different offsets (or seeds).  offset_device (may be NULL) is a 64-bit number in
- * device memory, read when the kernel runs and added to `offset`: a captured graph draws a new mask per replay when
- * something between replays changes it.  Row strides (`*_ld`) in elements, at least `channels`; any alignment of
+ * Calls that shall draw independent masks use different offsets (or seeds).  offset_device (may be NULL) is a 64-bit
+ * number in device memory, read when the kernel runs and added to `offset`: a captured graph draws a new mask per
+ * replay when something between replays changes it.  Row strides (`*_ld`) in elements, at least `channels`; any alignment of
  * the element type.  residual may be NULL (residual_ld is then ignored).  activations may be the buffer of inputs or
  * of residual (same pointer, same stride).  The sum is taken in fp32 and rounded once. */
 int unet_dropout_f32(const float *inputs, int64_t in_ld, const float *residual, int64_t residual_ld, float *activations,
@@ -363,14 +362,13 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  *   causal != 0: query i of a sequence sees the keys j <= i + (keys - queries), i.e. the last query sees all.
  *   lse [total_q][heads_q] (fp32, may be NULL: inference) = log sum_j exp(scale * q.k_j), for the backward.
  * A query that sees no key gets out = 0 and lse = -inf, and adds nothing to any gradient.  What a query does not see
- * does not reach it, whatever it holds (NaN and infinities included).  Rows of out and lse in front of the first or behind
- * the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
+ * does not reach it, whatever it holds (NaN and infinities included).  Rows of out and lse in front of the first or
+ * behind the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
  * accumulators are fp32; the bf16 form rounds the softmax weights to bf16 for their product with V.  Equal calls
  * give equal bits.  out must not overlap q, k or v.  total_q * heads_q and total_k * heads_kv may be up to about 2^29.
  * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
- * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the same
- * time need one each.  The calls allocate
- * nothing and can be captured into a graph. */
+ * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the
+ * same time need one each.  The calls allocate nothing and can be captured into a graph. */
 int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv,
                                        int head_dim, size_t *bytes_host);
 int unet_dot_attention_f32(const float *q, int64_t q_ld, const float *k, int64_t k_ld, const float *v, int64_t v_ld,
@@ -384,11 +382,11 @@ int unet_dot_attention_bf16(const uint16_t *q, int64_t q_ld, const uint16_t *k, 
                             size_t workspace_bytes, unet_stream_t stream);
 /* Gradients of the above from grad_out and the forward's out and lse: with P the softmax weights,
  * dP = grad_out V^T and dS = P * (dP - sum_d grad_out * out):
- *   grad_v = P^T grad_out, grad_q = scale * dS K, grad_k = scale * dS^T Q, all overwritten; grad_k and grad_v sum over the query heads that
- * share a key/value head.  The bf16 form rounds P and dS to bf16 for their products (dS for grad_q in two parts up to head_dim
- * 64).  No atomics: every sum has a
- * fixed order.  Rows outside the sequences are left as they were; keys that no query sees get 0.  The gradients must not
- * overlap the inputs or each other's columns (they may be column slices of one buffer). */
+ *   grad_v = P^T grad_out, grad_q = scale * dS K, grad_k = scale * dS^T Q, all overwritten; grad_k and grad_v sum over
+ * the query heads that share a key/value head.  The bf16 form rounds P and dS to bf16 for their products (dS for grad_q
+ * in two parts up to head_dim 64).  No atomics: every sum has a fixed order.  Rows outside the sequences are left as
+ * they were; keys that no query sees get 0.  The gradients must not overlap the inputs or each other's columns (they
+ * may be column slices of one buffer). */
 int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
                                                 int heads_kv, int head_dim, size_t *bytes_host);
 int unet_dot_attention_backward_f32(const float *grad_out, int64_t grad_out_ld, const float *q, int64_t q_ld,
