@@ -362,9 +362,11 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  *   causal != 0: query i of a sequence sees the keys j <= i + (keys - queries), i.e. the last query sees all.
  *   lse [total_q][heads_q] (fp32, may be NULL: inference) = log sum_j exp(scale * q.k_j), for the backward.
  * A query that sees no key gets out = 0 and lse = -inf, and adds nothing to any gradient.  What a query does not see
- * does not reach it, whatever it holds (NaN and infinities included).  Rows of out and lse in front of the first or
+ * does not reach it, whatever it holds (NaN and infinities included).  (An infinity that it does see counts as NaN in
+ * the fp32 form, whose products take operands apart.)  Rows of out and lse in front of the first or
  * behind the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
- * accumulators are fp32; the bf16 form rounds the softmax weights to bf16 for their product with V.  Equal calls
+ * accumulators are fp32 (weights are up to 2^8 before the division at the end, so values larger than the largest number
+ * over 256 * keys may overflow); the bf16 form rounds the softmax weights to bf16 for their product with V.  Equal calls
  * give equal bits.  out must not overlap q, k or v.  total_q * heads_q and total_k * heads_kv may be up to about 2^29.
  * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
  * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the

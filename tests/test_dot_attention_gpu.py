@@ -163,6 +163,52 @@ def test_many_queries(causal, dim):
     c.verify()
 
 
+# one call for each way to share the queries of a head dimension's kernels: 32, 64 and 128 of them in a workgroup
+SHARES = [(4, 20), (4, 60), (4, 96), (4, 128), (60, 30), (60, 64), (30, 80), (30, 128), (130, 32), (130, 50), (66, 88), (66, 120)]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("pad", [0, 3])
+@pytest.mark.parametrize("heads,dim", SHARES)
+def test_shares_of_the_queries(name, causal, pad, heads, dim):
+    c = Call(name, [333, 40], [340, 33], heads, heads // 2, dim, causal, pad=pad, behind=1)
+    c.forward()
+    c.backward()
+    c.verify()
+
+
+@pytest.mark.parametrize("power", [-100, -60, 60, 100, 113])
+def test_fp32_over_its_range(power):
+    """Values near both ends of fp32's range and gradients near the other: the results are linear in both, so their bounds
+    scale with them.  The products leave out at most 2 * 2^-7 * 2^-15 of each term, 8 U, which is less than the chains of
+    the bounds have.  113: every value is as large as the header allows, largest / (256 * 90 keys), rounded down to
+    largest / 2^15: the weights on the way are up to 2^8, and 2^8 * 90 < 2^15."""
+    c = Call("f32", [70, 9], [90, 9], 4, 2, 64, True)
+    if power == 113:
+        top = torch.finfo(torch.float32).max * 2.0 ** -15
+        c.v[:] = top * torch.where(torch.arange(c.v.shape[1], device=DEV) % 2 == 0, 1.0, -1.0)
+    else:
+        c.v *= 2.0 ** power
+    c.dout *= 2.0 ** -power
+    c.forward()
+    c.backward()
+    c.verify()
+
+
+def test_fp32_largest_numbers():
+    """The largest finite fp32 number as an element of every key, times the smallest normal one in the queries: a part of
+    the score of about 4 that needs all bits of the key.  (dK has 2^-126 of dS in that column: not looked at.)"""
+    c = Call("f32", [40], [75], 2, 1, 32, True)
+    c.k[:, 0] = torch.finfo(torch.float32).max
+    c.q[:, 0] = 2.0 ** -126
+    c.q[:, 32] = -2.0 ** -126
+    c.dout *= 2.0 ** -30
+    c.forward()
+    c.backward()
+    c.verify(("out", "lse", "dq", "dv"))
+
+
 @pytest.mark.parametrize("bad", [float("nan"), float("-inf")])
 def test_split_sums_keep_bad_keys_to_the_queries_that_see_them(bad):
     c = Call("bf16", [2, 1], [4000, 3500], 4, 2, 64, True)

@@ -1,4 +1,5 @@
-// Dot-product attention over packed sequences, forward and backward (fp32 and bf16 storage).
+// Dot-product attention over packed sequences, forward and backward (fp32 and bf16 storage; fp32 operands are taken as
+// three bf16 numbers, see Parts).
 //
 //   S = scale Q K^T,  P = softmax over the visible keys,  out = P V,  lse = log sum exp S
 //   delta = sum_d dout * out,  dP = dout V^T,  dS = P * (dP - delta)
@@ -27,9 +28,9 @@
 //   - short ones: the latency of a few tiles.  16 x 256 tokens, 16 heads of 64, bf16: forward 13 us, dQ 20.5, dK/dV 21 for
 //     34 to 50 MB each.
 //   - few queries: HBM.  4 queries over 53386 keys, 32/4 heads of 128, bf16: 20 us (5.5 TB/s) and 4 for the join.
-//   - fp32: the matrix cores and an uneven last round of workgroups.  3525 tokens in 4 sequences, 8 heads of 64: forward
-//     81 us, dQ 114, dK/dV 177 (81, 87 and 75 TFLOP/s of the products that they compute; a large library product
-//     reaches 154).
+//   - fp32: the matrix cores and, beside them, the vector instructions that split operands into parts.  3525 tokens in 4
+//     sequences, 8 heads of 64: forward 46 us, dQ 77, dK/dV 90, their join 10 (144, 129 and 147 TFLOP/s of the products that
+//     they compute; a large library product in fp32 reaches 154); one of 8192 tokens 702 us (196 TFLOP/s).
 #include <math.h>
 
 #include "rows_util.h"
@@ -48,23 +49,70 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 constexpr float LAZY = 8.f;
 constexpr unsigned NOWHERE = 0x80000000u;  // a byte offset behind the end of every buffer (a tile spans less than 2 GiB)
 
+// Eight elements of a matrix operand.  An fp32 number is the sum of three bf16 numbers: its upper 16 bits, what they leave
+// over (less than 2^-7 of it) rounded to bf16, and the rest, which has 8 bits and is at most 2^-15 of it.  Six products
+// of parts make the product of two such numbers up to 2^-21 of it: what is left out is the middle part of one times the
+// last part of the other, twice, with random signs; the matrix cores do the six in 3/8 of the time of one fp32 product.
+// (The upper part is cut off, not rounded: no finite number becomes infinite.  An infinity leaves NaN over.)  3525
+// tokens in 4 sequences, 8 heads of 64, forward and backward: 219 us and an error of 5.3e-7 of the result; with fp32
+// matrix instructions 366 us and 7.0e-7.
+struct Parts {
+  bf16x8 p[3];
+};
 template <typename T>
 struct FragOf;
 template <>
-struct FragOf<bf16_t> { typedef bf16x8 type; };
+struct FragOf<bf16_t> { typedef bf16x8 type, raw; };
 template <>
-struct FragOf<float> { typedef f32x8 type; };
+struct FragOf<float> { typedef Parts type; typedef f32x8 raw; };
 template <typename T>
 using Frag = typename FragOf<T>::type;
+template <typename T>
+using Raw = typename FragOf<T>::raw;  // the elements as they are stored
+template <typename T>
+constexpr int PARTS = sizeof(T) == 2 ? 1 : 3;
+
+__device__ __forceinline__ bf16x8 as_frag(const bf16x8 &x) { return x; }
+__device__ __forceinline__ Parts as_frag(const f32x8 &x) {
+  uint32_t w[3][4];
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const uint32_t u0 = __float_as_uint(x[j]), u1 = __float_as_uint(x[j + 1]);
+    w[0][j / 2] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // both upper halves
+    const f32x2 r = {x[j] - __uint_as_float(u0 & 0xffff0000u), x[j + 1] - __uint_as_float(u1 & 0xffff0000u)};
+    w[1][j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(r, bf16x2));
+    const f32x2 l = {r[0] - __uint_as_float(w[1][j / 2] << 16), r[1] - __uint_as_float(w[1][j / 2] & 0xffff0000u)};
+    w[2][j / 2] = __builtin_bit_cast(uint32_t, __builtin_convertvector(l, bf16x2));
+  }
+  Parts f;
+  __builtin_memcpy(f.p, w, sizeof(w));
+  return f;
+}
+__device__ __forceinline__ bf16x8 choose(bool c, const bf16x8 &a, const bf16x8 &b) { return c ? a : b; }
+__device__ __forceinline__ Parts choose(bool c, const Parts &a, const Parts &b) {
+  return Parts{{c ? a.p[0] : b.p[0], c ? a.p[1] : b.p[1], c ? a.p[2] : b.p[2]}};
+}
+// element j alone, zeros beside it; all zeros unless `c`
+__device__ __forceinline__ bf16x8 alone(bool c, int j, bf16x8 a) {
+#pragma unroll
+  for (int x = 0; x < 8; ++x) a[x] = c && x == j ? a[x] : (bf16x8{})[0];
+  return a;
+}
+__device__ __forceinline__ Parts alone(bool c, int j, const Parts &a) {
+  return Parts{{alone(c, j, a.p[0]), alone(c, j, a.p[1]), alone(c, j, a.p[2])}};
+}
 
 // c += A B over 16 k: lane l holds A[l % 32][8 * (l / 32) + j] and B[8 * (l / 32) + j][l % 32], j < 8.
 __device__ __forceinline__ f32x16 mma(bf16x8 a, bf16x8 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x16 mma(f32x8 a, f32x8 b, f32x16 c) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
-  return c;
+__device__ __forceinline__ f32x16 mma(const Parts &a, const Parts &b, f32x16 c) {
+  c = mma(a.p[2], b.p[0], c);
+  c = mma(a.p[0], b.p[2], c);
+  c = mma(a.p[1], b.p[1], c);
+  c = mma(a.p[1], b.p[0], c);
+  c = mma(a.p[0], b.p[1], c);
+  return mma(a.p[0], b.p[0], c);
 }
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
@@ -76,7 +124,7 @@ __device__ __forceinline__ f32x16 zero16() {
 // rounding the output once costs, and by less where many keys have a part in it.
 template <typename T>
 __device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
-  Frag<T> f;
+  Raw<T> f;
 #pragma unroll
   for (int j = 0; j < 8; j += 2) {
     if constexpr (sizeof(T) == 2) {  // as pairs: one conversion instruction for two
@@ -86,7 +134,7 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
       f[j] = w[8 * t + j], f[j + 1] = w[8 * t + j + 1];
     }
   }
-  return f;
+  return as_frag(f);
 }
 
 // ---- division by the group size (rows -> queries), by a multiplication -------------------------------
@@ -158,11 +206,12 @@ __device__ __forceinline__ Seq locate(const A &a, int g, int tile, int &row0) {
 
 // ---- tiles in LDS ----------------------------------------------------------------------------------------
 // DP: elements that are computed with, a multiple of 32 (rows of 96 are stored like rows of 128); NW: wavefronts of the
-// workgroup.
+// workgroup.  fp32: 16 rows of the first parts, then the same rows of the second and of the third.
 template <typename T, int DP, int ROWS, int NW = WAVES>
 struct Tile {
-  static constexpr int RB = (DP == 96 ? 128 : DP) * (int)sizeof(T), NC = RB / 16, CH = 16 / (int)sizeof(T);
-  static constexpr int BYTES = ROWS * RB, NT = 64 * NW, PER = ROWS * NC / NT;
+  static constexpr int RB = (DP == 96 ? 128 : DP) * 2, NC = RB / 16, CH = 8;  // of one part; 8 elements are a chunk
+  static constexpr int PART = 16 * RB, R16 = PARTS<T> * PART;
+  static constexpr int BYTES = ROWS / 16 * R16, NT = 64 * NW, PER = ROWS * NC / NT;
   static_assert(ROWS % 32 == 0 && ROWS * NC % NT == 0, "whole sub-tiles, whole chunks per thread");
   // 16 rows at one chunk (the reads along rows, 16 lanes at a time) and 4 rows of 64 bytes (the transposing reads, 32
   // lanes at a time) both cover the 256 bytes of a bank line.
@@ -175,26 +224,17 @@ struct Tile {
   // element 32 db + l % 32 of the rows 4 (l / 32) + j and 8 + 4 (l / 32) + j, j < 4).  t and db change bits of the chunk
   // number alone, so they are exclusive-ored into the offset.
   struct Lane {
-    int row, down[sizeof(T) == 2 ? 2 : 8];
+    int row, down[2];
   };
   static __device__ __forceinline__ Lane lane_offsets(int lane) {
     Lane o;
     const int h = lane >> 5, l = lane & 31;
-    if constexpr (sizeof(T) == 2) {
-      o.row = l * RB + (h ^ key(l)) * 16;
-      const int q = (lane & 15) >> 2, p = lane & 3;  // a 16-lane group transposes 4 rows x 16 elements
+    o.row = (l >> 4) * R16 + (l & 15) * RB + (h ^ key(l)) * 16;
+    const int q = (lane & 15) >> 2, p = lane & 3;  // a 16-lane group transposes 4 rows x 16 elements
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = 8 * i + 4 * h + q;
-        o.down[i] = r * RB + ((2 * ((lane >> 4) & 1) + (p >> 1)) ^ key(r)) * 16 + (p & 1) * 8;
-      }
-    } else {
-      o.row = l * RB + ((2 * h) ^ key(l)) * 16;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 8 * (i >> 2) + 4 * h + (i & 3);
-        o.down[i] = r * RB + ((l >> 2) ^ key(r)) * 16 + (l & 3) * 4;
-      }
+    for (int i = 0; i < 2; ++i) {
+      const int r = 8 * i + 4 * h + q;
+      o.down[i] = r * RB + ((2 * ((lane >> 4) & 1) + (p >> 1)) ^ key(r)) * 16 + (p & 1) * 8;
     }
     return o;
   }
@@ -207,26 +247,18 @@ struct Tile {
     return o;
   }
   static __device__ __forceinline__ Frag<T> along(const unsigned char *rows32, const Lane &o, int t) {
-    Frag<T> f;
+    const unsigned char *const at = rows32 + (o.row ^ (t * 32));
     if constexpr (sizeof(T) == 2) {
-      f = *reinterpret_cast<const bf16x8 *>(rows32 + (o.row ^ (t * 32)));
+      return *reinterpret_cast<const bf16x8 *>(at);
     } else {
-      const f32x4 a = *reinterpret_cast<const f32x4 *>(rows32 + (o.row ^ (t * 64)));
-      const f32x4 b = *reinterpret_cast<const f32x4 *>(rows32 + (o.row ^ (t * 64 + 16)));
-#pragma unroll
-      for (int j = 0; j < 4; ++j) f[j] = a[j], f[4 + j] = b[j];
+      return Parts{{*reinterpret_cast<const bf16x8 *>(at), *reinterpret_cast<const bf16x8 *>(at + PART),
+                    *reinterpret_cast<const bf16x8 *>(at + 2 * PART)}};
     }
-    return f;
   }
   static __device__ __forceinline__ Frag<T> down(const unsigned char *rows16, const Lane &o, int db) {
-    if constexpr (sizeof(T) == 2) {
-      return tr_read_pair(rows16 + (o.down[0] ^ (db * 64)), rows16 + (o.down[1] ^ (db * 64)));
-    } else {
-      Frag<T> f;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = *reinterpret_cast<const float *>(rows16 + (o.down[j] ^ (db * 128)));
-      return f;
-    }
+    const unsigned char *const a = rows16 + (o.down[0] ^ (db * 64)), *const b = rows16 + (o.down[1] ^ (db * 64));
+    if constexpr (sizeof(T) == 2) return tr_read_pair(a, b);
+    else return Parts{{tr_read_pair(a, b), tr_read_pair(a + PART, b + PART), tr_read_pair(a + 2 * PART, b + 2 * PART)}};
   }
   // ---- memory -> LDS, whole 16-byte chunks (FAST): direct loads, a wavefront moves 1 KB per instruction.  The swizzle is
   // on the side of the memory address: lane l of a wavefront's instruction i fills chunk `slot` of the tile.
@@ -255,63 +287,63 @@ struct Tile {
   // ---- memory -> registers -> LDS, any alignment and head dimension.  This thread's chunks of a tile on their way; row r
   // of the tile is row first + r of a sequence of n rows.  Rows and elements that do not exist become zeros.
   struct Chunks {
-    u32x4 c[PER];
+    Raw<T> c[PER];
   };
   template <typename Row>
   static __device__ __forceinline__ void fetch(Chunks &to, int first, int n, int D, Row row_ptr) {
     const int e = (threadIdx.x % NC) * CH, r0 = first + threadIdx.x / NC;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) to.c[i] = u32x4{0, 0, 0, 0};
+    for (int i = 0; i < PER; ++i) to.c[i] = Raw<T>{};
     if (first >= n) return;
     if (e < D) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const T *p = row_ptr(min(r0 + i * (NT / NC), n - 1)) + e;
         if (e + CH <= D) {
-          __builtin_memcpy(&to.c[i], p, 16);
+          __builtin_memcpy(&to.c[i], p, sizeof(Raw<T>));
         } else {
           T tmp[CH];
 #pragma unroll
           for (int x = 0; x < CH; ++x) tmp[x] = e + x < D ? p[x] : (T)0;
-          __builtin_memcpy(&to.c[i], tmp, 16);
+          __builtin_memcpy(&to.c[i], tmp, sizeof(tmp));
         }
       }
     }
     if (first + ROWS > n)
 #pragma unroll
       for (int i = 0; i < PER; ++i)
-        if (r0 + i * (NT / NC) >= n) to.c[i] = u32x4{0, 0, 0, 0};
+        if (r0 + i * (NT / NC) >= n) to.c[i] = Raw<T>{};
   }
   static __device__ __forceinline__ void put(const Chunks &from, unsigned char *tile) {
     const int chunk = threadIdx.x % NC;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = threadIdx.x / NC + i * (NT / NC);
-      *reinterpret_cast<u32x4 *>(tile + r * RB + ((chunk ^ key(r)) * 16)) = from.c[i];
+      unsigned char *const at = tile + (r >> 4) * R16 + (r & 15) * RB + (chunk ^ key(r)) * 16;
+      const Frag<T> f = as_frag(from.c[i]);
+#pragma unroll
+      for (int k = 0; k < PARTS<T>; ++k) *reinterpret_cast<bf16x8 *>(at + k * PART) = reinterpret_cast<const bf16x8 *>(&f)[k];
     }
   }
   // Whether any of 32 rows of the tile holds an infinity or NaN.
   static __device__ __forceinline__ bool not_finite(const unsigned char *rows32, const Lane &o) {
-    typedef typename std::conditional<sizeof(T) == 2, u16x2, uint32_t>::type Word;  // magnitudes: 16 bits twice, or 32
-    Word top = {};
+    u16x2 top = {};  // of the magnitudes (fp32: of their upper halves)
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) {
-      const Frag<T> f = along(rows32, o, t);
-      uint32_t w[sizeof(f) / 4];
+      const bf16x8 f = *reinterpret_cast<const bf16x8 *>(rows32 + (o.row ^ (t * 32)));
+      uint32_t w[4];
       __builtin_memcpy(w, &f, sizeof(f));
 #pragma unroll
-      for (int i = 0; i < (int)(sizeof(f) / 4); ++i)
-        top = __builtin_elementwise_max(top, __builtin_bit_cast(Word, w[i] & (sizeof(T) == 2 ? 0x7fff7fffu : 0x7fffffffu)));
+      for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu));
     }
-    if constexpr (sizeof(T) == 2) return __any(top[0] >= 0x7f80u || top[1] >= 0x7f80u);
-    else return __any(top >= 0x7f800000u);
+    return __any(top[0] >= 0x7f80u || top[1] >= 0x7f80u);
   }
   // acc[d][column] += sum over 32 rows of X[row][d] W[row][column].  edge: some rows are hidden from some columns, with
   // weight 0.  If such rows hold infinities or NaN, 0 * inf must not reach a column that does not see them: then the
   // rows are added one at a time, the result taken by the columns that see the row, and the common product reads
   // zeros instead.  Rare, so slow is fine; what matters is that the accumulators stay where they are.
   // TWICE: a bf16 weight is taken as the sum of two bf16 numbers, its rounding and what that left over.
-  static constexpr int ZEROS = 16 * RB;
+  static constexpr int ZEROS = R16;
   template <bool TWICE = false, typename Sees>
   static __device__ __forceinline__ void add(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const unsigned char *zeros,
                                              const Lane &o, const f32x16 &w, bool edge, Sees sees) {
@@ -323,24 +355,19 @@ struct Tile {
       for (int i = 0; i < 16; ++i) rest[i] = w[i] - (float)(i < 8 ? b0[i & 7] : b1[i & 7]);
       c0 = pack8<T>(rest, 0), c1 = pack8<T>(rest, 1);
     }
-    const unsigned char *low = rows32, *high = rows32 + 16 * RB;
+    const unsigned char *low = rows32, *high = rows32 + R16;
     if (edge && not_finite(rows32, o)) {
       const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll 1
       for (int k = 0; k < 32; ++k) {
         const int j = ((k >> 3) & 1) * 4 + (k & 3);
         const bool mine = ((k >> 2) & 1) == h, seen = sees(k);
-        Frag<T> b, c;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          b[x] = k < 16 ? b0[x] : b1[x];
-          if constexpr (TWICE) c[x] = k < 16 ? c0[x] : c1[x];
-        }
+        const Frag<T> b = choose(k < 16, b0, b1);
+        Frag<T> c;
+        if constexpr (TWICE) c = choose(k < 16, c0, c1);
 #pragma unroll
         for (int db = 0; db < DP / 32; ++db) {
-          Frag<T> f = down(rows32 + (k & 16) * RB, o, db);
-#pragma unroll
-          for (int x = 0; x < 8; ++x) f[x] = mine && x == j ? f[x] : 0;
+          const Frag<T> f = alone(mine, j, down(rows32 + (k >> 4) * R16, o, db));
           f32x16 r = mma(f, b, zero16());
           if constexpr (TWICE) r = mma(f, c, r);
 #pragma unroll
@@ -368,20 +395,14 @@ struct Tile {
 };
 
 // Eight consecutive elements p[e..e+8) of a row of D, zero from element D on, as (half of) a B operand.  WHOLE: D is a
-// multiple of the elements in 16 bytes; then without branches, from the row's first elements where there are none.
+// multiple of 8; then without branches, from the row's first elements where there are none.
 template <typename T, bool WHOLE>
-__device__ __forceinline__ Frag<T> load_frag(const T *p, int e, int D) {
-  Frag<T> f;
+__device__ __forceinline__ Raw<T> load_eight(const T *p, int e, int D) {
+  Raw<T> f;
   const int n = D - e;
   if constexpr (WHOLE) {
-    constexpr int N = 16 / (int)sizeof(T);
-#pragma unroll
-    for (int i = 0; i < 8; i += N) {
-      u32x4 v;
-      __builtin_memcpy(&v, p + (i < n ? e + i : 0), 16);
-      if (i >= n) v = u32x4{0, 0, 0, 0};
-      __builtin_memcpy((char *)&f + i * sizeof(T), &v, 16);
-    }
+    __builtin_memcpy(&f, p + (n > 0 ? e : 0), sizeof(f));
+    if (n <= 0) f = Raw<T>{};
   } else if (n >= 8) {
     __builtin_memcpy(&f, p + e, sizeof(f));
   } else {
@@ -391,6 +412,10 @@ __device__ __forceinline__ Frag<T> load_frag(const T *p, int e, int D) {
     __builtin_memcpy(&f, x, sizeof(f));
   }
   return f;
+}
+template <typename T, bool WHOLE>
+__device__ __forceinline__ Frag<T> load_frag(const T *p, int e, int D) {
+  return as_frag(load_eight<T, WHOLE>(p, e, D));
 }
 // Four consecutive results p[0..4), as many as n allows.
 template <typename T>
@@ -449,23 +474,23 @@ __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int
 // rows of 192 bytes and more
 //   - that go through registers: a thread then holds 16 of them for the tile that is on its way, and with 64 rows the
 //     kernels with two streamed matrices and 64 or 128 accumulators spill;
-//   - in fp32, where the matrix cores take long enough per tile (dQ and dK/dV of 3525 tokens, 8 heads of 64: 124 and 183
-//     us with 32 rows, 138 and 208 with 64, one workgroup a CU).
+//   - in fp32, whose tiles are three times as large.
 template <typename T, int DP, bool FAST, int WK>
 constexpr int tile_rows() {
-  return WK > 1 ? 32 * WK : DP * sizeof(T) >= 192 && !(FAST && sizeof(T) == 2) ? 32 : 64;
+  return WK > 1 ? 32 * WK : DP * sizeof(T) >= 192 && !FAST ? 32 : 64;
 }
 
-// Runs step(tile, buffer) for the tiles [0, n), the next tiles on their way to other buffers.  One barrier per tile:
-// behind it every wavefront has left the buffer that is written next, and sees the one that is read next.
+// Runs step(tile, buffer) for the tiles [0, n), the next tiles on their way to other buffers (or, where there is one
+// buffer, in registers).  One barrier per tile: behind it every wavefront has left the buffer that is written next, and
+// sees the one that is read next.  One buffer: two barriers, in front of its filling and behind it.
 //   FAST: move(t, buffer) starts the direct loads of tile t, at least PER of them per wavefront, into one of NB buffers;
 //         tile t is waited for in front of its barrier, while the NB - 2 tiles behind it may be in flight.  The loop has
 //         no other vector memory instructions: a wait of the compiler's for one of those would be for all direct loads
 //         as well.
-//   else: fetch(t) loads tile t to registers, put(buffer) writes them to one of two buffers.
+//   else: fetch(t) loads tile t to registers, put(buffer) writes them to a buffer.
 template <bool FAST, int NB, int PER, typename Move, typename Fetch, typename Put, typename Step>
 __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, Step step) {
-  static_assert(NB == 2 || (FAST && NB == 3), "two buffers, three for direct loads");
+  static_assert(NB == 2 || NB == (FAST ? 3 : 1), "two buffers, or three for direct loads, or one for loads by registers");
   if (n <= 0) return;
   if constexpr (FAST) {
     move(0, 0);
@@ -479,6 +504,16 @@ __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, S
       if (t + NB - 1 < n) move(t + NB - 1, free);
       step(t, buf);
       buf = buf == NB - 1 ? 0 : buf + 1;
+    }
+  } else if constexpr (NB == 1) {
+    fetch(0);
+#pragma unroll 1
+    for (int t = 0; t < n; ++t) {
+      if (t) __syncthreads();
+      put(0);
+      __syncthreads();
+      fetch(t + 1);
+      step(t, 0);
     }
   } else {
     fetch(0);
@@ -497,26 +532,26 @@ __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, S
 }
 // Buffers: three where the LDS of two or three workgroups a CU has room for them.  Short sequences spend their time
 // waiting for the first tiles: 16 x 256 tokens, 16 heads of 64, bf16, the backward's kernels together 40.7 us with three,
-// 41.7 with two, and the forward 13.0 with either.
+// 41.7 with two, and the forward 13.0 with either.  One for the long tiles of fp32 where wavefronts share queries: two
+// workgroups a CU (3525 tokens, 8 heads of 64: forward 57 us, with two buffers and one workgroup 90; or no room for more).
 template <typename T, int DP, bool FAST, int WK>
-constexpr int buffers() { return FAST && sizeof(T) == 2 && DP <= 64 && WK < 4 ? 3 : 2; }
+constexpr int buffers() { return FAST && DP <= 64 && WK < 4 ? 3 : sizeof(T) == 4 && WK > 1 ? 1 : 2; }
 
 // Whether the registers are to be limited so that two workgroups fit a CU.  The LDS of WK = 4 at rows of 256 bytes and
-// more, and the operands of fp32 at 96 elements and more, allow one.  (fp32, 3525 tokens, 8 heads of 64: forward 88 us
-// with one, 81 with two; the dK/dV kernel is slower with two, for lack of registers: 186 and 205.)
+// more, and the operands of fp32 at 96 elements and more, allow one.
 template <typename T, int DP, int WK>
-constexpr bool two_fit() { return sizeof(T) == 2 ? WK < 4 || DP <= 64 : WK < 4 && DP <= 64; }
+constexpr bool two_fit() { return sizeof(T) == 2 ? WK < 4 || DP <= 64 : WK <= 2 && DP <= 64; }
 
 // The sums of the wavefronts that share queries, each times its factor, for the blocks [db0, db1) of 32 elements: `all`
-// holds value i of block db of thread t at [(first + db * 16 + i) * 256 + t].
-template <int WK, int DB>
+// holds value i of block db of thread t at [(first + db * 16 + i) * NT + t], NT threads.
+template <int NT, int DB>
 __device__ __forceinline__ void leave_sums(float *mine, const f32x16 (&acc)[DB], int first) {
 #pragma unroll
   for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) mine[(first + db * 16 + i) * 256] = acc[db][i];
+    for (int i = 0; i < 16; ++i) mine[(first + db * 16 + i) * NT] = acc[db][i];
 }
-template <int WK, int DB>
+template <int WK, int NT, int DB>
 __device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], const float *all, int first, const float (&f)[WK], int db0, int db1) {
 #pragma unroll
   for (int db = 0; db < DB; ++db)
@@ -525,7 +560,7 @@ __device__ __forceinline__ void join_sums(f32x16 (&acc)[DB], const float *all, i
       for (int i = 0; i < 16; ++i) {
         float v = 0.f;
 #pragma unroll
-        for (int w = 0; w < WK; ++w) v += f[w] * all[(first + db * 16 + i) * 256 + w * (WAVES / WK) * 64];
+        for (int w = 0; w < WK; ++w) v += f[w] * all[(first + db * 16 + i) * NT + w * (NT / WK)];
         acc[db][i] = v;
       }
 }
@@ -602,10 +637,11 @@ __device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row
 // queries to fill the GPU.  NW = 8: 256 queries a workgroup, for long rows and many queries (see Plan).  splits > 1: the
 // workgroup takes a share of the key tiles and leaves its sums to attention_join_kernel.
 template <typename T, int DP, bool FAST, int WK, int NW = WAVES>
-__global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_kernel(const Args<T> a) {
-  constexpr int WQ = NW / WK, BQ = COLS * WQ, ROWS = WK == 1 ? 64 : 32 * WK, NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
+__global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 || NW == WAVES) ? 2 : 1)) void attention_kernel(const Args<T> a) {
+  constexpr int WQ = NW / WK, BQ = COLS * WQ, ROWS = sizeof(T) == 2 && WK == 1 ? 64 : tile_rows<T, DP, FAST, WK>();
+  constexpr int NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS, NW> TL;
-  constexpr int NB = NW == 8 ? 3 : buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * (DB * 16 + 2) * 4;
+  constexpr int NB = NW == 8 ? (FAST ? 3 : 2) : buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 64 * NW * (DB * 16 + 2) * 4;
   __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
@@ -639,7 +675,7 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void atten
   const unsigned lds0 = lds_address(lds);
   const int end = min(span.kend, (first + n) * ROWS);
   auto move = [&](int t, int buf) __attribute__((always_inline)) {
-    keys.move((first + t) * ROWS, end, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
+    if constexpr (FAST) keys.move((first + t) * ROWS, end, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
     if (!FAST) keys.fetch((first + t) * ROWS, end);
@@ -650,14 +686,14 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void atten
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const int key0 = (first + t) * ROWS + wk * 32;
     if (key0 > span.wave_some) return;
-    const unsigned char *const ldsK = lds + buf * STAGE + wk * 32 * TL::RB, *const ldsV = ldsK + TL::BYTES;
+    const unsigned char *const ldsK = lds + buf * STAGE + wk * 2 * TL::R16, *const ldsV = ldsK + TL::BYTES;
     const bool edge = key0 + NU * 32 - 1 > span.wave_all;
     f32x16 s[NU];
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       s[u] = zero16();
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) s[u] = mma(TL::along(ldsK + u * 32 * TL::RB, lo, x), q[x], s[u]);
+      for (int x = 0; x < DP / 16; ++x) s[u] = mma(TL::along(ldsK + u * 2 * TL::R16, lo, x), q[x], s[u]);
     }
     if (edge) {
 #pragma unroll
@@ -696,7 +732,7 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void atten
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int kb = key0 + u * 32;
-      TL::add(acc, ldsV + u * 32 * TL::RB, zeros, lo, s[u], edge && kb + 31 > span.wave_all,
+      TL::add(acc, ldsV + u * 2 * TL::R16, zeros, lo, s[u], edge && kb + 31 > span.wave_all,
               [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
@@ -708,8 +744,8 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void atten
     __syncthreads();
     float *const mine = reinterpret_cast<float *>(lds) + threadIdx.x;
     mine[0] = m;
-    mine[256] = l;
-    leave_sums<WK>(mine, acc, 2);
+    mine[64 * NW] = l;
+    leave_sums<64 * NW>(mine, acc, 2);
     __syncthreads();
     const float *const all = reinterpret_cast<const float *>(lds) + wq * 64 + lane;
     float f[WK];
@@ -719,11 +755,11 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() ? 2 : 1)) void atten
 #pragma unroll
     for (int w = 0; w < WK; ++w) {
       f[w] = __builtin_amdgcn_exp2f(all[w * WQ * 64] - (m == -INFINITY ? 0.f : m));
-      l += f[w] * all[256 + w * WQ * 64];
+      l += f[w] * all[64 * NW + w * WQ * 64];
     }
     db0 = min(wk * ((DB + WK - 1) / WK), DB);
     db1 = min(db0 + (DB + WK - 1) / WK, DB);
-    join_sums<WK>(acc, all, 2, f, db0, db1);
+    join_sums<WK, 64 * NW>(acc, all, 2, f, db0, db1);
   }
   if (!r.live) return;
   const i64 at = (i64)(r.s.q0 + r.query) * a.Hq + r.head;
@@ -805,10 +841,10 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
     for (int t = 0; t < DP / 16; ++t) {
       const int e = 16 * t + 8 * h;
       q[t] = load_frag<T, FAST>(p, e, a.D);
-      dout[t] = load_frag<T, FAST>(pd, e, a.D);
-      const Frag<T> o = load_frag<T, FAST>(po, e, a.D);
+      const Raw<T> d = load_eight<T, FAST>(pd, e, a.D), o = load_eight<T, FAST>(po, e, a.D);
+      dout[t] = as_frag(d);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) delta += (float)dout[t][j] * (float)o[j];
+      for (int j = 0; j < 8; ++j) delta += (float)d[j] * (float)o[j];
     }
     delta += __shfl_xor(delta, 32, 64);
   }
@@ -821,7 +857,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   KeyTiles<T, TL, FAST> keys(a, r.s, kvh);
   const unsigned lds0 = lds_address(lds);
   auto move = [&](int t, int buf) __attribute__((always_inline)) {
-    keys.move(t * ROWS, span.kend, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
+    if constexpr (FAST) keys.move(t * ROWS, span.kend, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
     if (!FAST) keys.fetch(t * ROWS, span.kend);
@@ -830,12 +866,12 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
     if (!FAST) keys.put(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
   };
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
-    const unsigned char *const ldsK = lds + buf * STAGE + wk * 32 * TL::RB, *const ldsV = ldsK + TL::BYTES;
+    const unsigned char *const ldsK = lds + buf * STAGE + wk * 2 * TL::R16, *const ldsV = ldsK + TL::BYTES;
 #pragma unroll 1
     for (int u = 0; u < NU; ++u) {
       const int kb = t * ROWS + (wk + u) * 32;
       if (kb > span.wave_some) break;
-      const unsigned char *const k32 = ldsK + u * 32 * TL::RB, *const v32 = ldsV + u * 32 * TL::RB;
+      const unsigned char *const k32 = ldsK + u * 2 * TL::R16, *const v32 = ldsV + u * 2 * TL::R16;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
       for (int x = 0; x < DP / 16; ++x) s = mma(TL::along(k32, lo, x), q[x], s);
@@ -874,14 +910,14 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
     __syncthreads();
-    leave_sums<WK>(reinterpret_cast<float *>(lds) + threadIdx.x, acc, 0);
+    leave_sums<256>(reinterpret_cast<float *>(lds) + threadIdx.x, acc, 0);
     __syncthreads();
     float f[WK];
 #pragma unroll
     for (int w = 0; w < WK; ++w) f[w] = 1.f;
     db0 = min(wk * ((DB + WK - 1) / WK), DB);
     db1 = min(db0 + (DB + WK - 1) / WK, DB);
-    join_sums<WK>(acc, reinterpret_cast<const float *>(lds) + wq * 64 + lane, 0, f, db0, db1);
+    join_sums<WK, 256>(acc, reinterpret_cast<const float *>(lds) + wq * 64 + lane, 0, f, db0, db1);
   }
   if (!r.live) return;
   if (h == 0 && wk == 0) {  // the wavefront that has seen the first keys
@@ -893,16 +929,18 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
 
 // dK and dV: keys in registers, the packed queries of the group streamed.
 template <typename T, int DP, bool FAST, int NW>
-__global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv_kernel(const Args<T> a) {
+__global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void attention_dkv_kernel(const Args<T> a) {
   constexpr int ROWS = tile_rows<T, DP, FAST, 1>();
   typedef Tile<T, DP, ROWS, NW> TL;
   constexpr int STAGE = 2 * TL::BYTES + 2 * 64 * 4;  // Q, dout, lse (base 2), delta (64 values: a wavefront's direct load)
-  constexpr int NB = buffers<T, DP, FAST, 1>();
-  // 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands, and the
-  // last two of K, stay in LDS, each wavefront's own, in the order in which the lanes read them.  (With six more
+  constexpr int NB = sizeof(T) == 4 ? 1 : buffers<T, DP, FAST, 1>();
+  // bf16, 128 elements: 128 accumulators, 32 scores and 32 of K leave no room for V in 256 registers.  Its operands, and
+  // the last two of K, stay in LDS, each wavefront's own, in the order in which the lanes read them.  (With six more
   // registers in use one operand is reloaded from scratch memory in every step, behind the direct loads in flight: 25 %
-  // slower.)
-  constexpr int KT = DP / 16, K_REG = DP < 128 ? KT : KT - 2, V_REG = DP < 128 ? KT : 0;
+  // slower.)  fp32 behind 32 elements: V's three parts, and one buffer, so that up to 64 elements two workgroups fit a CU
+  // (3525 tokens, 8 heads of 64: backward 191 us with one, 174 with two; 2048 tokens, 8 heads of 128: 522 -> 371).
+  constexpr bool ALL_REG = sizeof(T) == 2 ? DP < 128 : DP <= 32;
+  constexpr int KT = DP / 16, K_REG = ALL_REG || sizeof(T) == 4 ? KT : KT - 2, V_REG = ALL_REG ? KT : 0;
   constexpr int OWN = (2 * KT - K_REG - V_REG) * 64 * (int)sizeof(Frag<T>);
   __shared__ __align__(16) unsigned char lds[NB * STAGE + TL::ZEROS + NW * OWN];
   unsigned char *const zeros = lds + NB * STAGE;
@@ -1007,8 +1045,8 @@ __global__ __launch_bounds__(64 * NW, sizeof(T) == 2 ? 2 : 1) void attention_dkv
       const int rb = first + t * ROWS + u * 32;
       if (rb >= nrows) break;
       if (rb + 31 < wave_some) continue;
-      const unsigned char *const q32 = ldsQ + u * 32 * TL::RB, *const d32 = ldsD + u * 32 * TL::RB;
-      const auto lo = DP < 128 ? lane_at : TL::forget(lane_at);  // at 128 elements every register counts
+      const unsigned char *const q32 = ldsQ + u * 2 * TL::R16, *const d32 = ldsD + u * 2 * TL::R16;
+      const auto lo = sizeof(T) == 4 || DP < 128 ? lane_at : TL::forget(lane_at);  // at 128 elements every register counts
       f32x16 p = zero16(), ds = zero16();
 #pragma unroll
       for (int x = 0; x < DP / 16; ++x)
@@ -1125,18 +1163,20 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 // behind 64 elements), else 64, and 32 when it is a quarter or less: shorter workgroups fill the GPU evenly, but their
 // tiles serve fewer wavefronts.  Forward in us with 128 / 64 / 32 queries: 512 workgroups of 128 (16 x 256 tokens, 16
 // heads of 64, bf16) 12.6 / 17.4 / 23.6; 332 (8 sequences of up to 2049, 8/2 heads of 80, causal) 52.7 / 42.4 / 73; 224
-// (fp32, 3525 tokens, 8 heads of 64) 82 / 81 / 117; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
-// splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average (what a join
-// costs more would not be won back).
+// (fp32, 3525 tokens, 8 heads of 64) 65 / 47 / 108; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
+// splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average, 256 in fp32
+// (what a join costs more would not be won back; fp32, 4 queries over 12000 keys, 16/4 heads of 128: 59 us with 512, 37
+// with 256, but one image of 256 tokens 11.7 whole and 13.2 in two).
 // wide: 8 wavefronts and 256 queries a workgroup (forward, bf16 rows of 96 elements and more): half the direct loads, and
 // room for a third buffer; 8192 tokens, 16/4 heads of 128, causal: 293 -> 275 us.  (dQ gains nothing by it: its two
-// score products take twice as long per tile.)
+// score products take twice as long per tile.)  fp32 with 64 elements and wk = 2 takes 8 wavefronts, 128 queries, too: the
+// tiles are split into parts by twice as many threads (3525 tokens, 8 heads: 57 -> 46 us; dQ gains nothing).
 struct Plan {
   int wk, splits, tiles;  // tiles of queries: an upper bound
   bool wide;
 };
 template <typename T>
-constexpr int most_shared(int DP) { return DP * sizeof(T) > 256 ? 2 : 4; }  // the tiles of 4 would not fit the LDS
+constexpr int most_shared(int DP) { return sizeof(T) == 2 || DP <= 64 ? 4 : 2; }  // what the LDS has room for
 constexpr int padded_dim(int D) { return (D + 31) / 32 * 32; }
 template <typename T>
 Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
@@ -1145,12 +1185,14 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
   auto groups = [&](int bq) { const i64 t = (rows + bq - 1) / bq; return (t > num_seqs ? t : num_seqs) * Hkv; };
   Plan p;
   const i64 n = groups(BM);
-  p.wk = n >= places * 3 / 4 ? 1 : n > places / 4 || most == 2 ? 2 : 4;
+  p.wk = n >= places * 3 / 4 ? 1 : n > places / 4 ? 2 : 4;
+  if (p.wk > most) p.wk = most;
   p.wide = p.wk == 1 && groups(2 * BM) >= 384;
   i64 s = 1;
   if (p.wk == most && num_seqs > 0) {
     s = 256 / groups(BM / p.wk);
-    if (s > total_k / num_seqs / 512) s = total_k / num_seqs / 512;
+    const i64 most_splits = total_k / num_seqs / (sizeof(T) == 2 ? 512 : 256);
+    if (s > most_splits) s = most_splits;
   }
   p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
   p.tiles = (int)(rows / (BM / p.wk)) + num_seqs;
@@ -1163,17 +1205,21 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
 template <typename T>
 constexpr int dkv_waves(int DP) { return sizeof(T) == 2 && DP >= 96 ? 8 : WAVES; }
 // Row ranges into which their sums are split when there are few key tiles: `fit` workgroups run at once (one of 8
-// wavefronts a CU, one of fp32, else two), and where lengths differ as much as under a causal mask it takes twice as many
-// to fill the GPU evenly.  Each range costs a pass over fp32 dK and dV, so it should have 256 rows at least on the
-// average.  A power of two, so that workgroups of one range and head keep to one XCD and its L2 (workgroups go round over
-// the 8 XCDs): with 5 or 7 ranges the case above is 6 % slower than with 4; with one range it takes 1.9 ms.
+// wavefronts a CU, one of fp32 behind 64 elements, else two), and where lengths differ as much as under a causal mask it
+// takes twice as many to fill the GPU evenly.  Each range costs a pass over fp32 dK and dV, so it should have 128 rows at
+// least on the average, in bf16, and two of them are worth their join from 512 rows on (in us: 3 sequences, 1533 tokens,
+// 4/1 heads of 40, causal: ranges of 256 rows 47, of 128 37; but 4 x 256 tokens, 8 heads of 128: whole 36, in ranges of
+// 128 49); in fp32, where a row takes longer, 64 (one image of 256 tokens, 8 heads of 64: ranges of 256 46, 128 38, 64 34).
+// A power of two, so that workgroups of one range and head keep to one XCD and its L2 (workgroups go round over
+// the 8 XCDs): with 5 or 7 ranges the 8192 tokens above are 6 % slower than with 4; with one range they take 1.9 ms.
 template <typename T>
 int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, bool causal) {
-  const int nw = dkv_waves<T>(padded_dim(D)), fit = sizeof(T) == 2 && nw == 4 ? 512 : 256;
+  const int nw = dkv_waves<T>(padded_dim(D)), fit = nw == 4 && (sizeof(T) == 2 || D <= 64) ? 512 : 256;
   const i64 t = (total_k + COLS * nw - 1) / (COLS * nw), tiles = (t > num_seqs ? t : num_seqs) * Hkv;
-  const i64 rows = num_seqs ? total_q * (Hq / Hkv) / num_seqs : 0;
+  const i64 rows = num_seqs ? total_q * (Hq / Hkv) / num_seqs : 0, least = sizeof(T) == 2 ? 128 : 64;
   int s = 1;
-  while (s < 8 && s * tiles < fit * (causal ? 6 : 3) / 4 && 2 * s * 256 <= rows) s *= 2;
+  if (sizeof(T) == 2 && rows < 512) return s;
+  while (s < 8 && s * tiles < fit * (causal ? 6 : 3) / 4 && 2 * s * least <= rows) s *= 2;
   return s;
 }
 inline size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
@@ -1182,24 +1228,26 @@ inline size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
 inline size_t rows_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * 2 * sizeof(float) + 15) / 16 * 16; }
 
 // f(DP, FAST) with the head dimension padded to the tile's, and whether the streamed rows are whole aligned chunks.
-template <typename F>
+template <typename T, typename F>
 void with_dim(int D, bool fast, F f) {
   auto padded = [&](auto dp) {
-    if (fast) f(dp, std::true_type());
-    else f(dp, std::false_type());
+    if constexpr (sizeof(T) == 2)
+      if (fast) return f(dp, std::true_type());
+    f(dp, std::false_type());
   };
   if (D <= 32) padded(std::integral_constant<int, 32>());
   else if (D <= 64) padded(std::integral_constant<int, 64>());
   else if (D <= 96) padded(std::integral_constant<int, 96>());
   else padded(std::integral_constant<int, 128>());
 }
-// f(WK): the shared kernels exist for whole chunks; other inputs take workgroups of 128 queries whatever their number.
+// f(WK): bf16's shared kernels exist for whole chunks; other inputs take workgroups of 128 queries whatever their number.
 template <typename T, int DP, bool FAST, typename F>
 void with_shared(int wk, F f) {
-  if constexpr (FAST) {
+  if constexpr (FAST || sizeof(T) == 4) {
     if constexpr (most_shared<T>(DP) == 4)
       if (wk == 4) return f(std::integral_constant<int, 4>());
-    if (wk >= 2) return f(std::integral_constant<int, 2>());
+    if constexpr (most_shared<T>(DP) >= 2)
+      if (wk >= 2) return f(std::integral_constant<int, 2>());
   }
   f(std::integral_constant<int, 1>());
 }
@@ -1222,14 +1270,14 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   a.out = out, a.out_ld = out_ld, a.lse = lse;
   const bool whole = whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D);
   const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D);
-  a.tiles = whole ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+  a.tiles = whole || sizeof(T) == 4 ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   a.splits = plan.splits, a.partials = (float *)ws;
   if (plan.splits > 1) {
     const size_t need = forward_bytes(total_q, Hq, D, plan.splits);
     UNET_REQUIRE(ws && ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
     UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
   }
-  with_dim(D, whole, [&](auto dp, auto fast) {
+  with_dim<T>(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool FAST = decltype(fast)::value;
     if constexpr (FAST && sizeof(T) == 2 && DP >= 96)
@@ -1239,7 +1287,9 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
         return;
       }
     with_shared<T, DP, FAST>(plan.wk, [&](auto wk) {
-      attention_kernel<T, DP, FAST, decltype(wk)::value><<<(unsigned)a.tiles * Hkv * a.splits, 256, 0, st>>>(a);
+      constexpr int WK = decltype(wk)::value, NW = sizeof(T) == 4 && DP == 64 && WK == 2 ? 8 : WAVES;  // see Plan
+      if (NW == 8) a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+      attention_kernel<T, DP, FAST, WK, NW><<<(unsigned)a.tiles * Hkv * a.splits, 64 * NW, 0, st>>>(a);
     });
   });
   if (a.splits > 1) attention_join_kernel<T><<<cdiv_u(total_q * Hq, WAVES), 256, 0, st>>>(a);
@@ -1271,12 +1321,12 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   const bool whole =
       whole_chunks(q, q_ld, D) && whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D) && whole_chunks(dout, dout_ld, D);
   const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D);
-  a.tiles = whole ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+  a.tiles = whole || sizeof(T) == 4 ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   const int nw = dkv_waves<T>(padded_dim(D));
   const unsigned key_tiles = (unsigned)(total_k / (COLS * nw)) + num_seqs;
   a.splits = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
   a.partials = (float *)((char *)ws + rows_bytes(total_q, Hq));
-  with_dim(D, whole, [&](auto dp, auto fast) {
+  with_dim<T>(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value, NW = dkv_waves<T>(DP);
     constexpr bool FAST = decltype(fast)::value;
     if (total_q)
