@@ -991,6 +991,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
   float fl, fd;
   const unsigned lds0 = lds_address(lds);
   auto move = [&](int t, int buf) __attribute__((always_inline)) {
+    if (!FAST) return;
     const int r0 = first + t * ROWS, query0 = div_by(r0, a.G);
     unsigned qo[TL::MOVES], dof[TL::MOVES];
 #pragma unroll
@@ -1163,7 +1164,10 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 // behind 64 elements), else 64, and 32 when it is a quarter or less: shorter workgroups fill the GPU evenly, but their
 // tiles serve fewer wavefronts.  Forward in us with 128 / 64 / 32 queries: 512 workgroups of 128 (16 x 256 tokens, 16
 // heads of 64, bf16) 12.6 / 17.4 / 23.6; 332 (8 sequences of up to 2049, 8/2 heads of 80, causal) 52.7 / 42.4 / 73; 224
-// (fp32, 3525 tokens, 8 heads of 64) 65 / 47 / 108; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.
+// (fp32, 3525 tokens, 8 heads of 64) 65 / 47 / 108; 16 (256 tokens, 8 heads of 64) 10.0 / - / 6.6.  Under a causal mask
+// twice as many before it is 128: workgroups that all run at once take as long as the longest (forward + backward in us
+// with 128 / 64, 8 heads: one sequence of 6144, 64 elements, bf16 373 / 294, 128 elements 532 / 448; 8192, 64, fp32 1880 /
+// 1697; 16 of 384, 128, bf16 85 / 91).  It does not change the splits, which come with the smallest number.
 // splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average, 256 in fp32
 // (what a join costs more would not be won back; fp32, 4 queries over 12000 keys, 16/4 heads of 128: 59 us with 512, 37
 // with 256, but one image of 256 tokens 11.7 whole and 13.2 in two).
@@ -1179,13 +1183,13 @@ template <typename T>
 constexpr int most_shared(int DP) { return sizeof(T) == 2 || DP <= 64 ? 4 : 2; }  // what the LDS has room for
 constexpr int padded_dim(int D) { return (D + 31) / 32 * 32; }
 template <typename T>
-Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {
+Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, bool causal) {
   const int most = most_shared<T>(padded_dim(D)), places = sizeof(T) == 2 || D <= 64 ? 512 : 256;
   const i64 rows = total_q * (Hq / Hkv);
   auto groups = [&](int bq) { const i64 t = (rows + bq - 1) / bq; return (t > num_seqs ? t : num_seqs) * Hkv; };
   Plan p;
   const i64 n = groups(BM);
-  p.wk = n >= places * 3 / 4 ? 1 : n > places / 4 ? 2 : 4;
+  p.wk = n >= places * (causal ? 6 : 3) / 4 ? 1 : n > places / 4 ? 2 : 4;
   if (p.wk > most) p.wk = most;
   p.wide = p.wk == 1 && groups(2 * BM) >= 384;
   i64 s = 1;
@@ -1269,7 +1273,7 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   if (num_seqs == 0 || total_q == 0) return UNET_OK;
   a.out = out, a.out_ld = out_ld, a.lse = lse;
   const bool whole = whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D);
-  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D);
+  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
   a.tiles = whole || sizeof(T) == 4 ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   a.splits = plan.splits, a.partials = (float *)ws;
   if (plan.splits > 1) {
@@ -1320,7 +1324,7 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   a.dout_ld = dout_ld, a.o_ld = out_ld, a.dq_ld = dq_ld, a.dk_ld = dk_ld, a.dv_ld = dv_ld;
   const bool whole =
       whole_chunks(q, q_ld, D) && whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D) && whole_chunks(dout, dout_ld, D);
-  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D);
+  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
   a.tiles = whole || sizeof(T) == 4 ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   const int nw = dkv_waves<T>(padded_dim(D));
   const unsigned key_tiles = (unsigned)(total_k / (COLS * nw)) + num_seqs;

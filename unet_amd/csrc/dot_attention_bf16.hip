@@ -7,9 +7,9 @@ int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t to
                                        int head_dim, size_t *bytes_host) {
   UNET_REQUIRE(bytes_host, "dot_attention_workspace_bytes: NULL result");
   TRY(check_shape("dot_attention_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  const int f32 = make_plan<float>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim).splits;
-  const int bf16 = make_plan<bf16_t>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim).splits;
-  const int splits = f32 > bf16 ? f32 : bf16;  // the larger of the two types' plans
+  const int f32 = make_plan<float>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim, false).splits;
+  const int bf16 = make_plan<bf16_t>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim, false).splits;
+  const int splits = f32 > bf16 ? f32 : bf16;  // the larger of the two types' plans; a causal mask does not change them
   *bytes_host = forward_bytes(total_q, heads_q, head_dim, splits);
   return UNET_OK;
 }
