@@ -1210,10 +1210,12 @@ template <typename T>
 constexpr int dkv_waves(int DP) { return sizeof(T) == 2 && DP >= 96 ? 8 : WAVES; }
 // Row ranges into which their sums are split when there are few key tiles: `fit` workgroups run at once (one of 8
 // wavefronts a CU, one of fp32 behind 64 elements, else two), and where lengths differ as much as under a causal mask it
-// takes twice as many to fill the GPU evenly.  Each range costs a pass over fp32 dK and dV, so it should have 128 rows at
-// least on the average, in bf16, and two of them are worth their join from 512 rows on (in us: 3 sequences, 1533 tokens,
-// 4/1 heads of 40, causal: ranges of 256 rows 47, of 128 37; but 4 x 256 tokens, 8 heads of 128: whole 36, in ranges of
-// 128 49); in fp32, where a row takes longer, 64 (one image of 256 tokens, 8 heads of 64: ranges of 256 46, 128 38, 64 34).
+// takes twice as many to fill the GPU evenly, but 16 ranges only where 8 leave it empty (3 sequences, 3464 tokens, 8/1
+// heads of 80, backward: 142 us with 8, 107 with 16; 8 sequences, 5289 tokens, 8/2 heads of 80, causal: 124 and 141).
+// Each range costs a pass over fp32 dK and dV, so it should have 128 rows at least on the average, in bf16, and two of
+// them are worth their join from 512 rows on (backward in us: 3 sequences, 1533 tokens, 4/1 heads of 40, causal: ranges of
+// 256 rows 47, of 128 37; but 4 x 256 tokens, 8 heads of 128: whole 36, in ranges of 128 49); in fp32, where a row takes
+// longer, 64 (one image of 256 tokens, 8 heads of 64: ranges of 256 46, 128 38, 64 34).
 // A power of two, so that workgroups of one range and head keep to one XCD and its L2 (workgroups go round over
 // the 8 XCDs): with 5 or 7 ranges the 8192 tokens above are 6 % slower than with 4; with one range they take 1.9 ms.
 template <typename T>
@@ -1223,7 +1225,7 @@ int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
   const i64 rows = num_seqs ? total_q * (Hq / Hkv) / num_seqs : 0, least = sizeof(T) == 2 ? 128 : 64;
   int s = 1;
   if (sizeof(T) == 2 && rows < 512) return s;
-  while (s < 8 && s * tiles < fit * (causal ? 6 : 3) / 4 && 2 * s * least <= rows) s *= 2;
+  while (s < 16 && s * tiles < fit * (causal && s < 8 ? 6 : 3) / 4 && 2 * s * least <= rows) s *= 2;
   return s;
 }
 inline size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
