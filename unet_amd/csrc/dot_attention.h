@@ -22,8 +22,8 @@
 // spread over all banks.
 //
 // What bounds it, measured:
-//   - long sequences: the matrix cores.  8192 tokens, 16/4 heads of 128, causal, bf16: forward 275 us (1.0 PFLOP/s of the
-//     visible pairs), dQ 395, dK/dV 570-600, their join 23 (0.68 PFLOP/s on five products of two kernels that compute
+//   - long sequences: the matrix cores.  8192 tokens, 16/4 heads of 128, causal, bf16: forward 270 us (1.0 PFLOP/s of the
+//     visible pairs), dQ 390, dK/dV 560-590, their join 23 (0.69 PFLOP/s on five products of two kernels that compute
 //     seven; a large library product reaches 1.26).
 //   - short ones: the latency of a few tiles.  16 x 256 tokens, 16 heads of 64, bf16: forward 13 us, dQ 20.5, dK/dV 21 for
 //     34 to 50 MB each.
@@ -160,7 +160,7 @@ struct Args {
   T *out, *dq, *dk, *dv;
   i64 q_ld, k_ld, v_ld, o_ld, dout_ld, out_ld, dq_ld, dk_ld, dv_ld;
   float *lse, *partials;
-  float *rows;  // for the dK/dV kernel: lse in base 2, then delta, [total_q][Hq] each
+  float *rows;  // for the dK/dV kernel: lse in base 2, then -delta, [total_q][Hq] each
   const int *cu_q, *cu_k;
   int num_seqs, total_q, total_k, Hq, Hkv, D, causal, tiles, splits;
   Div G;
@@ -343,7 +343,7 @@ struct Tile {
   // rows are added one at a time, the result taken by the columns that see the row, and the common product reads
   // zeros instead.  Rare, so slow is fine; what matters is that the accumulators stay where they are.
   // TWICE: a bf16 weight is taken as the sum of two bf16 numbers, its rounding and what that left over.
-  static constexpr int ZEROS = R16;
+  static constexpr int ZEROS = sizeof(T) == 2 ? 2 * R16 : R16;
   template <bool TWICE = false, typename Sees>
   static __device__ __forceinline__ void add(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const unsigned char *zeros,
                                              const Lane &o, const f32x16 &w, bool edge, Sees sees) {
@@ -355,7 +355,7 @@ struct Tile {
       for (int i = 0; i < 16; ++i) rest[i] = w[i] - (float)(i < 8 ? b0[i & 7] : b1[i & 7]);
       c0 = pack8<T>(rest, 0), c1 = pack8<T>(rest, 1);
     }
-    const unsigned char *low = rows32, *high = rows32 + R16;
+    const unsigned char *low = rows32, *high = rows32 + R16;  // (bf16: low + R16 throughout, an offset in the instruction)
     if (edge && not_finite(rows32, o)) {
       const int h = (threadIdx.x & 63) >> 5;
 #pragma unroll 1
@@ -384,7 +384,7 @@ struct Tile {
     }
 #pragma unroll
     for (int db = 0; db < DP / 32; ++db) {
-      const Frag<T> x = down(high, o, db);
+      const Frag<T> x = down(ZEROS > R16 ? low + R16 : high, o, db);
       acc[db] = mma(x, b1, acc[db]);
       if constexpr (TWICE) acc[db] = mma(x, c1, acc[db]);
     }
@@ -690,11 +690,11 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 |
     const bool edge = key0 + NU * 32 - 1 > span.wave_all;
     f32x16 s[NU];
 #pragma unroll
-    for (int u = 0; u < NU; ++u) {
-      s[u] = zero16();
+    for (int u = 0; u < NU; ++u) s[u] = zero16();
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) s[u] = mma(TL::along(ldsK + u * 2 * TL::R16, lo, x), q[x], s[u]);
-    }
+    for (int x = 0; x < DP / 16; ++x)  // the pieces in turn: no product waits for the one in front of it
+#pragma unroll
+      for (int u = 0; u < NU; ++u) s[u] = mma(TL::along(ldsK + u * 2 * TL::R16, lo, x), q[x], s[u]);
     if (edge) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
@@ -874,9 +874,10 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
       const unsigned char *const k32 = ldsK + u * 2 * TL::R16, *const v32 = ldsV + u * 2 * TL::R16;
       f32x16 s = zero16(), dp = zero16();
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) s = mma(TL::along(k32, lo, x), q[x], s);
-#pragma unroll
-      for (int x = 0; x < DP / 16; ++x) dp = mma(TL::along(v32, lo, x), dout[x], dp);
+      for (int x = 0; x < DP / 16; ++x) {
+        s = mma(TL::along(k32, lo, x), q[x], s);
+        dp = mma(TL::along(v32, lo, x), dout[x], dp);
+      }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale2 - lse2);
       const bool edge = kb + 31 > span.wave_all;
@@ -922,7 +923,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   if (!r.live) return;
   if (h == 0 && wk == 0) {  // the wavefront that has seen the first keys
     a.rows[at] = lse2;
-    a.rows[at + (i64)a.total_q * a.Hq] = delta;
+    a.rows[at + (i64)a.total_q * a.Hq] = -delta;
   }
   store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale, db0, db1);
 }
@@ -1048,7 +1049,13 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
       if (rb + 31 < wave_some) continue;
       const unsigned char *const q32 = ldsQ + u * 2 * TL::R16, *const d32 = ldsD + u * 2 * TL::R16;
       const auto lo = sizeof(T) == 4 || DP < 128 ? lane_at : TL::forget(lane_at);  // at 128 elements every register counts
-      f32x16 p = zero16(), ds = zero16();
+      f32x16 p = zero16(), ds;  // dP - delta: the accumulators begin with -delta
+#pragma unroll
+      for (int b = 0; b < 4; ++b) {
+        const f32x4 d = *reinterpret_cast<const f32x4 *>(ldsDelta + u * 32 + 8 * b + 4 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ds[4 * b + i] = d[i];
+      }
 #pragma unroll
       for (int x = 0; x < DP / 16; ++x)
         p = mma(TL::along(q32, lo, x), x < K_REG ? kr[x < K_REG ? x : 0] : own[64 * (KT - V_REG + x - K_REG)], p);
@@ -1058,11 +1065,10 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(ldsL + u * 32 + 8 * b + 4 * h);
-        const f32x4 delta = *reinterpret_cast<const f32x4 *>(ldsDelta + u * 32 + 8 * b + 4 * h);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           p[4 * b + i] = __builtin_amdgcn_exp2f(p[4 * b + i] * a.scale2 - lse2[i]);
-          ds[4 * b + i] = p[4 * b + i] * (ds[4 * b + i] - delta[i]);
+          ds[4 * b + i] *= p[4 * b + i];
         }
       }
       const bool edge = rb < wave_all;
