@@ -867,7 +867,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   };
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const unsigned char *const ldsK = lds + buf * STAGE + wk * 2 * TL::R16, *const ldsV = ldsK + TL::BYTES;
-#pragma unroll 1
+#pragma unroll (sizeof(T) == 2 ? 2 : 1)  // two pieces share their addresses
     for (int u = 0; u < NU; ++u) {
       const int kb = t * ROWS + (wk + u) * 32;
       if (kb > span.wave_some) break;
@@ -1042,13 +1042,13 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const unsigned char *const ldsQ = lds + buf * STAGE, *const ldsD = ldsQ + TL::BYTES;
     const float *const ldsL = reinterpret_cast<const float *>(ldsD + TL::BYTES), *const ldsDelta = ldsL + 64;
-#pragma unroll 1
+#pragma unroll (sizeof(T) == 2 && DP < 128 ? 2 : 1)  // as above; at 128 elements every register counts
     for (int u = 0; u < ROWS / 32; ++u) {
       const int rb = first + t * ROWS + u * 32;
       if (rb >= nrows) break;
       if (rb + 31 < wave_some) continue;
       const unsigned char *const q32 = ldsQ + u * 2 * TL::R16, *const d32 = ldsD + u * 2 * TL::R16;
-      const auto lo = sizeof(T) == 4 || DP < 128 ? lane_at : TL::forget(lane_at);  // at 128 elements every register counts
+      const auto lo = sizeof(T) == 4 || DP < 128 ? lane_at : TL::forget(lane_at);
       f32x16 p = zero16(), ds;  // dP - delta: the accumulators begin with -delta
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
