@@ -865,9 +865,10 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   auto put = [&](int buf) __attribute__((always_inline)) {
     if (!FAST) keys.put(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
   };
+  constexpr int UNROLL = sizeof(T) == 2 ? 2 : 1;
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const unsigned char *const ldsK = lds + buf * STAGE + wk * 2 * TL::R16, *const ldsV = ldsK + TL::BYTES;
-#pragma unroll (sizeof(T) == 2 ? 2 : 1)  // two pieces share their addresses
+#pragma unroll UNROLL  // two pieces share their addresses
     for (int u = 0; u < NU; ++u) {
       const int kb = t * ROWS + (wk + u) * 32;
       if (kb > span.wave_some) break;
@@ -1039,10 +1040,11 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
       f[64] = fd;
     }
   };
+  constexpr int UNROLL = sizeof(T) == 2 && DP < 128 ? 2 : 1;
   auto step = [&](int t, int buf) __attribute__((always_inline)) {
     const unsigned char *const ldsQ = lds + buf * STAGE, *const ldsD = ldsQ + TL::BYTES;
     const float *const ldsL = reinterpret_cast<const float *>(ldsD + TL::BYTES), *const ldsDelta = ldsL + 64;
-#pragma unroll (sizeof(T) == 2 && DP < 128 ? 2 : 1)  // as above; at 128 elements every register counts
+#pragma unroll UNROLL  // as above; at 128 elements every register counts
     for (int u = 0; u < ROWS / 32; ++u) {
       const int rb = first + t * ROWS + u * 32;
       if (rb >= nrows) break;
