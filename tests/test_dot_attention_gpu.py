@@ -143,6 +143,27 @@ def test_split_sums(name, causal, shape, pad):
         assert torch.equal(a, b)
 
 
+# few heads and one or two sequences: dQ is summed in parts, and the workspace holds them where dK's and dV's need less
+FEW = [([700], [700], 2, 1, 128), ([600, 9], [1300, 40], 1, 1, 100), ([900], [2100], 2, 2, 40), ([300], [2500], 4, 2, 20), ([65, 0, 1], [800, 300, 700], 1, 1, 96)]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("pad", [0, 1])
+@pytest.mark.parametrize("shape", FEW, ids=lambda s: "x".join(map(str, [max(s[0]), max(s[1]), *s[2:]])))
+def test_few_heads(name, causal, pad, shape):
+    c = Call(name, *shape, causal, pad=pad, behind=4)
+    c.forward()
+    c.backward()
+    c.verify()
+    first = [t.clone() for t in (c.out, c.lse, c.dq, c.dk, c.dv)]
+    c.wsb.fill_(255)
+    c.forward()
+    c.backward()
+    for a, b in zip(first, (c.out, c.lse, c.dq, c.dk, c.dv)):
+        assert torch.equal(a, b)
+
+
 def test_thousands_of_sequences():
     """More sequences than 64 x 64: found in three looks.  Empty ones among them."""
     g = torch.Generator().manual_seed(9)

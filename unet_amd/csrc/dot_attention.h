@@ -812,7 +812,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const Args<T> a) {
   if (a.lse && lane == 0) a.lse[at] = none ? -INFINITY : (m + __builtin_amdgcn_logf(l)) * LN2;
 }
 
-// dQ, and lse and delta for the kernel below.  WK as in the forward.
+// dQ, and lse and delta for the kernel below.  WK and splits as in the forward.
 template <typename T, int DP, bool FAST, int WK>
 __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention_dq_kernel(const Args<T> a) {
   constexpr int WQ = WAVES / WK, BQ = COLS * WQ, ROWS = tile_rows<T, DP, FAST, WK>(), NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
@@ -821,8 +821,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
-  const int kvh = blockIdx.x % a.Hkv;
-  const int t0 = blockIdx.x / a.Hkv;
+  const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits, t0 = bs / a.splits;
   const int tile = a.causal ? a.tiles - 1 - t0 : t0;
   Rows r;
   int row0;
@@ -856,11 +855,18 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
   KeyTiles<T, TL, FAST> keys(a, r.s, kvh);
   const unsigned lds0 = lds_address(lds);
+  int first = 0, n = (span.kend + ROWS - 1) / ROWS;  // key tiles
+  if (a.splits > 1) {
+    const int per = (n + a.splits - 1) / a.splits;
+    first = min(split * per, n);
+    n = min(per, n - first);
+  }
+  const int end = min(span.kend, (first + n) * ROWS);
   auto move = [&](int t, int buf) __attribute__((always_inline)) {
-    if constexpr (FAST) keys.move(t * ROWS, span.kend, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
+    if constexpr (FAST) keys.move((first + t) * ROWS, end, lds0 + buf * STAGE, lds0 + buf * STAGE + TL::BYTES);
   };
   auto fetch = [&](int t) __attribute__((always_inline)) {
-    if (!FAST) keys.fetch(t * ROWS, span.kend);
+    if (!FAST) keys.fetch((first + t) * ROWS, end);
   };
   auto put = [&](int buf) __attribute__((always_inline)) {
     if (!FAST) keys.put(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
@@ -870,7 +876,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
     const unsigned char *const ldsK = lds + buf * STAGE + wk * 2 * TL::R16, *const ldsV = ldsK + TL::BYTES;
 #pragma unroll UNROLL  // two pieces share their addresses
     for (int u = 0; u < NU; ++u) {
-      const int kb = t * ROWS + (wk + u) * 32;
+      const int kb = (first + t) * ROWS + (wk + u) * 32;
       if (kb > span.wave_some) break;
       const unsigned char *const k32 = ldsK + u * 2 * TL::R16, *const v32 = ldsV + u * 2 * TL::R16;
       f32x16 s = zero16(), dp = zero16();
@@ -908,7 +914,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
                                                    [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
     }
   };
-  stream<FAST, NB, 2 * TL::MOVES>((span.kend + ROWS - 1) / ROWS, move, fetch, put, step);
+  stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step);
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
     __syncthreads();
@@ -922,11 +928,30 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
     join_sums<WK, 256>(acc, reinterpret_cast<const float *>(lds) + wq * 64 + lane, 0, f, db0, db1);
   }
   if (!r.live) return;
-  if (h == 0 && wk == 0) {  // the wavefront that has seen the first keys
+  const i64 plane = (i64)a.total_q * a.Hq;
+  if (h == 0 && wk == 0 && split == 0) {  // the wavefront that has seen the first keys
     a.rows[at] = lse2;
-    a.rows[at + (i64)a.total_q * a.Hq] = -delta;
+    a.rows[at + plane] = -delta;
+  }
+  if (a.splits > 1) {
+    store_column<float, DP>(a.partials + (split * plane + at) * a.D, a.D, acc, a.scale, db0, db1);
+    return;
   }
   store_column<T, DP>(a.dq + (i64)(r.s.q0 + r.query) * a.dq_ld + r.head * a.D, a.D, acc, a.scale, db0, db1);
+}
+
+// dQ from its sums over the shares of the keys, in their order.
+template <typename T>
+__global__ __launch_bounds__(256) void attention_dq_join_kernel(const Args<T> a) {
+  const int q0 = bound_of(a.cu_q, 0, a.total_q), q1 = max(bound_of(a.cu_q, a.num_seqs, a.total_q), q0);
+  const int cols = a.Hq * a.D;
+  const i64 plane = (i64)a.total_q * cols, end = (i64)q1 * cols;
+  for (i64 i = (i64)q0 * cols + (i64)blockIdx.x * 256 + threadIdx.x; i < end; i += (i64)gridDim.x * 256) {
+    float dq = 0.f;
+    for (int s = 0; s < a.splits; ++s) dq += a.partials[s * plane + i];
+    const i64 query = i / cols;
+    from_f32(dq, a.dq[query * a.dq_ld + i - query * cols]);
+  }
 }
 
 // dK and dV: keys in registers, the packed queries of the group streamed.
@@ -1177,14 +1202,17 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 // with 128 / 64, 8 heads: one sequence of 6144, 64 elements, bf16 373 / 294, 128 elements 532 / 448; 8192, 64, fp32 1880 /
 // 1697; 16 of 384, 128, bf16 85 / 91).  It does not change the splits, which come with the smallest number.
 // splits: ranges of the keys (forward), when that is still too few, each of at least 512 keys on the average, 256 in fp32
+// and for rows through registers
 // (what a join costs more would not be won back; fp32, 4 queries over 12000 keys, 16/4 heads of 128: 59 us with 512, 37
 // with 256, but one image of 256 tokens 11.7 whole and 13.2 in two).
 // wide: 8 wavefronts and 256 queries a workgroup (forward, bf16 rows of 96 elements and more): half the direct loads, and
 // room for a third buffer; 8192 tokens, 16/4 heads of 128, causal: 293 -> 275 us.  (dQ gains nothing by it: its two
 // score products take twice as long per tile.)  fp32 with 64 elements and wk = 2 takes 8 wavefronts, 128 queries, too: the
 // tiles are split into parts by twice as many threads (3525 tokens, 8 heads: 57 -> 46 us; dQ gains nothing).
+// dq_splits: the same for dQ, 256 keys at least in both types, at most 8 (backward in us: 3000 tokens, 2/1 heads of 128, fp32
+// 463 whole, 344 in two; 976 tokens, 2 heads of 100, bf16 99 whole, 68 in three).
 struct Plan {
-  int wk, splits, tiles;  // tiles of queries: an upper bound
+  int wk, splits, dq_splits, tiles;  // tiles of queries: an upper bound
   bool wide;
 };
 template <typename T>
@@ -1192,7 +1220,8 @@ constexpr int most_shared(int DP) { return sizeof(T) == 2 || DP <= 64 ? 4 : 2; }
 constexpr int padded_dim(int D) { return (D + 31) / 32 * 32; }
 template <typename T>
 Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, bool causal) {
-  const int most = most_shared<T>(padded_dim(D)), places = sizeof(T) == 2 || D <= 64 ? 512 : 256;
+  // (a bf16 row that is no whole number of 16-byte chunks takes 128 queries a workgroup always)
+  const int most = sizeof(T) == 2 && D % 8 ? 1 : most_shared<T>(padded_dim(D)), places = sizeof(T) == 2 || D <= 64 ? 512 : 256;
   const i64 rows = total_q * (Hq / Hkv);
   auto groups = [&](int bq) { const i64 t = (rows + bq - 1) / bq; return (t > num_seqs ? t : num_seqs) * Hkv; };
   Plan p;
@@ -1200,13 +1229,14 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
   p.wk = n >= places * (causal ? 6 : 3) / 4 ? 1 : n > places / 4 ? 2 : 4;
   if (p.wk > most) p.wk = most;
   p.wide = p.wk == 1 && groups(2 * BM) >= 384;
-  i64 s = 1;
-  if (p.wk == most && num_seqs > 0) {
-    s = 256 / groups(BM / p.wk);
-    const i64 most_splits = total_k / num_seqs / (sizeof(T) == 2 ? 512 : 256);
-    if (s > most_splits) s = most_splits;
-  }
-  p.splits = (int)(s < 1 ? 1 : s > 64 ? 64 : s);
+  auto shares = [&](i64 keys, i64 limit) {
+    if (p.wk != most || num_seqs == 0) return 1;
+    i64 s = 256 / groups(BM / p.wk);
+    if (s > total_k / num_seqs / keys) s = total_k / num_seqs / keys;
+    return (int)(s < 1 ? 1 : s > limit ? limit : s);
+  };
+  p.splits = shares(sizeof(T) == 2 && D % 8 == 0 ? 512 : 256, 64);
+  p.dq_splits = shares(256, 8);
   p.tiles = (int)(rows / (BM / p.wk)) + num_seqs;
   return p;
 }
@@ -1238,6 +1268,14 @@ int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
 }
 inline size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
   return splits > 1 ? (size_t)splits * total_q * Hq * (D + 2) * sizeof(float) : 0;
+}
+template <typename T>
+size_t partial_bytes(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {  // of the backward: dQ's, then dK's and dV's
+  const int dkv = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, true);  // causal calls take no fewer than others
+  const int dq = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D, true).dq_splits;  // and the same number here
+  const size_t b_dkv = dkv > 1 ? (size_t)dkv * 2 * total_k * Hkv * D * sizeof(float) : 0;
+  const size_t b_dq = dq > 1 ? (size_t)dq * total_q * Hq * D * sizeof(float) : 0;
+  return b_dkv > b_dq ? b_dkv : b_dq;
 }
 inline size_t rows_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * 2 * sizeof(float) + 15) / 16 * 16; }
 
@@ -1338,15 +1376,17 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   a.tiles = whole || sizeof(T) == 4 ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   const int nw = dkv_waves<T>(padded_dim(D));
   const unsigned key_tiles = (unsigned)(total_k / (COLS * nw)) + num_seqs;
-  a.splits = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
   a.partials = (float *)((char *)ws + rows_bytes(total_q, Hq));
+  a.splits = plan.dq_splits;
   with_dim<T>(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value, NW = dkv_waves<T>(DP);
     constexpr bool FAST = decltype(fast)::value;
     if (total_q)
       with_shared<T, DP, FAST>(plan.wk, [&](auto wk) {
-        attention_dq_kernel<T, DP, FAST, decltype(wk)::value><<<(unsigned)a.tiles * Hkv, 256, 0, st>>>(a);
+        attention_dq_kernel<T, DP, FAST, decltype(wk)::value><<<(unsigned)a.tiles * Hkv * a.splits, 256, 0, st>>>(a);
       });
+    if (total_q && a.splits > 1) attention_dq_join_kernel<T><<<ew_grid(total_q * Hq * D), 256, 0, st>>>(a);
+    a.splits = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
     if (total_k) attention_dkv_kernel<T, DP, FAST, NW><<<key_tiles * Hkv * a.splits, 64 * NW, 0, st>>>(a);
   });
   if (total_k && a.splits > 1) attention_dkv_join_kernel<T><<<ew_grid(total_k * Hkv * D), 256, 0, st>>>(a);

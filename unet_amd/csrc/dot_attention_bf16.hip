@@ -17,11 +17,9 @@ int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, i
                                                 int heads_kv, int head_dim, size_t *bytes_host) {
   UNET_REQUIRE(bytes_host, "dot_attention_backward_workspace_bytes: NULL result");
   TRY(check_shape("dot_attention_backward_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  const int f32 = dkv_splits<float>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim, true);
-  const int bf16 = dkv_splits<bf16_t>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim, true);
-  const int splits = f32 > bf16 ? f32 : bf16;  // the larger of the two types' plans; causal calls take no fewer than others
-  *bytes_host = rows_bytes(total_q, heads_q) +
-                (splits > 1 ? (size_t)splits * 2 * total_k * heads_kv * head_dim * sizeof(float) : 0);
+  const size_t f32 = partial_bytes<float>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim);
+  const size_t bf16 = partial_bytes<bf16_t>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim);
+  *bytes_host = rows_bytes(total_q, heads_q) + (f32 > bf16 ? f32 : bf16);
   return UNET_OK;
 }
 
