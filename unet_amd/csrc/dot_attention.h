@@ -634,7 +634,7 @@ __device__ __forceinline__ Span span_of(const Args<T> &a, const Rows &r, int row
 
 // The forward.  WK wavefronts share the same 32 queries and take the 32-row pieces of a tile in turn: with WK = 1 a
 // workgroup has 128 queries (every tile serves four times 32), with WK > 1 it has fewer, for calls that have too few
-// queries to fill the GPU.  NW = 8: 256 queries a workgroup, for long rows and many queries (see Plan).  splits > 1: the
+// queries to fill the GPU.  NW = 8: twice as many (see Plan for when).  splits > 1: the
 // workgroup takes a share of the key tiles and leaves its sums to attention_join_kernel.
 template <typename T, int DP, bool FAST, int WK, int NW = WAVES>
 __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 || NW == WAVES) ? 2 : 1)) void attention_kernel(const Args<T> a) {
