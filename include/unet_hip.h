@@ -368,6 +368,7 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  * accumulators are fp32 (weights are up to 2^8 before the division at the end, so values larger than the largest number
  * over 256 * keys may overflow); the bf16 form rounds the softmax weights to bf16 for their product with V.  Equal calls
  * give equal bits.  out must not overlap q, k or v.  total_q * heads_q and total_k * heads_kv may be up to about 2^29.
+ * heads_q * head_dim is less than 2^31.
  * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
  * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the
  * same time need one each.  The calls allocate nothing and can be captured into a graph. */

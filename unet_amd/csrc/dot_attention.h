@@ -1152,9 +1152,11 @@ inline int check_shape(const char *name, int num_seqs, i64 total_q, i64 total_k,
   UNET_REQUIRE(Hq >= 1 && Hkv >= 1 && Hq % Hkv == 0, "%s: %d query heads are no multiple of %d key/value heads", name, Hq, Hkv);
   UNET_REQUIRE(D >= 1, "%s: head_dim %d", name, D);
   if (D > 128) return unet_set_error(UNET_ERR_UNSUPPORTED, "%s: head_dim %d is larger than 128", name, D);
-  // rows are counted in 32 bits, and a launch has fewer than 2^32 threads (512 a workgroup at most, splits only for few)
-  const i64 most = ((i64)1 << 31) - 256, groups = (i64)1 << 22, rows = total_q * (Hq / Hkv);
-  UNET_REQUIRE(total_q <= most && total_k <= most && rows <= most && rows / BM + num_seqs <= groups / Hkv &&
+  // a token's elements and the rows are counted in 32 bits, and a launch has fewer than 2^32 threads (512 a workgroup at
+  // most, splits only for few)
+  UNET_REQUIRE((i64)Hq * D < (i64)1 << 31, "%s: %d heads of %d elements are too many", name, Hq, D);
+  const i64 most = ((i64)1 << 31) - 256, groups = (i64)1 << 22, g = Hq / Hkv;
+  UNET_REQUIRE(total_q <= most && total_k <= most && total_q * g <= most && total_q * g / BM + num_seqs <= groups / Hkv &&
                    total_k / BM + num_seqs <= groups / Hkv,
                "%s: too many tokens (%lld queries, %lld keys, %d and %d heads)", name, (long long)total_q, (long long)total_k,
                Hq, Hkv);
