@@ -371,7 +371,8 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  * heads_q * head_dim is less than 2^31.
  * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
  * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the
- * same time need one each.  The calls allocate nothing and can be captured into a graph. */
+ * same time need one each.  That size does for every call with the same heads and head_dim, no more queries and no more
+ * keys, however many sequences; so does the backward's.  The calls allocate nothing and can be captured into a graph. */
 int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q, int heads_kv,
                                        int head_dim, size_t *bytes_host);
 int unet_dot_attention_f32(const float *q, int64_t q_ld, const float *k, int64_t k_ld, const float *v, int64_t v_ld,

@@ -1,0 +1,49 @@
+"""Dot-product attention and layer norm at the ends of what their header allows: workspaces of other sizes than the call's own,
+infinities that a query sees, the largest numbers, sums of a few and of very many terms.  Definitions and bounds: seq_ref.py."""
+import ctypes
+
+import pytest
+import torch
+
+from gpu_util import DEV
+from test_dot_attention_gpu import Call
+from unet_amd import capi
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- workspaces -----------------------------------------------------------------------------------------
+
+def poisoned(f, *shape):
+    """A workspace of the size that f names for the shape, 4 KB behind it, all bytes 255."""
+    n = ctypes.c_size_t()
+    f(*shape, ctypes.byref(n))
+    whole = torch.full((n.value + 4096,), 255, dtype=torch.uint8, device=DEV)
+    return whole[:n.value], whole[n.value:]
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lens_q,lens_k,hq,hk,d", [([1024], [1024], 8, 8, 64), ([300, 211], [300, 211], 4, 1, 100), ([1, 1], [5000, 3000], 8, 1, 128),
+                                                   ([700], [700], 2, 1, 128), ([3] * 40, [9] * 40, 2, 2, 16), ([257], [4000], 1, 1, 40)])
+def test_a_workspace_for_a_larger_call(name, causal, lens_q, lens_k, hq, hk, d):
+    c = Call(name, lens_q, lens_k, hq, hk, d, causal, behind=2)
+    large = (70, 60000, 600000, hq, hk, d)
+    c.ws, behind = poisoned(capi.unet_dot_attention_workspace_bytes, *large)
+    c.wsb, behind_b = poisoned(capi.unet_dot_attention_backward_workspace_bytes, *large)
+    c.forward()
+    c.backward()
+    c.verify()
+    assert (behind == 255).all() and (behind_b == 255).all()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("lens_q,lens_k,hq,hk,d", [([1024], [1024], 8, 8, 64), ([1, 1], [5000, 3000], 8, 1, 128), ([700], [700], 2, 1, 128)])
+def test_nothing_is_written_behind_a_workspace(name, lens_q, lens_k, hq, hk, d):
+    c = Call(name, lens_q, lens_k, hq, hk, d, True)
+    c.ws, behind = poisoned(capi.unet_dot_attention_workspace_bytes, *c.shape)
+    c.wsb, behind_b = poisoned(capi.unet_dot_attention_backward_workspace_bytes, *c.shape)
+    c.forward()
+    c.backward()
+    c.verify()
+    assert (behind == 255).all() and (behind_b == 255).all()

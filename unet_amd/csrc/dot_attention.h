@@ -1220,6 +1220,7 @@ struct Plan {
 template <typename T>
 constexpr int most_shared(int DP) { return sizeof(T) == 2 || DP <= 64 ? 4 : 2; }  // what the LDS has room for
 constexpr int padded_dim(int D) { return (D + 31) / 32 * 32; }
+constexpr int MOST_SHARES = 64, MOST_DQ_SHARES = 8, MOST_RANGES = 16;  // of the keys (forward, dQ), of the rows (dK and dV)
 template <typename T>
 Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, bool causal) {
   // (a bf16 row that is no whole number of 16-byte chunks takes 128 queries a workgroup always)
@@ -1237,8 +1238,8 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
     if (s > total_k / num_seqs / keys) s = total_k / num_seqs / keys;
     return (int)(s < 1 ? 1 : s > limit ? limit : s);
   };
-  p.splits = shares(sizeof(T) == 2 && D % 8 == 0 ? 512 : 256, 64);
-  p.dq_splits = shares(256, 8);
+  p.splits = shares(sizeof(T) == 2 && D % 8 == 0 ? 512 : 256, MOST_SHARES);
+  p.dq_splits = shares(256, MOST_DQ_SHARES);
   p.tiles = (int)(rows / (BM / p.wk)) + num_seqs;
   return p;
 }
@@ -1265,19 +1266,27 @@ int dkv_splits(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
   const i64 rows = num_seqs ? total_q * (Hq / Hkv) / num_seqs : 0, least = sizeof(T) == 2 ? 128 : 64;
   int s = 1;
   if (sizeof(T) == 2 && rows < 512) return s;
-  while (s < 16 && s * tiles < fit * (causal && s < 8 ? 6 : 3) / 4 && 2 * s * least <= rows) s *= 2;
+  while (s < MOST_RANGES && s * tiles < fit * (causal && s < 8 ? 6 : 3) / 4 && 2 * s * least <= rows) s *= 2;
   return s;
 }
-inline size_t forward_bytes(i64 total_q, int Hq, int D, int splits) {
-  return splits > 1 ? (size_t)splits * total_q * Hq * (D + 2) * sizeof(float) : 0;
+// What the shares of a plan take in the workspace: fp32 rows of D + 2 (forward), D (dQ) and 2 D (dK and dV) numbers.
+inline i64 share_rows(i64 shares, i64 rows) { return shares > 1 ? shares * rows : 0; }
+inline size_t forward_bytes(i64 rows, int D) { return (size_t)rows * (D + 2) * sizeof(float); }
+inline size_t backward_bytes(i64 dq_rows, i64 dkv_rows, int D) {
+  return (size_t)(dq_rows > 2 * dkv_rows ? dq_rows : 2 * dkv_rows) * D * sizeof(float);
 }
-template <typename T>
-size_t partial_bytes(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D) {  // of the backward: dQ's, then dK's and dV's
-  const int dkv = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, true);  // causal calls take no fewer than others
-  const int dq = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D, true).dq_splits;  // and the same number here
-  const size_t b_dkv = dkv > 1 ? (size_t)dkv * 2 * total_k * Hkv * D * sizeof(float) : 0;
-  const size_t b_dq = dq > 1 ? (size_t)dq * total_q * Hq * D * sizeof(float) : 0;
-  return b_dkv > b_dq ? b_dkv : b_dq;
+// Rows enough for either storage type, with a causal mask or without, any number of sequences and no more queries and keys
+// than these.  (Not those of the plan with these sizes: fewer tokens are cut into more shares.)
+//   - make_plan has at most 256 / workgroups shares of the keys, and a workgroup has at most BM of the total_q * Hq rows:
+//     together 256 * BM rows; a share has 256 keys at least on the average.
+//   - dkv_splits doubles while shares * tiles < 3 / 2 fit, and a tile has 32 * waves of the total_k * Hkv keys: together less
+//     than 3 * fit * 32 * waves rows, which is 3 * 512 * BM for 4 waves and for 8; a share has 64 rows at least.
+inline i64 least_of(i64 a, i64 b) { return a < b ? a : b; }
+inline i64 most_query_rows(i64 total_q, i64 total_k, int Hq, i64 shares) {
+  return least_of(share_rows(least_of(shares, total_k / 256), total_q * Hq), 256 * BM);
+}
+inline i64 most_key_rows(i64 total_q, i64 total_k, int Hq, int Hkv) {
+  return least_of(share_rows(least_of(MOST_RANGES, total_q * (Hq / Hkv) / 64), total_k * Hkv), 3 * 512 * BM);
 }
 inline size_t rows_bytes(i64 total_q, int Hq) { return ((size_t)total_q * Hq * 2 * sizeof(float) + 15) / 16 * 16; }
 
@@ -1327,7 +1336,7 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   a.tiles = whole || sizeof(T) == 4 ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   a.splits = plan.splits, a.partials = (float *)ws;
   if (plan.splits > 1) {
-    const size_t need = forward_bytes(total_q, Hq, D, plan.splits);
+    const size_t need = forward_bytes(share_rows(plan.splits, total_q * Hq), D);
     UNET_REQUIRE(ws && ws_bytes >= need, "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
     UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
   }
@@ -1365,8 +1374,10 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   TRY(check_matrix(name, "grad_k", (const T *)dk, dk_ld, total_k, (i64)Hkv * D));
   TRY(check_matrix(name, "grad_v", (const T *)dv, dv_ld, total_k, (i64)Hkv * D));
   UNET_REQUIRE((lse || total_q == 0) && aligned<float>(lse), "%s: lse is NULL or misaligned", name);
-  size_t need = 0;
-  TRY(unet_dot_attention_backward_workspace_bytes(num_seqs, total_q, total_k, Hq, Hkv, D, &need));
+  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
+  const int dkv = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
+  const size_t need =
+      rows_bytes(total_q, Hq) + backward_bytes(share_rows(plan.dq_splits, total_q * Hq), share_rows(dkv, total_k * Hkv), D);
   UNET_REQUIRE(ws_bytes >= need && (ws || !need), "%s: workspace of %zu bytes, needs %zu", name, ws_bytes, need);
   UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "%s: the workspace is not 16-byte aligned", name);
   if (num_seqs == 0 || (total_q == 0 && total_k == 0)) return UNET_OK;
@@ -1374,7 +1385,6 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
   a.dout_ld = dout_ld, a.o_ld = out_ld, a.dq_ld = dq_ld, a.dk_ld = dk_ld, a.dv_ld = dv_ld;
   const bool whole =
       whole_chunks(q, q_ld, D) && whole_chunks(k, k_ld, D) && whole_chunks(v, v_ld, D) && whole_chunks(dout, dout_ld, D);
-  const Plan plan = make_plan<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
   a.tiles = whole || sizeof(T) == 4 ? plan.tiles : (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
   const int nw = dkv_waves<T>(padded_dim(D));
   const unsigned key_tiles = (unsigned)(total_k / (COLS * nw)) + num_seqs;
@@ -1388,7 +1398,7 @@ int backward(const T *dout, i64 dout_ld, const T *q, i64 q_ld, const T *k, i64 k
         attention_dq_kernel<T, DP, FAST, decltype(wk)::value><<<(unsigned)a.tiles * Hkv * a.splits, 256, 0, st>>>(a);
       });
     if (total_q && a.splits > 1) attention_dq_join_kernel<T><<<ew_grid(total_q * Hq * D), 256, 0, st>>>(a);
-    a.splits = dkv_splits<T>(num_seqs, total_q, total_k, Hq, Hkv, D, a.causal);
+    a.splits = dkv;
     if (total_k) attention_dkv_kernel<T, DP, FAST, NW><<<key_tiles * Hkv * a.splits, 64 * NW, 0, st>>>(a);
   });
   if (total_k && a.splits > 1) attention_dkv_join_kernel<T><<<ew_grid(total_k * Hkv * D), 256, 0, st>>>(a);

@@ -7,19 +7,15 @@ int unet_dot_attention_workspace_bytes(int num_seqs, int64_t total_q, int64_t to
                                        int head_dim, size_t *bytes_host) {
   UNET_REQUIRE(bytes_host, "dot_attention_workspace_bytes: NULL result");
   TRY(check_shape("dot_attention_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  const int f32 = make_plan<float>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim, false).splits;
-  const int bf16 = make_plan<bf16_t>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim, false).splits;
-  const int splits = f32 > bf16 ? f32 : bf16;  // the larger of the two types' plans; a causal mask does not change them
-  *bytes_host = forward_bytes(total_q, heads_q, head_dim, splits);
+  *bytes_host = forward_bytes(most_query_rows(total_q, total_k, heads_q, MOST_SHARES), head_dim);
   return UNET_OK;
 }
 int unet_dot_attention_backward_workspace_bytes(int num_seqs, int64_t total_q, int64_t total_k, int heads_q,
                                                 int heads_kv, int head_dim, size_t *bytes_host) {
   UNET_REQUIRE(bytes_host, "dot_attention_backward_workspace_bytes: NULL result");
   TRY(check_shape("dot_attention_backward_workspace_bytes", num_seqs, total_q, total_k, heads_q, heads_kv, head_dim));
-  const size_t f32 = partial_bytes<float>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim);
-  const size_t bf16 = partial_bytes<bf16_t>(num_seqs, total_q, total_k, heads_q, heads_kv, head_dim);
-  *bytes_host = rows_bytes(total_q, heads_q) + (f32 > bf16 ? f32 : bf16);
+  *bytes_host = rows_bytes(total_q, heads_q) + backward_bytes(most_query_rows(total_q, total_k, heads_q, MOST_DQ_SHARES),
+                                                             most_key_rows(total_q, total_k, heads_q, heads_kv), head_dim);
   return UNET_OK;
 }
 
