@@ -365,9 +365,10 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  * does not reach it, whatever it holds (NaN and infinities included).  (An infinity that it does see counts as NaN in
  * the fp32 form, whose products take operands apart.)  Rows of out and lse in front of the first or
  * behind the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
- * accumulators are fp32 (weights are up to 2^8 before the division at the end, so values larger than the largest number
- * over 256 * keys may overflow); the bf16 form rounds the softmax weights to bf16 for their product with V.  Equal calls
- * give equal bits.  out must not overlap q, k or v.  total_q * heads_q and total_k * heads_kv may be up to about 2^29.
+ * accumulators are fp32; no finite value of v overflows on the way (one within 2^-16 of the largest number may be rounded over
+ * it at the end), and values below about 2^-126 * 2^8 * keys lose bits.  The bf16 form rounds the softmax weights to bf16 for
+ * their product with V.  Equal calls give equal bits.  out must not overlap q, k or v.  total_q * heads_q and
+ * total_k * heads_kv may be up to about 2^29.
  * heads_q * head_dim is less than 2^31.
  * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
  * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the

@@ -47,3 +47,19 @@ def test_nothing_is_written_behind_a_workspace(name, lens_q, lens_k, hq, hk, d):
     c.backward()
     c.verify()
     assert (behind == 255).all() and (behind_b == 255).all()
+
+
+# ---- the largest numbers --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("lens_q,lens_k,hq,hk,d,pad", [([70, 9], [90, 9], 4, 2, 64, 0), ([300], [513], 66, 66, 100, 1), ([3, 1], [5000, 1], 8, 1, 128, 0),
+                                                       ([130], [1500], 2, 1, 40, 0)])
+def test_values_near_the_largest_number(name, lens_q, lens_k, hq, hk, d, pad):
+    """A weighted mean is never larger than its terms, so the result is finite; the gradients of small dout are, too."""
+    c = Call(name, lens_q, lens_k, hq, hk, d, True, pad)
+    c.v *= 0.98 * torch.finfo(c.dtype).max / float(c.v.abs().max())  # half a step of bf16 on top: 0.984
+    c.v[::3] = 0.98 * torch.finfo(c.dtype).max
+    c.dout *= 2.0 ** -100
+    c.forward()
+    c.backward()
+    c.verify()

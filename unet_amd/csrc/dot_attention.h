@@ -44,8 +44,9 @@ constexpr int COLS = 32;            // columns (queries or keys) per wavefront
 constexpr int WAVES = 4;
 constexpr int BM = COLS * WAVES;    // columns per workgroup
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-// The running maximum follows a score only when that exceeds it by this much (in powers of two): until then the
-// weights are at most 2^8 and nothing is rescaled.  The final division makes up for it exactly.
+// The running maximum follows a score only when that exceeds it by this much (in powers of two): until then nothing is
+// rescaled.  The reference that the weights are taken from lies LAZY + ceil(log2 keys) above it, so that a sequence's weights
+// add up to 1 at most and no finite value overflows on the way.  The final division makes up for both exactly.
 constexpr float LAZY = 8.f;
 constexpr unsigned NOWHERE = 0x80000000u;  // a byte offset behind the end of every buffer (a tile spans less than 2 GiB)
 
@@ -663,7 +664,9 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 |
   f32x16 acc[DB];
 #pragma unroll
   for (int db = 0; db < DB; ++db) acc[db] = zero16();
-  float m = -INFINITY, l = 0.f;  // of the scores times scale2 (base 2); l over this lane's rows only
+  // m: the reference, at most `lift` above the largest score times scale2 (base 2); l: over this lane's rows only
+  float m = -INFINITY, l = 0.f;
+  const float lift = LAZY + (float)(32 - __builtin_clz(max(r.s.nk, 1)));
 
   int first = 0, n = (span.kend + ROWS - 1) / ROWS;  // key tiles
   if (a.splits > 1) {
@@ -708,7 +711,7 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 |
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[u][i]);
-    top *= a.scale2;
+    top = top * a.scale2 + lift;
     if (__any(top > m + LAZY)) {
       const float m_new = fmaxf(m, fmaxf(top, __shfl_xor(top, 32, 64)));
       const float f = m_new == m ? 1.f : __builtin_amdgcn_exp2f(m - m_new);
