@@ -5,6 +5,7 @@ import ctypes
 import pytest
 import torch
 
+import seq_ref
 from gpu_util import DEV
 from test_dot_attention_gpu import Call
 from unet_amd import capi
@@ -63,3 +64,48 @@ def test_values_near_the_largest_number(name, lens_q, lens_k, hq, hk, d, pad):
     c.forward()
     c.backward()
     c.verify()
+
+
+# ---- infinities that a query sees -----------------------------------------------------------------------
+# A score of -inf is a weight of 0, as in the definition.
+
+VISIBLE = [(4, 20), (60, 30), (130, 32), (4, 60), (60, 64), (130, 50), (4, 96), (66, 88), (4, 128), (66, 120)]  # heads, dim: each way to share the queries
+LENS_Q, LENS_K = [333, 40], [340, 33]
+
+
+def visible(name, heads, dim, causal, pad):
+    return Call(name, LENS_Q, LENS_K, heads, heads // 2, dim, causal, pad=pad, behind=1)
+
+
+def seeing(c, key):
+    """The queries that see a key (a truth value each), both numbered over all sequences."""
+    s = 0 if key < c.lens_k[0] else 1
+    query = torch.arange(c.nq)
+    mine = (query >= c.lens_q[0]) == bool(s)
+    at, nq, nk = (query - s * c.lens_q[0], c.lens_q[s], c.lens_k[s])
+    return mine & (at + nk - nq >= key - s * c.lens_k[0]) if c.causal else mine
+
+
+def check(c, val, bnd, names):
+    for n in names:
+        seq_ref.check(getattr(c, n)[:val[n].shape[0]], val[n], bnd[n], n)
+
+
+@pytest.mark.parametrize("name", ["bf16"])
+@pytest.mark.parametrize("causal,pad", [(False, 0), (True, 3)])
+@pytest.mark.parametrize("heads,dim", VISIBLE)
+def test_keys_with_infinite_scores(name, causal, pad, heads, dim):
+    """Element 3 of the queries is positive and of some keys -inf: those keys have weight 0 with every query, so only grad_q's
+    element 3, a product of 0 and the infinity, is NaN.  The definition has -1e30 in their place: weight 0 as well."""
+    c = visible(name, heads, dim, causal, pad)
+    bad = [7, 50, 51, 200, 345]
+    c.q[:, 3::dim] = c.q[:, 3::dim].abs() + 0.125
+    for key in bad:
+        c.k[key, 3::dim] = -1e30
+    val, bnd = c.exact()
+    for key in bad:
+        c.k[key, 3::dim] = -float("inf")
+        val["dq"][seeing(c, key), 3::dim] = float("nan")
+    c.forward()
+    c.backward()
+    check(c, val, bnd, ("out", "lse", "dq", "dk", "dv"))

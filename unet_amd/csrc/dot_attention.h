@@ -1102,12 +1102,13 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
         }
       }
       const bool edge = rb < wave_all;
-      if (edge) {
-        const int rel = lim - rb - 4 * h;
+      if (edge || rb + 32 > nrows) {  // (a row that does not exist is zeros, but with an infinite key they make NaN)
+        const int rel = lim - rb - 4 * h, end = nrows - rb - 4 * h;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          p[i] = 8 * (i / 4) + i % 4 >= rel ? p[i] : 0.f;
-          ds[i] = 8 * (i / 4) + i % 4 >= rel ? ds[i] : 0.f;
+          const bool seen = 8 * (i / 4) + i % 4 >= rel && 8 * (i / 4) + i % 4 < end;
+          p[i] = seen ? p[i] : 0.f;
+          ds[i] = seen ? ds[i] : 0.f;
         }
       }
       auto sees = [&](int i) __attribute__((always_inline)) { return rb + i >= lim; };
