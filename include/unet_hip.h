@@ -362,8 +362,9 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  *   causal != 0: query i of a sequence sees the keys j <= i + (keys - queries), i.e. the last query sees all.
  *   lse [total_q][heads_q] (fp32, may be NULL: inference) = log sum_j exp(scale * q.k_j), for the backward.
  * A query that sees no key gets out = 0 and lse = -inf, and adds nothing to any gradient.  What a query does not see
- * does not reach it, whatever it holds (NaN and infinities included).  (An infinity that it does see counts as NaN in
- * the fp32 form, whose products take operands apart.)  Rows of out and lse in front of the first or
+ * does not reach it, whatever it holds (NaN and infinities included).  What it does see acts as in the formula: a score of
+ * -inf is a weight of 0, an infinite value an infinite output (fp32 takes several times as long where there are any, since
+ * its products take operands apart).  Rows of out and lse in front of the first or
  * behind the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
  * accumulators are fp32; no finite value of v overflows on the way (one within 2^-16 of the largest number may be rounded over
  * it at the end), and values below about 2^-126 * 2^8 * keys lose bits.  The bf16 form rounds the softmax weights to bf16 for

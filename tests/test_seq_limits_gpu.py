@@ -67,9 +67,9 @@ def test_values_near_the_largest_number(name, lens_q, lens_k, hq, hk, d, pad):
 
 
 # ---- infinities that a query sees -----------------------------------------------------------------------
-# A score of -inf is a weight of 0, as in the definition.
+# Both types treat them as the definition does: a score of -inf is a weight of 0, an infinite value makes an infinite output.
 
-VISIBLE = [(4, 20), (60, 30), (130, 32), (4, 60), (60, 64), (130, 50), (4, 96), (66, 88), (4, 128), (66, 120)]  # heads, dim: each way to share the queries
+VISIBLE = [(4, 20), (60, 30), (130, 32), (4, 60), (60, 64), (130, 50), (4, 96), (66, 88), (4, 128), (66, 120)]  # heads, dim: each kernel of fp32
 LENS_Q, LENS_K = [333, 40], [340, 33]
 
 
@@ -91,7 +91,7 @@ def check(c, val, bnd, names):
         seq_ref.check(getattr(c, n)[:val[n].shape[0]], val[n], bnd[n], n)
 
 
-@pytest.mark.parametrize("name", ["bf16"])
+@pytest.mark.parametrize("name", ["f32", "bf16"])
 @pytest.mark.parametrize("causal,pad", [(False, 0), (True, 3)])
 @pytest.mark.parametrize("heads,dim", VISIBLE)
 def test_keys_with_infinite_scores(name, causal, pad, heads, dim):
@@ -109,3 +109,66 @@ def test_keys_with_infinite_scores(name, causal, pad, heads, dim):
     c.forward()
     c.backward()
     check(c, val, bnd, ("out", "lse", "dq", "dk", "dv"))
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("causal,pad", [(False, 0), (True, 3)])
+@pytest.mark.parametrize("heads,dim", VISIBLE)
+def test_infinite_values_and_gradients(name, causal, pad, heads, dim):
+    """An infinite element of V makes that element of the outputs infinite, one of grad_out that element of grad_v."""
+    c = visible(name, heads, dim, causal, pad)
+    clean, bnd = c.exact()
+    val = {n: t.clone() for n, t in clean.items()}
+    for key, e, inf in ((40, 1, float("inf")), (339, 1, float("inf")), (372, 4, float("inf")), (3, 5, -float("inf"))):
+        c.v[key, e::dim] = inf
+        val["out"][seeing(c, key), e::dim] = inf
+    c.forward()
+    check(c, val, bnd, ("out", "lse"))
+    c = visible(name, heads, dim, causal, pad)
+    val = {n: t.clone() for n, t in clean.items()}
+    for query in (0, 331, 372):
+        c.dout[query, 2::dim] = float("inf")
+        val["dv"][torch.stack([seeing(c, key)[query] for key in range(c.nk)]), 2::dim] = float("inf")
+    c.forward()
+    c.backward()
+    check(c, val, bnd, ("out", "lse", "dv"))
+
+
+@pytest.mark.parametrize("heads,dim", VISIBLE)
+def test_nan_whose_upper_half_is_an_infinity(heads, dim):
+    c = visible("f32", heads, dim, True, 0)
+    val, bnd = c.exact()
+    for t, key in ((c.k, 60), (c.v, 345)):
+        t[key] = torch.full_like(t[key], 0).view(torch.int32).fill_(0x7F800001).view(torch.float32)
+        val["out"][seeing(c, key)] = float("nan")
+    val["lse"][seeing(c, 60)] = float("nan")
+    c.forward()
+    assert (c.k[60].view(torch.int32) == 0x7F800001).all()
+    check(c, val, bnd, ("out", "lse"))
+
+
+@pytest.mark.parametrize("heads,dim", VISIBLE)
+def test_scores_beyond_the_largest_number(heads, dim):
+    """Products of -1e50 and more in one element: -inf in fp32, so weight 0, whatever their parts are."""
+    c = visible("f32", heads, dim, True, 0)
+    g = torch.Generator().manual_seed(1)
+    c.q[:, 3::dim] = (torch.rand(c.tq, heads, generator=g) * 1e25 + 1e25).to(DEV)
+    c.k[:, 3::dim] = 0.0
+    c.k[[5, 100, 250], 3::dim] = -(torch.rand(3, c.hk, generator=g) * 1e25 + 1e25).to(DEV)
+    c.forward()
+    c.backward()
+    c.verify()
+
+
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+def test_infinities_in_split_sums(name):
+    c = Call(name, [2, 1], [4000, 3500], 8, 2, 64, False)
+    c.q[:, 3::64] = c.q[:, 3::64].abs() + 0.125
+    bad = [0, 1, 3100, 5000]
+    c.k[bad, 3::64] = -1e30
+    val, bnd = c.exact()
+    c.k[bad, 3::64] = -float("inf")
+    c.v[[10, 6000], 1::64] = float("inf")
+    val["out"][:, 1::64] = float("inf")
+    c.forward()
+    check(c, val, bnd, ("out", "lse"))

@@ -54,7 +54,7 @@ constexpr unsigned NOWHERE = 0x80000000u;  // a byte offset behind the end of ev
 // over (less than 2^-7 of it) rounded to bf16, and the rest, which has 8 bits and is at most 2^-15 of it.  Six products
 // of parts make the product of two such numbers up to 2^-21 of it: what is left out is the middle part of one times the
 // last part of the other, twice, with random signs; the matrix cores do the six in 3/8 of the time of one fp32 product.
-// (The upper part is cut off, not rounded: no finite number becomes infinite.  An infinity leaves NaN over.)  3525
+// (The upper part is cut off, not rounded: no finite number becomes infinite.  An infinity leaves NaN over, see below.)  3525
 // tokens in 4 sequences, 8 heads of 64, forward and backward: 219 us and an error of 5.3e-7 of the result; with fp32
 // matrix instructions 366 us and 7.0e-7.
 struct Parts {
@@ -115,6 +115,52 @@ __device__ __forceinline__ f32x16 mma(const Parts &a, const Parts &b, f32x16 c) 
   c = mma(a.p[0], b.p[1], c);
   return mma(a.p[0], b.p[0], c);
 }
+// ---- fp32 with infinities --------------------------------------------------------------------------------
+// An infinity, or a product that overflows, makes NaN of the six products, whatever it should have become: the parts that it
+// leaves over are NaN, or infinite with the other sign.  So a workgroup of the fp32 kernels that ends with a sum that is not
+// finite begins again with products that take infinities apart, two to three times as slow and slower yet at the edge of a
+// mask: the first parts alone tell whether a sum is infinite or NaN, and which; where it is neither, it is the sum of the
+// six products without the elements that are not finite (a finite sum has none).  Calls with finite results pay for the check
+// and for larger kernels: 3525 tokens, 8 heads of 64, forward and backward 232 -> 234 us, one image of 256 48 -> 49, 4
+// queries over 12000 keys, 16/4 heads of 128, 37 -> 39.
+__device__ __forceinline__ f32x8 quiet(f32x8 x) {  // a signaling NaN's upper half alone could be an infinity
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = __builtin_canonicalizef(x[j]);
+  return x;
+}
+__device__ __forceinline__ bf16x8 quiet(const bf16x8 &x) { return x; }
+__device__ __forceinline__ Parts finite_part(Parts f) {
+  uint32_t w[3][4];
+  __builtin_memcpy(w, f.p, sizeof(w));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    asm volatile("" : "+v"(w[0][i]));  // not to be taken out of a loop: kept beside the operand itself it would fill the registers
+    const uint32_t keep = ((w[0][i] & 0x7f80u) != 0x7f80u ? 0xffffu : 0u) | ((w[0][i] & 0x7f800000u) != 0x7f800000u ? 0xffff0000u : 0u);
+#pragma unroll
+    for (int k = 0; k < 3; ++k) w[k][i] &= keep;
+  }
+  __builtin_memcpy(f.p, w, sizeof(w));
+  return f;
+}
+// A sum of products: `first` of the first parts, `rest` of all.
+// (A template so that the bf16 kernels, which have no use for it, leave it alone.)
+template <bool CAREFUL>
+struct Sum {
+  f32x16 first, rest;
+};
+template <bool CAREFUL>
+__device__ __forceinline__ void mma(const Parts &a, const Parts &b, Sum<CAREFUL> &c) {
+  c.first = mma(a.p[0], b.p[0], c.first);
+  c.rest = mma(finite_part(a), finite_part(b), c.rest);
+  __builtin_amdgcn_sched_barrier(0);  // one after the other: the operands of several would not fit the registers
+}
+template <bool CAREFUL>
+__device__ __forceinline__ f32x16 total(const Sum<CAREFUL> &c) {
+  f32x16 r;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = fabsf(c.first[i]) < INFINITY ? c.rest[i] : c.first[i];
+  return r;
+}
 __device__ __forceinline__ f32x16 zero16() {
   f32x16 z;
 #pragma unroll
@@ -123,7 +169,7 @@ __device__ __forceinline__ f32x16 zero16() {
 }
 // Weights of 16 rows as a B operand; bf16 rounds them.  Each is off by at most 2^-8 of itself, so the sum by no more than
 // rounding the output once costs, and by less where many keys have a part in it.
-template <typename T>
+template <typename T, bool CAREFUL = false>
 __device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
   Raw<T> f;
 #pragma unroll
@@ -135,6 +181,7 @@ __device__ __forceinline__ Frag<T> pack8(const f32x16 &w, int t) {
       f[j] = w[8 * t + j], f[j + 1] = w[8 * t + j + 1];
     }
   }
+  if constexpr (CAREFUL) f = quiet(f);
   return as_frag(f);
 }
 
@@ -315,13 +362,14 @@ struct Tile {
       for (int i = 0; i < PER; ++i)
         if (r0 + i * (NT / NC) >= n) to.c[i] = Raw<T>{};
   }
+  template <bool CAREFUL = false>
   static __device__ __forceinline__ void put(const Chunks &from, unsigned char *tile) {
     const int chunk = threadIdx.x % NC;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int r = threadIdx.x / NC + i * (NT / NC);
       unsigned char *const at = tile + (r >> 4) * R16 + (r & 15) * RB + (chunk ^ key(r)) * 16;
-      const Frag<T> f = as_frag(from.c[i]);
+      const Frag<T> f = as_frag(CAREFUL ? quiet(from.c[i]) : from.c[i]);
 #pragma unroll
       for (int k = 0; k < PARTS<T>; ++k) *reinterpret_cast<bf16x8 *>(at + k * PART) = reinterpret_cast<const bf16x8 *>(&f)[k];
     }
@@ -390,6 +438,30 @@ struct Tile {
       if constexpr (TWICE) acc[db] = mma(x, c1, acc[db]);
     }
   }
+  // The same with products that take infinities apart; at the edge of a mask row by row.
+  template <typename Sees>
+  static __device__ __forceinline__ void add_careful(f32x16 (&acc)[DP / 32], const unsigned char *rows32, const Lane &o, const f32x16 &w,
+                                                     bool edge, Sees sees) {
+    const Parts b0 = pack8<T, true>(w, 0), b1 = pack8<T, true>(w, 1);
+    const int h = (threadIdx.x & 63) >> 5;
+#pragma unroll 1
+    for (int k = 0; k < 32; k += edge ? 1 : 16) {
+      const int j = ((k >> 3) & 1) * 4 + (k & 3);
+      const bool mine = ((k >> 2) & 1) == h, seen = !edge || sees(k);
+      Parts b = choose(k < 16, b0, b1);
+      if (edge) b = alone(mine, j, b);
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) {
+        Parts f = down(rows32 + (k >> 4) * R16, o, db);
+        if (edge) f = alone(mine, j, f);
+        Sum<true> c = {zero16(), zero16()};
+        mma(f, b, c);
+        const f32x16 r = total(c);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[db][i] += seen ? r[i] : 0.f;
+      }
+    }
+  }
   static __device__ __forceinline__ void clear(unsigned char *zeros) {
     for (int i = threadIdx.x * 16; i < ZEROS; i += NT * 16) *reinterpret_cast<u32x4 *>(zeros + i) = u32x4{0, 0, 0, 0};
   }
@@ -416,7 +488,7 @@ __device__ __forceinline__ Raw<T> load_eight(const T *p, int e, int D) {
 }
 template <typename T, bool WHOLE>
 __device__ __forceinline__ Frag<T> load_frag(const T *p, int e, int D) {
-  return as_frag(load_eight<T, WHOLE>(p, e, D));
+  return as_frag(quiet(load_eight<T, WHOLE>(p, e, D)));
 }
 // Four consecutive results p[0..4), as many as n allows.
 template <typename T>
@@ -489,8 +561,10 @@ constexpr int tile_rows() {
 //         no other vector memory instructions: a wait of the compiler's for one of those would be for all direct loads
 //         as well.
 //   else: fetch(t) loads tile t to registers, put(buffer) writes them to a buffer.
-template <bool FAST, int NB, int PER, typename Move, typename Fetch, typename Put, typename Step>
-__device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, Step step) {
+// `how` (a std::bool_constant) is handed on to put and step in front of their arguments.  True (see Sum): each tile is loaded
+// when its turn comes, so that its registers are free for the step.
+template <bool FAST, int NB, int PER, typename Move, typename Fetch, typename Put, typename Step, typename How>
+__device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, Step step, How how) {
   static_assert(NB == 2 || NB == (FAST ? 3 : 1), "two buffers, or three for direct loads, or one for loads by registers");
   if (n <= 0) return;
   if constexpr (FAST) {
@@ -503,31 +577,40 @@ __device__ __forceinline__ void stream(int n, Move move, Fetch fetch, Put put, S
       else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
       const int free = buf == 0 ? NB - 1 : buf - 1;
       if (t + NB - 1 < n) move(t + NB - 1, free);
-      step(t, buf);
+      step(how, t, buf);
       buf = buf == NB - 1 ? 0 : buf + 1;
+    }
+  } else if constexpr (How::value) {
+#pragma unroll 1
+    for (int t = 0; t < n; ++t) {
+      fetch(t);
+      __syncthreads();
+      put(how, 0);
+      __syncthreads();
+      step(how, t, 0);
     }
   } else if constexpr (NB == 1) {
     fetch(0);
 #pragma unroll 1
     for (int t = 0; t < n; ++t) {
       if (t) __syncthreads();
-      put(0);
+      put(how, 0);
       __syncthreads();
       fetch(t + 1);
-      step(t, 0);
+      step(how, t, 0);
     }
   } else {
     fetch(0);
-    put(0);
+    put(how, 0);
     fetch(1);
 #pragma unroll 1
     for (int t = 0; t < n; ++t) {
       __syncthreads();
       if (t + 1 < n) {
-        put((t + 1) & 1);
+        put(how, (t + 1) & 1);
         fetch(t + 2);
       }
-      step(t, t & 1);
+      step(how, t, t & 1);
     }
   }
 }
@@ -575,6 +658,27 @@ __device__ __forceinline__ void direct_load_dword(const float *base, unsigned at
                :
                : "s"(__builtin_amdgcn_readfirstlane(lds)), "v"(at), "s"(rsrc));
 }
+// 0, or NaN if a sum is not finite.
+template <int DB>
+__device__ __forceinline__ float finite_check(const f32x16 (&acc)[DB]) {
+  float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) z[i & 3] += acc[db][i] * 0.f;
+  return (z[0] + z[1]) + (z[2] + z[3]);
+}
+// Whether that is NaN in any thread of the workgroup.  Behind its barrier no tile is read any more.  `flags`: NW words of LDS
+// for this alone, once a kernel.
+template <int NW>
+__device__ __forceinline__ bool anywhere(float z, int *flags) {
+  flags[threadIdx.x >> 6] = __any(z != 0.f) ? 1 : 0;
+  __syncthreads();
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) any |= flags[w];
+  return __builtin_amdgcn_readfirstlane(any);
+}
 // Where a workgroup's LDS array begins, as the direct loads want it.
 __device__ __forceinline__ unsigned lds_address(unsigned char *lds) {
   return (unsigned)(uintptr_t)(__attribute__((address_space(3))) unsigned char *)lds;
@@ -608,9 +712,10 @@ struct KeyTiles {
     TL::fetch(ck, first, end, D, [&](int j) __attribute__((always_inline)) { return k + j * k_ld; });
     TL::fetch(cv, first, end, D, [&](int j) __attribute__((always_inline)) { return v + j * v_ld; });
   }
+  template <bool CAREFUL>
   __device__ __forceinline__ void put(unsigned char *lds_k, unsigned char *lds_v) {
-    TL::put(ck, lds_k);
-    TL::put(cv, lds_v);
+    TL::template put<CAREFUL>(ck, lds_k);
+    TL::template put<CAREFUL>(cv, lds_v);
   }
 };
 
@@ -644,6 +749,7 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 |
   typedef Tile<T, DP, ROWS, NW> TL;
   constexpr int NB = NW == 8 ? (FAST ? 3 : 2) : buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 64 * NW * (DB * 16 + 2) * 4;
   __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
+  __shared__ int flags[sizeof(T) == 4 ? NW : 1];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits, t0 = bs / a.splits;
@@ -683,21 +789,32 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 |
   auto fetch = [&](int t) __attribute__((always_inline)) {
     if (!FAST) keys.fetch((first + t) * ROWS, end);
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-    if (!FAST) keys.put(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
+  auto put = [&](auto careful, int buf) __attribute__((always_inline)) {
+    if (!FAST) keys.template put<decltype(careful)::value>(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
   };
-  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+  auto step = [&](auto careful, int t, int buf) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
     const int key0 = (first + t) * ROWS + wk * 32;
     if (key0 > span.wave_some) return;
     const unsigned char *const ldsK = lds + buf * STAGE + wk * 2 * TL::R16, *const ldsV = ldsK + TL::BYTES;
     const bool edge = key0 + NU * 32 - 1 > span.wave_all;
     f32x16 s[NU];
+    if constexpr (CAREFUL) {
 #pragma unroll
-    for (int u = 0; u < NU; ++u) s[u] = zero16();
+      for (int u = 0; u < NU; ++u) {
+        Sum<CAREFUL> c = {zero16(), zero16()};
 #pragma unroll
-    for (int x = 0; x < DP / 16; ++x)  // the pieces in turn: no product waits for the one in front of it
+        for (int x = 0; x < DP / 16; ++x) mma(TL::along(ldsK + u * 2 * TL::R16, lo, x), q[x], c);
+        s[u] = total(c);
+      }
+    } else {
 #pragma unroll
-      for (int u = 0; u < NU; ++u) s[u] = mma(TL::along(ldsK + u * 2 * TL::R16, lo, x), q[x], s[u]);
+      for (int u = 0; u < NU; ++u) s[u] = zero16();
+#pragma unroll
+      for (int x = 0; x < DP / 16; ++x)  // the pieces in turn: no product waits for the one in front of it
+#pragma unroll
+        for (int u = 0; u < NU; ++u) s[u] = mma(TL::along(ldsK + u * 2 * TL::R16, lo, x), q[x], s[u]);
+    }
     if (edge) {
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
@@ -735,11 +852,19 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 |
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       const int kb = key0 + u * 32;
-      TL::add(acc, ldsV + u * 2 * TL::R16, zeros, lo, s[u], edge && kb + 31 > span.wave_all,
-              [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
+      auto sees = [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; };
+      if constexpr (CAREFUL) TL::add_careful(acc, ldsV + u * 2 * TL::R16, lo, s[u], edge, sees);
+      else TL::add(acc, ldsV + u * 2 * TL::R16, zeros, lo, s[u], edge && kb + 31 > span.wave_all, sees);
     }
   };
-  stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step);
+  stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step, std::false_type());
+  if constexpr (sizeof(T) == 4)
+    if (anywhere<NW>(l * 0.f + finite_check(acc), flags)) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) acc[db] = zero16();
+      m = -INFINITY, l = 0.f;
+      stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step, std::true_type());
+    }
   l += __shfl_xor(l, 32, 64);
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
@@ -822,6 +947,7 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   typedef Tile<T, DP, ROWS> TL;
   constexpr int NB = buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 256 * DB * 16 * 4;
   __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
+  __shared__ int flags[sizeof(T) == 4 ? WAVES : 1];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
   const int lane = threadIdx.x & 63, h = lane >> 5, wave = wave_index(), wq = wave % WQ, wk = wave / WQ;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits, t0 = bs / a.splits;
@@ -843,13 +969,14 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
     for (int t = 0; t < DP / 16; ++t) {
       const int e = 16 * t + 8 * h;
       q[t] = load_frag<T, FAST>(p, e, a.D);
-      const Raw<T> d = load_eight<T, FAST>(pd, e, a.D), o = load_eight<T, FAST>(po, e, a.D);
+      const Raw<T> d = quiet(load_eight<T, FAST>(pd, e, a.D)), o = load_eight<T, FAST>(po, e, a.D);
       dout[t] = as_frag(d);
 #pragma unroll
       for (int j = 0; j < 8; ++j) delta += (float)d[j] * (float)o[j];
     }
     delta += __shfl_xor(delta, 32, 64);
   }
+  const float stored_delta = delta;
   const i64 at = (i64)(r.s.q0 + r.query) * a.Hq + r.head;
   const float lse2 = a.lse[at] * LOG2E;  // (a row that does not exist repeats the last one and is not stored)
 
@@ -871,11 +998,12 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
   auto fetch = [&](int t) __attribute__((always_inline)) {
     if (!FAST) keys.fetch((first + t) * ROWS, end);
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-    if (!FAST) keys.put(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
+  auto put = [&](auto careful, int buf) __attribute__((always_inline)) {
+    if (!FAST) keys.template put<decltype(careful)::value>(lds + buf * STAGE, lds + buf * STAGE + TL::BYTES);
   };
-  constexpr int UNROLL = sizeof(T) == 2 ? 2 : 1;
-  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+  auto step = [&](auto careful, int t, int buf) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    constexpr int UNROLL = sizeof(T) == 2 ? 2 : 1;
     const unsigned char *const ldsK = lds + buf * STAGE + wk * 2 * TL::R16, *const ldsV = ldsK + TL::BYTES;
 #pragma unroll UNROLL  // two pieces share their addresses
     for (int u = 0; u < NU; ++u) {
@@ -883,10 +1011,21 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
       if (kb > span.wave_some) break;
       const unsigned char *const k32 = ldsK + u * 2 * TL::R16, *const v32 = ldsV + u * 2 * TL::R16;
       f32x16 s = zero16(), dp = zero16();
+      if constexpr (CAREFUL) {
+        Sum<CAREFUL> c = {s, s};
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x) {
-        s = mma(TL::along(k32, lo, x), q[x], s);
-        dp = mma(TL::along(v32, lo, x), dout[x], dp);
+        for (int x = 0; x < DP / 16; ++x) mma(TL::along(k32, lo, x), q[x], c);
+        s = total(c);
+        c = {dp, dp};
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) mma(TL::along(v32, lo, x), dout[x], c);
+        dp = total(c);
+      } else {
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {
+          s = mma(TL::along(k32, lo, x), q[x], s);
+          dp = mma(TL::along(v32, lo, x), dout[x], dp);
+        }
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] * a.scale2 - lse2);
@@ -913,11 +1052,19 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
       // dS of a query adds up to zero, so its product with K loses the part that the keys have in common, but the
       // roundings of dS do not: with few elements (that part is then large beside the rest) they are kept out.  (16 x 256
       // tokens, 16 heads of 64: 21.2 us instead of 18.9, and an error of 1.0 instead of 1.45 output roundings.)
-      TL::template add<sizeof(T) == 2 && DP <= 64>(acc, k32, zeros, lo, s, edge,
-                                                   [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; });
+      auto sees = [&](int k) __attribute__((always_inline)) { return kb + k <= r.lim; };
+      if constexpr (CAREFUL) TL::add_careful(acc, k32, lo, s, edge, sees);
+      else TL::template add<sizeof(T) == 2 && DP <= 64>(acc, k32, zeros, lo, s, edge, sees);
     }
   };
-  stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step);
+  stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step, std::false_type());
+  if constexpr (sizeof(T) == 4)
+    if (anywhere<WAVES>(finite_check(acc), flags)) {
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) acc[db] = zero16();
+      delta = stored_delta;
+      stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step, std::true_type());
+    }
   int db0 = 0, db1 = DB;  // the blocks of 32 elements that this wavefront writes
   if constexpr (WK > 1) {
     __syncthreads();
@@ -973,6 +1120,7 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
   constexpr int KT = DP / 16, K_REG = ALL_REG || sizeof(T) == 4 ? KT : KT - 2, V_REG = ALL_REG ? KT : 0;
   constexpr int OWN = (2 * KT - K_REG - V_REG) * 64 * (int)sizeof(Frag<T>);
   __shared__ __align__(16) unsigned char lds[NB * STAGE + TL::ZEROS + NW * OWN];
+  __shared__ int flags[sizeof(T) == 4 ? NW : 1];
   unsigned char *const zeros = lds + NB * STAGE;
   const int kvh = blockIdx.x % a.Hkv, bs = blockIdx.x / a.Hkv, split = bs % a.splits;
   int key0;
@@ -1058,18 +1206,19 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
       fd = a.rows[at + (i64)a.total_q * a.Hq];
     }
   };
-  auto put = [&](int buf) __attribute__((always_inline)) {
+  auto put = [&](auto careful, int buf) __attribute__((always_inline)) {
     unsigned char *const st = lds + buf * STAGE;
-    TL::put(cq, st);
-    TL::put(cd, st + TL::BYTES);
+    TL::template put<decltype(careful)::value>(cq, st);
+    TL::template put<decltype(careful)::value>(cd, st + TL::BYTES);
     if (threadIdx.x < ROWS) {
       float *const f = reinterpret_cast<float *>(st + 2 * TL::BYTES) + threadIdx.x;
       f[0] = fl;
       f[64] = fd;
     }
   };
-  constexpr int UNROLL = sizeof(T) == 2 && DP < 128 ? 2 : 1;
-  auto step = [&](int t, int buf) __attribute__((always_inline)) {
+  auto step = [&](auto careful, int t, int buf) __attribute__((always_inline)) {
+    constexpr bool CAREFUL = decltype(careful)::value;
+    constexpr int UNROLL = sizeof(T) == 2 && DP < 128 ? 2 : 1;
     const unsigned char *const ldsQ = lds + buf * STAGE, *const ldsD = ldsQ + TL::BYTES;
     const float *const ldsL = reinterpret_cast<const float *>(ldsD + TL::BYTES), *const ldsDelta = ldsL + 64;
 #pragma unroll UNROLL  // as above; at 128 elements every register counts
@@ -1086,12 +1235,23 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
 #pragma unroll
         for (int i = 0; i < 4; ++i) ds[4 * b + i] = d[i];
       }
+      auto key_part = [&](int x) __attribute__((always_inline)) { return x < K_REG ? kr[x < K_REG ? x : 0] : own[64 * (KT - V_REG + x - K_REG)]; };
+      auto value_part = [&](int x) __attribute__((always_inline)) { return x < V_REG ? vr[x < V_REG ? x : 0] : own[64 * (x - V_REG)]; };
+      if constexpr (CAREFUL) {
+        Sum<CAREFUL> c = {p, p};
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x)
-        p = mma(TL::along(q32, lo, x), x < K_REG ? kr[x < K_REG ? x : 0] : own[64 * (KT - V_REG + x - K_REG)], p);
+        for (int x = 0; x < DP / 16; ++x) mma(TL::along(q32, lo, x), key_part(x), c);
+        p = total(c);
+        c = {zero16(), zero16()};
 #pragma unroll
-      for (int x = 0; x < DP / 16; ++x)
-        ds = mma(TL::along(d32, lo, x), x < V_REG ? vr[x < V_REG ? x : 0] : own[64 * (x - V_REG)], ds);
+        for (int x = 0; x < DP / 16; ++x) mma(TL::along(d32, lo, x), value_part(x), c);
+        ds += total(c);
+      } else {
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) p = mma(TL::along(q32, lo, x), key_part(x), p);
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) ds = mma(TL::along(d32, lo, x), value_part(x), ds);
+      }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         const f32x4 lse2 = *reinterpret_cast<const f32x4 *>(ldsL + u * 32 + 8 * b + 4 * h);
@@ -1112,11 +1272,23 @@ __global__ __launch_bounds__(64 * NW, (sizeof(T) == 2 || DP <= 64 ? 2 : 1)) void
         }
       }
       auto sees = [&](int i) __attribute__((always_inline)) { return rb + i >= lim; };
-      TL::add(dv, d32, zeros, lo, p, edge, sees);
-      TL::add(dk, q32, zeros, lo, ds, edge, sees);
+      if constexpr (CAREFUL) {
+        TL::add_careful(dv, d32, lo, p, edge, sees);
+        TL::add_careful(dk, q32, lo, ds, edge, sees);
+      } else {
+        TL::add(dv, d32, zeros, lo, p, edge, sees);
+        TL::add(dk, q32, zeros, lo, ds, edge, sees);
+      }
     }
   };
-  stream<FAST, NB, 2 * TL::MOVES>((nrows - first + ROWS - 1) / ROWS, move, fetch, put, step);
+  const int n = (nrows - first + ROWS - 1) / ROWS;
+  stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step, std::false_type());
+  if constexpr (sizeof(T) == 4)
+    if (anywhere<NW>(finite_check(dk) + finite_check(dv), flags)) {
+#pragma unroll
+      for (int db = 0; db < DP / 32; ++db) dk[db] = dv[db] = zero16();
+      stream<FAST, NB, 2 * TL::MOVES>(n, move, fetch, put, step, std::true_type());
+    }
   if (!live) return;
   if (a.splits > 1) {
     const i64 at = ((i64)(s.k0 + key) * a.Hkv + kvh) * a.D, plane = (i64)a.total_k * a.Hkv * a.D;
