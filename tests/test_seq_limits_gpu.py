@@ -172,3 +172,51 @@ def test_infinities_in_split_sums(name):
     val["out"][:, 1::64] = float("inf")
     c.forward()
     check(c, val, bnd, ("out", "lse"))
+
+
+# ---- a few keys -----------------------------------------------------------------------------------------
+
+def grad_q_of_few_keys(c, most):
+    """grad_q in 64 bits and its bound for queries that see 1 to `most` keys, heads of up to 64 elements, bf16: what dS is made of
+    is fp32, delta included (a sum over the weights: not dout * out, whose out was rounded to bf16), and dS goes into its
+    product in two bf16 parts, off by half a step of the second, 2^-8 * 2^-8."""
+    U, d, g = seq_ref.U, c.d, c.hq // c.hk
+    q, k, v, do = (t.double().cpu().reshape(t.shape[0], -1, d) for t in (c.q, c.k, c.v, c.dout))
+    val, bnd, rows = torch.zeros(c.nq, c.hq, d).double(), torch.zeros(c.nq, c.hq, d).double(), torch.zeros(c.nq, dtype=torch.bool)
+    bq = bk = 0
+    for nq, nk in zip(c.lens_q, c.lens_k):
+        for i in range(nq):
+            n = min(nk, i + 1 + nk - nq) if c.causal else nk
+            if not 1 <= n <= most:
+                continue
+            rows[bq + i] = True
+            for h in range(c.hq):
+                qi, kj, vj, doi = q[bq + i, h], k[bk:bk + n, h // g], v[bk:bk + n, h // g], do[bq + i, h]
+                s = kj @ qi * c.scale
+                lse = torch.logsumexp(s, 0)
+                p, dp = torch.exp(s - lse), vj @ doi
+                ds = p * (dp - p @ dp)
+                # as in seq_ref.attention: a score's roundings, the exponent's, those of the sum behind lse
+                e_w = (d / 16 + 8) * U * c.scale * (kj.abs() @ qi.abs()) + 8 * U * (s.abs() + lse.abs() + 12)
+                e_p = e_w + p @ e_w + 65 * U + 8 * U * lse.abs()
+                e_dp = (d / 16 + 8) * U * (vj.abs() @ doi.abs())
+                e_delta = p @ (e_dp + dp.abs() * (e_p + 40 * U))
+                e_ds = p * (e_dp + e_delta) + ds.abs() * (e_p + 2.0 ** -16 + 4 * U)
+                val[bq + i, h] = ds @ kj * c.scale
+                bnd[bq + i, h] = c.scale * ((e_ds + 65 * U * ds.abs()) @ kj.abs()) + (seq_ref.half_step(c.dtype) + U) * val[bq + i, h].abs()
+        bq, bk = bq + nq, bk + nk
+    return val.reshape(c.nq, -1)[rows], bnd.reshape(c.nq, -1)[rows] + 1e-34, rows
+
+
+@pytest.mark.parametrize("dim", [20, 32, 64])
+@pytest.mark.parametrize("lens_q,lens_k,hq,hk,causal", [([50, 7], [32, 32], 6, 2, False), ([50, 7], [31, 1], 6, 2, False), ([40], [40], 32, 1, True),
+                                                        ([40, 33], [40, 60], 3, 3, True)])
+def test_grad_q_of_queries_that_see_up_to_32_keys(lens_q, lens_k, hq, hk, causal, dim):
+    """Keys with a large part in common: dS adds up to zero, so that part falls out of grad_q, but an error of delta does not."""
+    c = Call("bf16", lens_q, lens_k, hq, hk, dim, causal, spread=0.25)
+    c.k += 4.0
+    c.forward()
+    c.backward()
+    val, bnd, rows = grad_q_of_few_keys(c, 32)
+    assert rows.any()
+    seq_ref.check(c.dq[:c.nq][rows.to(DEV)], val, bnd, "dq")

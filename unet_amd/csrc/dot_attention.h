@@ -1037,15 +1037,15 @@ __global__ __launch_bounds__(256, (two_fit<T, DP, WK>() ? 2 : 1)) void attention
           s[i] = 8 * (i / 4) + i % 4 <= rel ? s[i] : 0.f;
           dp[i] = 8 * (i / 4) + i % 4 <= rel ? dp[i] : 0.f;
         }
-        if (kb == 0) {
-          // A query whose keys all lie here has its delta from the weights themselves: dout * out takes out as it was
-          // stored, rounded, and with few keys, where out is large, that would be the largest error of dS.
-          float d = 0.f;
+      }
+      if (kb == 0 && span.wave_all < 32) {  // (the first query sees the fewest keys)
+        // A query whose keys all lie here has its delta from the weights themselves: dout * out takes out as it was
+        // stored, rounded, and with few keys, where out is large, that would be the largest error of dS.
+        float d = 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) d += s[i] * dp[i];
-          d += __shfl_xor(d, 32, 64);
-          delta = r.lim < 32 ? d : delta;
-        }
+        for (int i = 0; i < 16; ++i) d += s[i] * dp[i];
+        d += __shfl_xor(d, 32, 64);
+        delta = r.lim < 32 ? d : delta;
       }
 #pragma unroll
       for (int i = 0; i < 16; ++i) s[i] *= dp[i] - delta;
