@@ -240,7 +240,8 @@ __global__ __launch_bounds__(256) void layer_norm_wgrad_kernel(const float *__re
   }
 }
 
-// Rows longer than the registers of a workgroup: one workgroup per row reads it once per pass.
+// Rows longer than the registers of a workgroup: one workgroup per row reads it once per pass.  A thread's share may be
+// hundreds of thousands of elements, so it is added up in double (the passes wait for memory).
 template <typename T>
 __global__ __launch_bounds__(256) void layer_norm_long_kernel(const FwdArgs<T> a) {
   __shared__ float red[8];
@@ -248,15 +249,17 @@ __global__ __launch_bounds__(256) void layer_norm_long_kernel(const FwdArgs<T> a
   for (i64 row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *x = a.x + row * a.x_ld;
     T *y = a.y + row * a.y_ld;
-    float s[1] = {0.f};
-    for (int c = threadIdx.x; c < a.C; c += 256) s[0] += to_f32(x[c]);
+    double t = 0.0;
+    for (int c = threadIdx.x; c < a.C; c += 256) t += (double)to_f32(x[c]);
+    float s[1] = {(float)t};
     group_sum<256, 1>(s, red, phase);
     const float mean = s[0] / (float)a.C;
-    s[0] = 0.f;
+    t = 0.0;
     for (int c = threadIdx.x; c < a.C; c += 256) {
-      const float d = to_f32(x[c]) - mean;
-      s[0] += d * d;
+      const double d = (double)(to_f32(x[c]) - mean);
+      t += d * d;
     }
+    s[0] = (float)t;
     group_sum<256, 1>(s, red, phase);
     const float rstd = 1.f / sqrtf(s[0] / (float)a.C + a.eps);
     if (a.stats && threadIdx.x == 0) {
@@ -276,12 +279,13 @@ __global__ __launch_bounds__(256) void layer_norm_long_dx_kernel(const BwdArgs<T
   for (i64 row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T *x = a.x + row * a.x_ld, *dy = a.dy + row * a.dy_ld;
     const float mean = a.stats[2 * row], rstd = a.stats[2 * row + 1];
-    float s[2] = {0.f, 0.f};
+    double t0 = 0.0, t1 = 0.0;
     for (int c = threadIdx.x; c < a.C; c += 256) {
       const float g = to_f32(dy[c]) * (a.w ? a.w[2 * (i64)c] : 1.f);
-      s[0] += g;
-      s[1] += g * ((to_f32(x[c]) - mean) * rstd);
+      t0 += (double)g;
+      t1 += (double)g * (double)((to_f32(x[c]) - mean) * rstd);
     }
+    float s[2] = {(float)t0, (float)t1};
     group_sum<256, 2>(s, red, phase);
     const float m0 = s[0] / (float)a.C, m1 = s[1] / (float)a.C;
     for (int c = threadIdx.x; c < a.C; c += 256) {
@@ -296,15 +300,15 @@ __global__ __launch_bounds__(256) void layer_norm_long_columns_kernel(const BwdA
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= a.C) return;
   const i64 r0 = blockIdx.y * rows_per, r1 = min(a.rows, r0 + rows_per);
-  float dga = 0.f, dbe = 0.f;
+  double dga = 0.0, dbe = 0.0;
   for (i64 r = r0; r < r1; ++r) {
-    const float dy = to_f32(a.dy[r * a.dy_ld + c]);
-    dga += dy * ((to_f32(a.x[r * a.x_ld + c]) - a.stats[2 * r]) * a.stats[2 * r + 1]);
+    const double dy = (double)to_f32(a.dy[r * a.dy_ld + c]);
+    dga += dy * (double)((to_f32(a.x[r * a.x_ld + c]) - a.stats[2 * r]) * a.stats[2 * r + 1]);
     dbe += dy;
   }
   float *out = a.partials + (i64)blockIdx.y * 2 * a.C + 2 * (i64)c;
-  out[0] = dga;
-  out[1] = dbe;
+  out[0] = (float)dga;
+  out[1] = (float)dbe;
 }
 
 // f(G, NV) with the lanes per row and 16-byte pieces per lane that hold a row of `pieces` pieces; false: too long.
