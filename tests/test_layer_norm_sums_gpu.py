@@ -62,3 +62,46 @@ def test_rows_of_millions_of_channels(c):
     size = rstd * (g.abs() + g.abs().mean(1, keepdim=True) + xhat.abs() * (g * xhat).abs().mean(1, keepdim=True))
     # the statistics that it was given are off by their own bounds: twice
     seq_ref.check(dx, want, 2 * (by_xhat + size * (rel + 24 * U)), "dx")
+
+
+@pytest.mark.parametrize("rows,c", [((1 << 25) + 5, 4), ((1 << 23) + 3, 100), (1 << 20, 260)])
+def test_columns_of_millions_of_rows(rows, c):
+    """All rows of a column hold the same x and dy.  A lane adds at most 256 rows (each a rounding of the sum, of the product and
+    of xhat behind the stored statistics), then 16 groups of a workgroup, at most 16 launches here, and 512 partial rows in double."""
+    g = torch.Generator().manual_seed(3)
+    one = torch.randn(1, c, generator=g).to(DEV)
+    x, stats, dw = one.expand(rows, c).contiguous(), empty((rows, 2)), empty((c, 2))
+    dy = torch.full_like(x, UNEVEN)
+    dy[:, 1] = -UNEVEN / 3
+    dx = empty((rows, c))
+    capi.unet_layer_norm_f32(x.data_ptr(), c, dx.data_ptr(), c, None, stats.data_ptr(), rows, c, 1e-5, stream())
+    assert torch.equal(stats, stats[:1].expand(rows, 2))
+    backward(dy, x, stats, None, dx, dw)
+    xhat = (one[0].double() - stats[0, 0].double()) * stats[0, 1].double()
+    want = torch.stack([dy[0].double() * xhat, dy[0].double()], 1) * rows
+    seq_ref.check(dw, want, (256 + 16 + 16 + 4) * U * want.abs(), "dweights")
+    assert torch.equal(dx, dx[:1].expand(rows, c))  # every launch's rows
+
+
+def test_rows_of_several_launches():
+    """Different rows, strides and a skip gradient: each launch begins at its own rows.  dx alone is one launch of the same rows."""
+    rows, c = 300001, 1100  # a workgroup holds a row; 131072 rows a launch
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    x, dy, skip = (torch.randn(rows, c + p, generator=gen, device=DEV)[:, :c] for p in (4, 0, 8))
+    w = torch.randn(c, 2, generator=gen, device=DEV)
+    stats, dx, alone, dw = empty((rows, 2)), empty((rows, c)), empty((rows, c)), empty((c, 2))
+    capi.unet_layer_norm_f32(x.data_ptr(), x.stride(0), dx.data_ptr(), c, w.data_ptr(), stats.data_ptr(), rows, c, 1e-5, stream())
+    n = ctypes.c_size_t()
+    capi.unet_layer_norm_backward_workspace_bytes(rows, c, ctypes.byref(n))
+    ws = torch.full((n.value + 4096,), 255, dtype=torch.uint8, device=DEV)
+    args = (dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), stats.data_ptr(), w.data_ptr(), skip.data_ptr(), skip.stride(0))
+    capi.unet_layer_norm_backward_f32(*args, dx.data_ptr(), c, dw.data_ptr(), rows, c, ws.data_ptr(), n.value, stream())
+    capi.unet_layer_norm_backward_f32(*args, alone.data_ptr(), c, None, rows, c, None, 0, stream())
+    assert torch.equal(dx, alone) and (ws[n.value:] == 255).all()
+    want, size = torch.zeros(c, 2, dtype=torch.float64, device=DEV), torch.zeros(c, 2, dtype=torch.float64, device=DEV)
+    for r in range(0, rows, 50000):
+        d = dy[r:r + 50000].double()
+        t = torch.stack([d * (x[r:r + 50000].double() - stats[r:r + 50000, :1].double()) * stats[r:r + 50000, 1:].double(), d], 2)
+        want += t.sum(0)
+        size += t.abs().sum(0)
+    seq_ref.check(dw, want, (256 + 16 + 4) * U * size, "dweights")

@@ -13,8 +13,10 @@
 // last-level cache), backward with the weight's gradient 83 us (4.9 TB/s, the rate of a large copy).
 //
 // The sums over rows (dgamma, dbeta) are kept per lane for the columns it owns, added up inside the workgroup in a
-// fixed order and written as one partial row [2C] per workgroup; a second launch adds the partial rows, in double
-// (it reads at most BWD_BLOCKS of them).  No atomics, so equal calls give equal bits.
+// fixed order and written as one partial row [2C] per workgroup; a last launch adds the partial rows, in double
+// (it reads at most BWD_BLOCKS of them).  More than CHAIN rows a group (131072 rows and more) are taken by several
+// launches, each adding to the partial rows, so that a sum over millions of rows is no chain of thousands.  No atomics,
+// so equal calls give equal bits.
 #include "rows_util.h"
 
 namespace {
@@ -22,6 +24,7 @@ namespace {
 constexpr int FWD_BLOCKS = 2048;  // at most 8 workgroups of 4 wavefronts per CU: all resident
 constexpr int BWD_BLOCKS = 512;   // 2 per CU: fewer partial rows for the second launch to read
 constexpr int MOST_CHANNELS = 1 << 26;  // the column sums' launch has 32 threads a channel, of fewer than 2^32
+constexpr int CHAIN = 256;        // rows of a group in one fp32 chain of the column sums
 constexpr int LONG_SPLITS = 64;   // row ranges of the column sums of rows that do not fit registers
 
 template <typename T>
@@ -42,6 +45,7 @@ struct BwdArgs {
   float *partials;  // [gridDim.x][2C], NULL: no weight gradient
   i64 dy_ld, x_ld, skip_ld, dx_ld, rows;
   int C;
+  bool add;  // to the partials, which earlier rows have left
 };
 
 // gamma (and beta) of the row's columns in LDS, in the order in which the lanes take them: value i of piece v of lane l at
@@ -208,8 +212,20 @@ __global__ __launch_bounds__(256) void layer_norm_backward_kernel(const BwdArgs<
           }
       __syncthreads();
     }
-    for (int c = threadIdx.x; c < 2 * a.C; c += 256) out[c] = sums[c];
+    if (a.add)
+      for (int c = threadIdx.x; c < 2 * a.C; c += 256) out[c] += sums[c];
+    else
+      for (int c = threadIdx.x; c < 2 * a.C; c += 256) out[c] = sums[c];
   } else {
+    if (a.add)
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int c = 2 * min((lane + v * G) * N + i, a.C - 1);
+          dga[v][i] += out[c];
+          dbe[v][i] += out[c + 1];
+        }
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
@@ -374,14 +390,23 @@ int layer_norm_backward(const T *dy, i64 dy_ld, const T *x, i64 x_ld, const floa
     UNET_REQUIRE(ws_bytes >= need && (ws || !need), "layer_norm_backward: workspace of %zu bytes, needs %zu", ws_bytes, need);
     UNET_REQUIRE(((uintptr_t)ws & 15) == 0, "layer_norm_backward: the workspace is not 16-byte aligned");
   }
-  BwdArgs<T> a{dy, x, skip, stats, w, dx, dw ? (float *)ws : nullptr, dy_ld, x_ld, skip_ld, dx_ld, rows, C};
+  BwdArgs<T> a{dy, x, skip, stats, w, dx, dw ? (float *)ws : nullptr, dy_ld, x_ld, skip_ld, dx_ld, rows, C, false};
   if (!dw && (!dx || rows == 0)) return UNET_OK;
   int n = 0;  // partial rows written
   if (rows > 0) {
     const bool held = with_row_shape(pieces_of<T>(C), [&](auto g, auto nv) {
-      const i64 blocks = (rows + 256 / g - 1) / (256 / g);
-      n = (int)(blocks < BWD_BLOCKS ? blocks : BWD_BLOCKS);
-      layer_norm_backward_kernel<T, decltype(g)::value, decltype(nv)::value><<<n, 256, 0, st>>>(a);
+      const i64 most = dw ? (i64)CHAIN * BWD_BLOCKS * (256 / g) : rows;
+      for (i64 done = 0; done < rows; done += most) {
+        BwdArgs<T> b = a;
+        b.dy += done * dy_ld, b.x += done * x_ld, b.stats += 2 * done, b.add = done > 0;
+        if (skip) b.skip += done * skip_ld;
+        if (dx) b.dx += done * dx_ld;
+        b.rows = rows - done < most ? rows - done : most;
+        const i64 blocks = (b.rows + 256 / g - 1) / (256 / g);
+        const int grid = (int)(blocks < BWD_BLOCKS ? blocks : BWD_BLOCKS);
+        if (!done) n = grid;
+        layer_norm_backward_kernel<T, decltype(g)::value, decltype(nv)::value><<<grid, 256, 0, st>>>(b);
+      }
     });
     if (!held) {
       if (dw) {  // before dx, which may overwrite what it reads
