@@ -747,7 +747,7 @@ __global__ __launch_bounds__(64 * NW, (two_fit<T, DP, WK>() && (sizeof(T) == 2 |
   constexpr int WQ = NW / WK, BQ = COLS * WQ, ROWS = sizeof(T) == 2 && WK == 1 ? 64 : tile_rows<T, DP, FAST, WK>();
   constexpr int NU = WK == 1 ? ROWS / 32 : 1, DB = DP / 32;
   typedef Tile<T, DP, ROWS, NW> TL;
-  constexpr int NB = NW == 8 ? (FAST ? 3 : 2) : buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 64 * NW * (DB * 16 + 2) * 4;
+  constexpr int NB = NW == 8 ? 2 : buffers<T, DP, FAST, WK>(), STAGE = 2 * TL::BYTES, MERGE = WK == 1 ? 0 : 64 * NW * (DB * 16 + 2) * 4;
   __shared__ __align__(16) unsigned char lds[(NB * STAGE > MERGE ? NB * STAGE : MERGE) + TL::ZEROS];
   __shared__ int flags[sizeof(T) == 4 ? NW : 1];
   unsigned char *const zeros = lds + sizeof(lds) - TL::ZEROS;
@@ -1383,15 +1383,14 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 // and for rows through registers
 // (what a join costs more would not be won back; fp32, 4 queries over 12000 keys, 16/4 heads of 128: 59 us with 512, 37
 // with 256, but one image of 256 tokens 11.7 whole and 13.2 in two).
-// wide: 8 wavefronts and 256 queries a workgroup (forward, bf16 rows of 96 elements and more): half the direct loads, and
-// room for a third buffer; 8192 tokens, 16/4 heads of 128, causal: 293 -> 275 us.  (dQ gains nothing by it: its two
-// score products take twice as long per tile.)  fp32 with 64 elements and wk = 2 takes 8 wavefronts, 128 queries, too: the
-// tiles are split into parts by twice as many threads (3525 tokens, 8 heads: 57 -> 46 us; dQ gains nothing).
+// fp32 with 64 elements and wk = 2 takes 8 wavefronts, 128 queries: the
+// tiles are split into parts by twice as many threads (3525 tokens, 8 heads: 57 -> 46 us; dQ gains nothing).  (bf16 rows of 96
+// elements and more gain by 8 wavefronts and 256 queries only where the workgroups come out as whole rounds of the GPU: 8192
+// tokens, 16/4 heads of 128, causal, 294 -> 273 us; one sequence of 5000, 32 heads, 218 -> 231; 25 of 256, 16 heads, 33 -> 63.)
 // dq_splits: the same for dQ, 256 keys at least in both types, at most 8 (backward in us: 3000 tokens, 2/1 heads of 128, fp32
 // 463 whole, 344 in two; 976 tokens, 2 heads of 100, bf16 99 whole, 68 in three).
 struct Plan {
   int wk, splits, dq_splits, tiles;  // tiles of queries: an upper bound
-  bool wide;
 };
 template <typename T>
 constexpr int most_shared(int DP) { return sizeof(T) == 2 || DP <= 64 ? 4 : 2; }  // what the LDS has room for
@@ -1407,7 +1406,6 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
   const i64 n = groups(BM);
   p.wk = n >= places * (causal ? 6 : 3) / 4 ? 1 : n > places / 4 ? 2 : 4;
   if (p.wk > most) p.wk = most;
-  p.wide = p.wk == 1 && groups(2 * BM) >= 384;
   auto shares = [&](i64 keys, i64 limit) {
     if (p.wk != most || num_seqs == 0) return 1;
     i64 s = 256 / groups(BM / p.wk);
@@ -1519,12 +1517,6 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
   with_dim<T>(D, whole, [&](auto dp, auto fast) {
     constexpr int DP = decltype(dp)::value;
     constexpr bool FAST = decltype(fast)::value;
-    if constexpr (FAST && sizeof(T) == 2 && DP >= 96)
-      if (plan.wide) {
-        a.tiles = (int)(total_q * (Hq / Hkv) / (2 * BM)) + num_seqs;
-        attention_kernel<T, DP, FAST, 1, 8><<<(unsigned)a.tiles * Hkv, 512, 0, st>>>(a);
-        return;
-      }
     with_shared<T, DP, FAST>(plan.wk, [&](auto wk) {
       constexpr int WK = decltype(wk)::value, NW = sizeof(T) == 4 && DP == 64 && WK == 2 ? 8 : WAVES;  // see Plan
       if (NW == 8) a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
