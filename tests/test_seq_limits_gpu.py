@@ -69,7 +69,7 @@ def test_values_near_the_largest_number(name, lens_q, lens_k, hq, hk, d, pad):
 # ---- infinities that a query sees -----------------------------------------------------------------------
 # Both types treat them as the definition does: a score of -inf is a weight of 0, an infinite value makes an infinite output.
 
-VISIBLE = [(4, 20), (60, 30), (130, 32), (4, 60), (60, 64), (130, 50), (4, 96), (66, 88), (4, 128), (66, 120)]  # heads, dim: each kernel of fp32
+VISIBLE = [(4, 20), (60, 30), (130, 32), (4, 60), (60, 64), (80, 50), (130, 50), (4, 96), (66, 88), (4, 128), (66, 120)]  # heads, dim: each kernel of fp32
 LENS_Q, LENS_K = [333, 40], [340, 33]
 
 
@@ -220,3 +220,14 @@ def test_grad_q_of_queries_that_see_up_to_32_keys(lens_q, lens_k, hq, hk, causal
     val, bnd, rows = grad_q_of_few_keys(c, 32)
     assert rows.any()
     seq_ref.check(c.dq[:c.nq][rows.to(DEV)], val, bnd, "dq")
+
+
+# ---- each way to share the queries of fp32's 33 to 64 elements -------------------------------------------
+
+@pytest.mark.parametrize("lens,hq,hk,dim,causal", [([128] * 12, 12, 12, 64, False), ([384] * 7, 8, 8, 48, True), ([300, 20], 60, 60, 40, False),
+                                                   ([700], 32, 32, 64, True), ([65] * 9, 30, 30, 33, True)])
+def test_fp32_of_up_to_64_elements(lens, hq, hk, dim, causal):
+    c = Call("f32", lens, lens, hq, hk, dim, causal, behind=2)
+    c.forward()
+    c.backward()
+    c.verify()

@@ -1383,14 +1383,18 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 // and for rows through registers
 // (what a join costs more would not be won back; fp32, 4 queries over 12000 keys, 16/4 heads of 128: 59 us with 512, 37
 // with 256, but one image of 256 tokens 11.7 whole and 13.2 in two).
-// fp32 with 64 elements and wk = 2 takes 8 wavefronts, 128 queries: the
-// tiles are split into parts by twice as many threads (3525 tokens, 8 heads: 57 -> 46 us; dQ gains nothing).  (bf16 rows of 96
+// eight: 8 wavefronts and 128 queries a workgroup, one a CU (forward, fp32 rows of 33 to 64 elements, wk = 2): the tiles are
+// split into parts by twice as many threads.  Where one round of workgroups does, or a single sequence leaves no empty
+// workgroups among them; else a few CUs take two in a row.  us with 4 / 8 wavefronts, 8 heads of 64: 3525 tokens in 4 sequences
+// 56 / 46; one of 5000 422 / 407, causal 204 / 198; 3 of 1024 60 / 49; but 16 of 256 25 / 37, 17 of 384, causal, 40 / 66, 4/2 heads,
+// 2 of 4086, 223 / 309.  (dQ gains nothing by it.)  (bf16 rows of 96
 // elements and more gain by 8 wavefronts and 256 queries only where the workgroups come out as whole rounds of the GPU: 8192
 // tokens, 16/4 heads of 128, causal, 294 -> 273 us; one sequence of 5000, 32 heads, 218 -> 231; 25 of 256, 16 heads, 33 -> 63.)
 // dq_splits: the same for dQ, 256 keys at least in both types, at most 8 (backward in us: 3000 tokens, 2/1 heads of 128, fp32
 // 463 whole, 344 in two; 976 tokens, 2 heads of 100, bf16 99 whole, 68 in three).
 struct Plan {
   int wk, splits, dq_splits, tiles;  // tiles of queries: an upper bound
+  bool eight;
 };
 template <typename T>
 constexpr int most_shared(int DP) { return sizeof(T) == 2 || DP <= 64 ? 4 : 2; }  // what the LDS has room for
@@ -1406,6 +1410,7 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
   const i64 n = groups(BM);
   p.wk = n >= places * (causal ? 6 : 3) / 4 ? 1 : n > places / 4 ? 2 : 4;
   if (p.wk > most) p.wk = most;
+  p.eight = sizeof(T) == 4 && p.wk == 2 && D > 32 && D <= 64 && (num_seqs == 1 || (rows / BM + num_seqs) * Hkv <= 256);
   auto shares = [&](i64 keys, i64 limit) {
     if (p.wk != most || num_seqs == 0) return 1;
     i64 s = 256 / groups(BM / p.wk);
@@ -1518,9 +1523,14 @@ int forward(const T *q, i64 q_ld, const T *k, i64 k_ld, const T *v, i64 v_ld, T 
     constexpr int DP = decltype(dp)::value;
     constexpr bool FAST = decltype(fast)::value;
     with_shared<T, DP, FAST>(plan.wk, [&](auto wk) {
-      constexpr int WK = decltype(wk)::value, NW = sizeof(T) == 4 && DP == 64 && WK == 2 ? 8 : WAVES;  // see Plan
-      if (NW == 8) a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
-      attention_kernel<T, DP, FAST, WK, NW><<<(unsigned)a.tiles * Hkv * a.splits, 64 * NW, 0, st>>>(a);
+      constexpr int WK = decltype(wk)::value;
+      if constexpr (sizeof(T) == 4 && DP == 64 && WK == 2)
+        if (plan.eight) {
+          a.tiles = (int)(total_q * (Hq / Hkv) / BM) + num_seqs;
+          attention_kernel<T, DP, FAST, WK, 8><<<(unsigned)a.tiles * Hkv, 512, 0, st>>>(a);
+          return;
+        }
+      attention_kernel<T, DP, FAST, WK><<<(unsigned)a.tiles * Hkv * a.splits, 256, 0, st>>>(a);
     });
   });
   if (a.splits > 1) attention_join_kernel<T><<<cdiv_u(total_q * Hq, WAVES), 256, 0, st>>>(a);
