@@ -1423,11 +1423,13 @@ Plan make_plan(int num_seqs, i64 total_q, i64 total_k, int Hq, int Hkv, int D, b
   return p;
 }
 
-// Wavefronts of a dK/dV workgroup.  bf16 rows of 96 elements and more: 8 wavefronts, 256 keys, share a tile of queries,
-// because two workgroups of 4 would ask for 16 bytes of direct loads per clock and CU, which is all there is (8192
-// tokens, 16/4 heads of 128, causal: 805 us with 4, 600 with 8).
+// Wavefronts of a dK/dV workgroup.  bf16 rows of more than 96 elements: 8 wavefronts, 256 keys, share a tile of queries,
+// because two workgroups of 4 would ask for 16 bytes of direct loads per clock and CU, which is all there is (forward and
+// backward in us with 4 / 8, heads of 128: 8192 tokens, 16/4 heads, causal, 1807 / 1305; 8 of 512, 8 heads, 122 / 103; but 50 of 256, 16
+// heads, 333 / 362).  Up to 96 elements they ask for less, and 128 keys leave less of a short sequence's last tile empty (heads
+// of 96: 8192 tokens 1059 / 1057; 4 of 1024, 8 heads, 116 / 116; 16 of 256, 16 heads, 74 / 93; one of 256, 8 heads, 33 / 38).
 template <typename T>
-constexpr int dkv_waves(int DP) { return sizeof(T) == 2 && DP >= 96 ? 8 : WAVES; }
+constexpr int dkv_waves(int DP) { return sizeof(T) == 2 && DP >= 128 ? 8 : WAVES; }
 // Row ranges into which their sums are split when there are few key tiles: `fit` workgroups run at once (one of 8
 // wavefronts a CU, one of fp32 behind 64 elements, else two), and where lengths differ as much as under a causal mask it
 // takes twice as many to fill the GPU evenly, but 16 ranges only where 8 leave it empty (3 sequences, 3464 tokens, 8/1
