@@ -200,7 +200,8 @@ int unet_batch_norm_relu_backward_f32(const float *grad_activations, const float
  *   mean = sum_c x / C, rstd = 1 / sqrt(sum_c (x - mean)^2 / C + eps)
  *   activations = gamma * (x - mean) * rstd + beta
  * row_stats (may be NULL: inference) receives [mean, rstd] per row for the backward.  Statistics are fp32 from two
- * passes over the values; one rounding to the storage type at the end.  activations may be the inputs' own buffer
+ * passes over the values (so (x - mean)^2 has to fit fp32: magnitudes up to about 2^60); one rounding to the storage type at
+ * the end.  activations may be the inputs' own buffer
  * (same pointer, same stride).  rows = 0 is a valid empty call.  At most 2^26 channels. */
 int unet_layer_norm_f32(const float *inputs, int64_t in_ld, float *activations, int64_t out_ld, const float *weights,
                         float *row_stats, int64_t rows, int channels, float eps, unet_stream_t stream);
@@ -367,7 +368,8 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  * its products take operands apart).  Rows of out and lse in front of the first or
  * behind the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
  * accumulators are fp32; no finite value of v overflows on the way (one within 2^-16 of the largest number may be rounded over
- * it at the end), and values below about 2^-126 * 2^8 * keys lose bits.  The bf16 form rounds the softmax weights to bf16 for
+ * it at the end), and values below about 2^-126 * 2^8 * keys lose bits.  The fp32 form's products leave out less than 2^-21 of
+ * each term (2^-25 on the average; fp32's own rounding is 2^-24).  The bf16 form rounds the softmax weights to bf16 for
  * their product with V.  Equal calls give equal bits.  out must not overlap q, k or v.  total_q * heads_q and
  * total_k * heads_kv may be up to about 2^29.
  * heads_q * head_dim is less than 2^31.

@@ -22,15 +22,16 @@
 // spread over all banks.
 //
 // What bounds it, measured:
-//   - long sequences: the matrix cores.  8192 tokens, 16/4 heads of 128, causal, bf16: forward 270 us (1.0 PFLOP/s of the
-//     visible pairs), dQ 390, dK/dV 560-590, their join 23 (0.69 PFLOP/s on five products of two kernels that compute
-//     seven; a large library product reaches 1.26).
-//   - short ones: the latency of a few tiles.  16 x 256 tokens, 16 heads of 64, bf16: forward 13 us, dQ 20.5, dK/dV 21 for
+//   - long sequences: the matrix cores.  8192 tokens, 16/4 heads of 128, causal, bf16: forward 315 us (0.87 PFLOP/s of the
+//     visible pairs), dQ 421, dK/dV 594, their join 23.5 (0.66 PFLOP/s on five products of two kernels that compute
+//     seven; a large library product reaches 1.24).
+//   - short ones: the latency of a few tiles.  16 x 256 tokens, 16 heads of 64, bf16: forward 13 us, dQ 21, dK/dV 20 for
 //     34 to 50 MB each.
-//   - few queries: HBM.  4 queries over 53386 keys, 32/4 heads of 128, bf16: 20 us (5.5 TB/s) and 4 for the join.
+//   - few queries: HBM.  4 queries over 53386 keys, 32/4 heads of 128, bf16: 22 us (5.0 TB/s) and 4 for the join.
 //   - fp32: the matrix cores and, beside them, the vector instructions that split operands into parts.  3525 tokens in 4
-//     sequences, 8 heads of 64: forward 46 us, dQ 77, dK/dV 90, their join 10 (144, 129 and 147 TFLOP/s of the products that
-//     they compute; a large library product in fp32 reaches 154); one of 8192 tokens 702 us (196 TFLOP/s).
+//     sequences, 8 heads of 64: forward 51 us, dQ 77, dK/dV 94, their join 10 (130, 129 and 141 TFLOP/s of the products that
+//     they compute; a large library product in fp32 reaches 154); forward of one of 8192 tokens 731 us (188 TFLOP/s).
+// (Medians of 20 calls in a kernel trace; cards differ by up to 5 %.)
 #include <math.h>
 
 #include "rows_util.h"
@@ -53,10 +54,11 @@ constexpr unsigned NOWHERE = 0x80000000u;  // a byte offset behind the end of ev
 // Eight elements of a matrix operand.  An fp32 number is the sum of three bf16 numbers: its upper 16 bits, what they leave
 // over (less than 2^-7 of it) rounded to bf16, and the rest, which has 8 bits and is at most 2^-15 of it.  Six products
 // of parts make the product of two such numbers up to 2^-21 of it: what is left out is the middle part of one times the
-// last part of the other, twice, with random signs; the matrix cores do the six in 3/8 of the time of one fp32 product.
+// last part of the other, twice, with random signs (2^-25 on the average); the matrix cores do the six in 3/8 of the time of one
+// fp32 product.
 // (The upper part is cut off, not rounded: no finite number becomes infinite.  An infinity leaves NaN over, see below.)  3525
-// tokens in 4 sequences, 8 heads of 64, forward and backward: 219 us and an error of 5.3e-7 of the result; with fp32
-// matrix instructions 366 us and 7.0e-7.
+// tokens in 4 sequences, 8 heads of 64, forward and backward: 225 us, with fp32 matrix instructions 366; errors 5.3e-7 and 7.0e-7 of
+// the result on the same inputs.
 struct Parts {
   bf16x8 p[3];
 };
@@ -547,7 +549,8 @@ __device__ __forceinline__ bool rows_of(const Args<T> &a, int tile, int kvh, int
 // rows of 192 bytes and more
 //   - that go through registers: a thread then holds 16 of them for the tile that is on its way, and with 64 rows the
 //     kernels with two streamed matrices and 64 or 128 accumulators spill;
-//   - in fp32, whose tiles are three times as large.
+//   - in fp32, whose tiles are three times as large.  (With 128 elements dQ and dK/dV spill registers all the same: dQ 5
+//     and, for WK = 2, 25, nearly all outside the loop over finite tiles; dK/dV 54, some of them inside.)
 template <typename T, int DP, bool FAST, int WK>
 constexpr int tile_rows() {
   return WK > 1 ? 32 * WK : DP * sizeof(T) >= 192 && !FAST ? 32 : 64;

@@ -9,8 +9,8 @@
 // to 1024; longer rows are read again by the *_long kernels), which takes the statistics from the registers in two
 // passes (mean, then squared deviations: no cancellation).  Groups walk over rows, gamma and beta stay on the CU
 // across rows (in LDS: in registers they would cost half of the wavefronts), and the next row is requested before the
-// current one is worked on.  65536 rows of 1024 bf16 channels: forward 44 us (6.1 TB/s; both tensors just fit the
-// last-level cache), backward with the weight's gradient 83 us (4.9 TB/s, the rate of a large copy).
+// current one is worked on.  65536 rows of 1024 bf16 channels: forward 47 us (5.7 TB/s; both tensors just fit the
+// last-level cache), backward 77 us and 5 for the partial rows of the weight's gradient (4.9 TB/s, the rate of a large copy).
 //
 // The sums over rows (dgamma, dbeta) are kept per lane for the columns it owns, added up inside the workgroup in a
 // fixed order and written as one partial row [2C] per workgroup; a last launch adds the partial rows, in double
@@ -21,7 +21,8 @@
 
 namespace {
 
-constexpr int FWD_BLOCKS = 2048;  // at most 8 workgroups of 4 wavefronts per CU: all resident
+constexpr int FWD_BLOCKS = 2048;  // 8 workgroups of 4 wavefronts per CU: all resident for rows of up to 192 pieces; of longer
+                                  // rows 6 to 2, whose gamma and beta take up to 64 KB of LDS
 constexpr int BWD_BLOCKS = 512;   // 2 per CU: fewer partial rows for the second launch to read
 constexpr int MOST_CHANNELS = 1 << 26;  // the column sums' launch has 32 threads a channel, of fewer than 2^32
 constexpr int CHAIN = 256;        // rows of a group in one fp32 chain of the column sums
