@@ -201,8 +201,8 @@ int unet_batch_norm_relu_backward_f32(const float *grad_activations, const float
  *   activations = gamma * (x - mean) * rstd + beta
  * row_stats (may be NULL: inference) receives [mean, rstd] per row for the backward.  Statistics are fp32 from two
  * passes over the values (so (x - mean)^2 has to fit fp32: magnitudes up to about 2^60); one rounding to the storage type at
- * the end.  activations may be the inputs' own buffer
- * (same pointer, same stride).  rows = 0 is a valid empty call.  At most 2^26 channels. */
+ * the end.  activations may be the inputs' own buffer (same pointer, same stride).  rows = 0 is a valid empty call.  At most
+ * 2^26 channels. */
 int unet_layer_norm_f32(const float *inputs, int64_t in_ld, float *activations, int64_t out_ld, const float *weights,
                         float *row_stats, int64_t rows, int channels, float eps, unet_stream_t stream);
 int unet_layer_norm_bf16(const uint16_t *inputs, int64_t in_ld, uint16_t *activations, int64_t out_ld,
@@ -364,15 +364,14 @@ int unet_attention_backward_bf16(const uint16_t *dy, int dy_ld, const uint16_t *
  *   lse [total_q][heads_q] (fp32, may be NULL: inference) = log sum_j exp(scale * q.k_j), for the backward.
  * A query that sees no key gets out = 0 and lse = -inf, and adds nothing to any gradient.  What a query does not see
  * does not reach it, whatever it holds (NaN and infinities included).  What it does see acts as in the formula: a score of
- * -inf is a weight of 0, an infinite value an infinite output (fp32 takes several times as long where there are any, since
- * its products take operands apart).  Rows of out and lse in front of the first or
+ * -inf is a weight of 0, one of +inf makes out and lse NaN, an infinite value an infinite output (fp32 takes several times as
+ * long where there are any, since its products take operands apart).  Rows of out and lse in front of the first or
  * behind the last sequence are left as they were.  1 <= head_dim <= 128, scale > 0.  Sums, softmax statistics and products'
  * accumulators are fp32; no finite value of v overflows on the way (one within 2^-16 of the largest number may be rounded over
  * it at the end), and values below about 2^-126 * 2^8 * keys lose bits.  The fp32 form's products leave out less than 2^-21 of
  * each term (2^-25 on the average; fp32's own rounding is 2^-24).  The bf16 form rounds the softmax weights to bf16 for
  * their product with V.  Equal calls give equal bits.  out must not overlap q, k or v.  total_q * heads_q and
- * total_k * heads_kv may be up to about 2^29.
- * heads_q * head_dim is less than 2^31.
+ * total_k * heads_kv may be up to about 2^29; heads_q * head_dim is less than 2^31.
  * `workspace`: device memory of at least unet_dot_attention_workspace_bytes() bytes (which may be 0: then NULL will
  * do), 16-byte aligned, free for other use once the call's work on `stream` has finished; calls that may run at the
  * same time need one each.  That size does for every call with the same heads and head_dim, no more queries and no more
