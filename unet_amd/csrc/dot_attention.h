@@ -1389,10 +1389,10 @@ int common_args(const char *name, Args<T> &a, const T *q, i64 q_ld, const T *k, 
 // eight: 8 wavefronts and 128 queries a workgroup, one a CU (forward, fp32 rows of 33 to 64 elements, wk = 2): the tiles are
 // split into parts by twice as many threads.  Where one round of workgroups does, or a single sequence leaves no empty
 // workgroups among them; else a few CUs take two in a row.  us with 4 / 8 wavefronts, 8 heads of 64: 3525 tokens in 4 sequences
-// 56 / 46; one of 5000 422 / 407, causal 204 / 198; 3 of 1024 60 / 49; but 16 of 256 25 / 37, 17 of 384, causal, 40 / 66, 4/2 heads,
-// 2 of 4086, 223 / 309.  (dQ gains nothing by it.)  (bf16 rows of 96
-// elements and more gain by 8 wavefronts and 256 queries only where the workgroups come out as whole rounds of the GPU: 8192
-// tokens, 16/4 heads of 128, causal, 294 -> 273 us; one sequence of 5000, 32 heads, 218 -> 231; 25 of 256, 16 heads, 33 -> 63.)
+// 67 / 56; one of 5000 422 / 407, causal 204 / 198; 3 of 1024 60 / 49; but 16 of 256 25 / 37, 17 of 384, causal, 40 / 66, 4/2
+// heads, 2 of 4086, 223 / 309.  (dQ gains nothing by it.  bf16 rows of 96 elements and more gain by 8 wavefronts and 256 queries
+// only where the workgroups come out as whole rounds of the GPU: 8192 tokens, 16/4 heads of 128, causal, 294 -> 273 us; one
+// sequence of 5000, 32 heads, 218 -> 231; 25 of 256, 16 heads, 33 -> 63.)
 // dq_splits: the same for dQ, 256 keys at least in both types, at most 8 (backward in us: 3000 tokens, 2/1 heads of 128, fp32
 // 463 whole, 344 in two; 976 tokens, 2 heads of 100, bf16 99 whole, 68 in three).
 struct Plan {
